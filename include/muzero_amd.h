@@ -570,6 +570,56 @@ int mz_bn_relu_train_bwd_acc(const void* x, const void* dy, const void* y, const
                              void* dresidual, float* dgamma, float* dbeta, int32_t accumulate, void* workspace,
                              int64_t workspace_bytes, mz_stream_t stream);
 
+/* ------------------------------------------------------------------ *
+ * Training-block operators: layer norm, the gated feed-forward projection and dropout, for trunks and heads built from
+ * residual feed-forward blocks next to the BatchNorm blocks above.  The reference has no counterpart.  Tensors are
+ * matrices of rows (every dimension but the last) with elements of one type:
+ * ------------------------------------------------------------------ */
+#define MZ_F32 0
+#define MZ_BF16 1
+#define MZ_F16 2
+
+/* Layer norm over the last dimension: y = (x - mean) * rstd * weight + bias per row, rstd = 1 / sqrt(var + eps), the
+ * biased variance, sums in float32.  x: [rows] rows of C elements of `dtype`, ldx elements apart (ldx >= C); y
+ * contiguous.  weight, bias (either may be NULL: 1 and 0): [C] of affine_dtype, which is MZ_F32 or dtype.  mean, rstd:
+ * float [rows] for the backward pass, or both NULL.  No alignment beyond the elements' is needed.
+ * Backward: from dy (rows lddy apart) dx (contiguous), dweight and dbias ([C] of affine_dtype); any of the three may
+ * be NULL.  workspace (for dweight / dbias): mz_layer_norm_workspace_bytes(rows, C) bytes.  No atomics. */
+int mz_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, int32_t affine_dtype, double eps,
+                      int64_t rows, int32_t C, int32_t dtype, void* y, float* mean, float* rstd, mz_stream_t stream);
+int64_t mz_layer_norm_workspace_bytes(int64_t rows, int32_t C);
+int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const void* weight, int32_t affine_dtype,
+                      const float* mean, const float* rstd, int64_t rows, int32_t C, int32_t dtype, void* dx, void* dweight,
+                      void* dbias, void* workspace, int64_t workspace_bytes, mz_stream_t stream);
+
+/* Gated feed-forward projection in one kernel: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up).  x: [M] rows of K
+ * elements, ldx apart; w_gate, w_up: [F][K]; b_gate, b_up: [F] or NULL; h: [M][F]; all of `dtype`, float32
+ * accumulation.  activation: 0 SiLU, 1 GELU (erf), 2 ReLU, 3 sigmoid.  K, F up to 2^20.  Where K is a whole number of
+ * 16-byte units, x, w_gate, w_up and the rows of x start on 16 bytes; other K have no such condition (the operands are
+ * copied to padded rows in the workspace).  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which may
+ * be 0 (then NULL will do).
+ * Backward: recomputes both products; dh [M][F] -> dx [M][K], dw_gate / dw_up [F][K] (both or neither), db_gate / db_up
+ * [F]; NULL for what is not wanted.  The gradients of the two products are rounded to `dtype` between the launches.
+ * workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 1) bytes, 16-byte aligned.  No atomics. */
+int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward);
+int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                    int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation, void* h, void* workspace,
+                    int64_t workspace_bytes, mz_stream_t stream);
+int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                    const void* dh, int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation, void* dx,
+                    void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace, int64_t workspace_bytes,
+                    mz_stream_t stream);
+
+/* Dropout with a counter-based generator: y = [residual +] (keep ? x / (1 - p') : 0) for n contiguous elements of
+ * `dtype`; p' = p rounded to a multiple of 2^-16.  Element e is kept when 16 bits of Philox4x32-10 (key = rng[0],
+ * counter = (e / 8, call, low and high half of rng[1]); bits 16 * (e % 2) .. of word (e % 8) / 2) are at least
+ * 65536 p'.  rng: int64 [2] in device memory (seed, offset), read when the kernel runs - a captured graph draws a new
+ * mask when the program has changed them.  `call` tells the calls of one step apart.  The mask is not stored: the
+ * gradient is the same call on dy without residual.  Dropped elements are zero whatever x holds.  residual or y may be
+ * x itself.  n <= 2^35. */
+int mz_dropout(const void* x, const void* residual, void* y, int64_t n, double p, const int64_t* rng, uint32_t call,
+               int32_t dtype, mz_stream_t stream);
+
 /* ReplayBuffer.sample_batch's draw (model.py:580-588) on device-resident priorities: double prio [n], one per
  * stored position, oldest game first.  u: double [batch], the [0,1) draws np.random.choice would consume.
  * Outputs: flat int32 [batch] = #(cdf <= u) with cdf the normalised cumulative sum of prio / sum(prio)

@@ -1,0 +1,546 @@
+// The gated feed-forward operator's matrix products (gated_ff.hip has the entry points and the mathematics):
+//
+//   kForward   h  = act(x Wg^T + bg) * (x Wu^T + bu)                       out[token][feature]
+//   kGateGrad  dg = dh u act'(g), du = dh act(g), g and u recomputed        out[token][feature], twice
+//   kInputGrad dx = dg Wg + du Wu                                           out[token][column]
+//   kWeightGrad dWg = dg^T x, dWu = du^T x                                  out[feature][column]
+//
+// All are D[r][c] = sum_k R(r, k) C(c, k) with the operand whose index runs fastest in the output as R: the matrix
+// instruction gives a lane four consecutive r of one c, an 8- or 16-byte store.  What differs is which of an operand's
+// two indices is contiguous in memory - k ("along", staged [row][128 bytes of k]) or the other one ("across", staged
+// [k][row]); 16-bit operands staged across are read with the transposing LDS read (ds_read_b64_tr_b16).
+//
+// A workgroup computes a BR x BC tile, its wavefronts split it WR x WC.  Per step 128 bytes of k (64 16-bit values, 32
+// float32) of both operands go to one of two LDS buffers; the next step's travel in registers meanwhile, loaded through
+// a buffer descriptor that returns zeros for what lies outside the matrix (ragged edges cost a compare, no branch).
+// One barrier a step.
+#pragma once
+#include "block_common.h"
+
+namespace mz_gff {
+
+enum Mode { kForward = 0, kGateGrad = 1, kInputGrad = 2, kWeightGrad = 3 };
+enum Activation { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
+
+struct Args {
+  // operands: one matrix for gate and one for up where there are two, the same twice where there is one
+  const void* r[2];
+  const void* c[2];
+  long ldr, ldc;             // elements between rows of the matrices as they lie in memory
+  long nr, nc, nk;           // extents of r (kForward / kGateGrad: features), c and k
+  void* out[2];
+  long ldo;
+  const void* bias[2];
+  const void* dh;            // kGateGrad: [nc][nr]
+  long lddh;
+  float* col_partial;        // kGateGrad, optional: [tiles of c][2][nr] sums of dg and du over the tile's tokens
+  float* partial;            // kInputGrad / kWeightGrad with splits > 1: [splits][problems][nc][nr]
+  long nr_pad;               // kGateGrad: columns of out, nr rounded up to whole 16-byte units, written with zeros
+  int activation, splits, steps_per_split;
+};
+
+// launchers, one translation unit per element type; tile: 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 64
+int launch_bf16(const Args& a, int mode, int tile, hipStream_t s);
+int launch_f16(const Args& a, int mode, int tile, hipStream_t s);
+int launch_f32(const Args& a, int mode, int tile, hipStream_t s);
+// x in at most 64 rows: out = forward
+int launch_few_bf16(const Args& a, hipStream_t s);
+int launch_few_f16(const Args& a, hipStream_t s);
+int launch_few_f32(const Args& a, hipStream_t s);
+
+constexpr int tile_side(int tile) { return tile == 0 ? 256 : tile == 1 ? 128 : 64; }
+
+}  // namespace mz_gff
+
+#ifdef MZ_GFF_KERNELS
+namespace {
+
+using mz_gff::Args;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+template <typename T> using vec4 = T __attribute__((ext_vector_type(4)));
+template <typename T> using vec8 = T __attribute__((ext_vector_type(8)));
+
+// D += R C over the k that a lane's 16 bytes of each operand hold: 32 values of k a matrix instruction for the 16-bit
+// types; float32 takes four instructions of 4, k = 4 (lane / 16) + j in the j-th - the same k for both operands, which
+// is all that matters.
+__device__ __forceinline__ f32x4 mma(u32x4 r, u32x4 c, f32x4 d, __bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(vec8<__bf16>, r), __builtin_bit_cast(vec8<__bf16>, c), d, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(u32x4 r, u32x4 c, f32x4 d, _Float16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vec8<_Float16>, r), __builtin_bit_cast(vec8<_Float16>, c), d, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(u32x4 r, u32x4 c, f32x4 d, float) {
+  const f32x4 a = __builtin_bit_cast(f32x4, r), b = __builtin_bit_cast(f32x4, c);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) d = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], d, 0, 0, 0);
+  return d;
+}
+
+// exp and reciprocal of the 16-bit types' activations: the hardware's, good to float32's last bits near zero and to
+// 2^-17 relative at |x| = 80 - far below the 2^-9 / 2^-12 rounding of the result.  float32 results take the library's.
+template <typename T> __device__ __forceinline__ float act_exp(float v) { return __expf(v); }
+template <> __device__ __forceinline__ float act_exp<float>(float v) { return expf(v); }
+template <typename T> __device__ __forceinline__ float act_rcp(float v) { return __builtin_amdgcn_rcpf(v); }
+template <> __device__ __forceinline__ float act_rcp<float>(float v) { return 1.f / v; }
+
+template <typename T> __device__ __forceinline__ float activate(int kind, float g) {
+  if (kind == mz_gff::kRelu) return g < 0.f ? 0.f : g;      // a NaN stays one
+  if (kind == mz_gff::kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  const float sig = act_rcp<T>(1.f + act_exp<T>(-g));
+  return kind == mz_gff::kSilu ? g * sig : sig;
+}
+// act(g) and act'(g)
+template <typename T> __device__ __forceinline__ void activate_grad(int kind, float g, float& act, float& slope) {
+  if (kind == mz_gff::kRelu) {
+    act = g < 0.f ? 0.f : g;
+    slope = g > 0.f ? 1.f : 0.f;
+  } else if (kind == mz_gff::kGelu) {
+    const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
+    act = g * cdf;
+    slope = cdf + g * act_exp<T>(-0.5f * g * g) * 0.39894228040143268f;
+  } else {
+    const float sig = act_rcp<T>(1.f + act_exp<T>(-g));
+    act = kind == mz_gff::kSilu ? g * sig : sig;
+    slope = kind == mz_gff::kSilu ? sig * (1.f + g * (1.f - sig)) : sig * (1.f - sig);
+  }
+}
+
+// four consecutive elements from / to memory; `vec`: all four exist and the address suits one access
+template <typename T> __device__ __forceinline__ void load4(const T* p, int n, bool vec, float (&v)[4]) {
+  if (vec) {
+    const vec4<T> t = *reinterpret_cast<const vec4<T>*>(p);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = (float)t[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = j < n ? (float)p[j] : 0.f;
+  }
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, int n, bool vec, const float (&v)[4]) {
+  if (vec) {
+    vec4<T> t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = (T)v[j];
+    *reinterpret_cast<vec4<T>*>(p) = t;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n) p[j] = (T)v[j];
+  }
+}
+
+constexpr unsigned kOutside = 0x80000000u;   // a byte offset no descriptor below covers: the load returns zeros
+
+// One operand's share of a step.  ACROSS: the matrix lies [k][row], else [row][k].  B rows a tile, NT threads.
+template <typename T, bool ACROSS, int B, int NT> struct Operand {
+  static constexpr int EC = 16 / (int)sizeof(T);        // elements of a 16-byte unit
+  static constexpr int KS = 128 / (int)sizeof(T);       // k of a step
+  static constexpr int UNITS = B * 8 / NT;              // 16-byte units a thread moves per step
+  static constexpr int UPR = ACROSS ? B / EC : 8;       // units of a staged row
+  static_assert(B * 8 % NT == 0 && NT % UPR == 0, "whole rows per round of threads");
+  static constexpr int RPR = NT / UPR;                  // staged rows a round covers
+  unsigned off[UNITS];                                  // byte offset from the step's origin
+  int row0, unit;                                       // staged row of the first unit; unit within the row
+
+  // the unit of a staged row where global unit u of that row is kept, so that the 16 x 16 blocks the wavefronts read
+  // fall on different banks: along - 16 rows at one unit, rows are 128 bytes and the banks 256, so pairs of rows move
+  // together; across - 16-bit: rows {8 g + 0..3} (or + 4..7) of two lane groups, a block being two units; float32:
+  // rows 4 g + j of four lane groups, a block being four units.
+  static __device__ __forceinline__ int place(int row, int u) {
+    if constexpr (!ACROSS) return u ^ ((row >> 1) & 7);
+    else if constexpr (sizeof(T) == 4) return u ^ (((row >> 2) & 3) << 2);
+    else return u ^ (across_swizzle(row) << 1);
+  }
+  static __device__ __forceinline__ int across_swizzle(int row) {
+    if constexpr (B >= 128) return (row & 3) | (((row >> 3) & 1) << 2);
+    else return ((row >> 1) & 1) | (((row >> 3) & 1) << 1);   // four blocks a row, two rows to 256 bytes
+  }
+
+  // row0_of(round) tells the matrix row of staged row 0 of the tile for `along`
+  __device__ __forceinline__ void init(int tid, long ld, long rows_left) {
+    row0 = tid / UPR;
+    unit = tid % UPR;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const int row = row0 + i * RPR;
+      if constexpr (ACROSS) off[i] = (long)unit * EC < rows_left ? (unsigned)(row * ld * (long)sizeof(T) + unit * 16) : kOutside;
+      else off[i] = row < rows_left ? (unsigned)(row * ld * (long)sizeof(T) + unit * 16) : kOutside;
+    }
+  }
+  // origin: the matrix element of (tile row 0, k = k0); k_left = nk - k0 > 0
+  __device__ __forceinline__ void load(const T* origin, long k_left, u32x4 (&v)[UNITS]) const {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(origin), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const bool inside = ACROSS ? row0 + i * RPR < k_left : (long)unit * EC < k_left;
+      v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(inside ? off[i] : kOutside), 0, 0));
+    }
+  }
+  __device__ __forceinline__ void stage(char* lds, const u32x4 (&v)[UNITS]) const {
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const int row = row0 + i * RPR;
+      *reinterpret_cast<u32x4*>(lds + row * (UPR * 16) + place(row, unit) * 16) = v[i];
+    }
+  }
+  // lane's 16 bytes of block `blk` (rows 16 blk ..) at sub-step `sub` of the step's two
+  static __device__ __forceinline__ u32x4 fragment(const char* lds, int blk, int sub, int lane) {
+    const int g = lane >> 4, l = lane & 15;
+    if constexpr (!ACROSS) {
+      const int row = blk * 16 + l;
+      return *reinterpret_cast<const u32x4*>(lds + row * 128 + (((sub * 4 + g) ^ ((row >> 1) & 7)) << 4));
+    } else if constexpr (sizeof(T) == 2) {
+      s16x8 out;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = sub * 32 + g * 8 + h * 4 + (l >> 2);
+        const char* p = lds + row * (UPR * 16) + ((blk ^ across_swizzle(row)) << 5) + (l & 3) * 8;
+        const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[h * 4 + j] = t[j];
+      }
+      return __builtin_bit_cast(u32x4, out);
+    } else {
+      u32x4 out;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = sub * 16 + g * 4 + j;
+        out[j] = *reinterpret_cast<const unsigned*>(lds + row * (UPR * 16) + ((blk ^ ((row >> 2) & 3)) << 6) + l * 4);
+      }
+      return out;
+    }
+  }
+};
+
+template <typename T, int MODE, int BR, int BC, int WR, int WC>
+__global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) void gff_gemm_kernel(Args a) {
+  using namespace mz_gff;
+  constexpr int NT = WR * WC * 64;
+  constexpr bool kPair = MODE == kForward || MODE == kGateGrad;       // a tile's R rows: half gate, half up features
+  constexpr bool kRAcross = !kPair, kCAcross = MODE == kWeightGrad;
+  using OpR = Operand<T, kRAcross, BR, NT>;
+  using OpC = Operand<T, kCAcross, BC, NT>;
+  constexpr int KS = OpR::KS;
+  constexpr int RM = BR / WR / 16, CN = BC / WC / 16;                 // 16 x 16 blocks of a wavefront
+  constexpr int TR = kPair ? BR / 2 : BR;                             // output rows (r) of a tile
+  extern __shared__ __attribute__((aligned(16))) char lds[];          // 2 x (BR + BC) x 128 bytes
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wave / WC, wc = wave % WC;
+
+  // ---- this workgroup's tile.  Workgroups go to the 8 XCDs in turn: XCD x takes the x-th run of consecutive tiles, and
+  // consecutive tiles walk 8 tiles of c under each tile of r, so that an L2 holds what its workgroups share.
+  const unsigned tiles_r = (unsigned)((a.nr + TR - 1) / TR), tiles_c = (unsigned)((a.nc + BC - 1) / BC);
+  const unsigned problems = MODE == kWeightGrad ? 2 : 1;
+  const unsigned per_problem = tiles_r * tiles_c, total = per_problem * problems * (unsigned)a.splits;
+  const unsigned per_xcd = (total + 7) / 8;
+  const unsigned id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (id >= total) return;
+  const unsigned job = id / per_problem, t = id - job * per_problem;
+  const int which = MODE == kWeightGrad ? (int)(job % 2) : 0;
+  const int split = (int)(MODE == kWeightGrad ? job / 2 : job);
+  constexpr unsigned kGroup = 8;
+  const unsigned band = t / (kGroup * tiles_r), in_band = t - band * (kGroup * tiles_r);
+  const unsigned band_c = tiles_c - band * kGroup < kGroup ? tiles_c - band * kGroup : kGroup;
+  const long r0 = (long)(in_band / band_c) * TR, c0 = (long)(band * kGroup + in_band % band_c) * BC;
+
+  // ---- operands
+  OpR opr;
+  OpC opc;
+  // a pair tile's two halves are two matrices: the rounds of threads split evenly between them
+  constexpr int kHalf = kPair ? OpR::UNITS / 2 : OpR::UNITS;
+  static_assert(!kPair || (OpR::UNITS % 2 == 0 && kHalf * OpR::RPR == BR / 2), "rounds cover a half");
+  opr.init(tid, a.ldr, a.nr - r0);
+  if constexpr (kPair) {          // rows of the second half are rows 0 .. BR/2 of the other matrix
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) opr.off[kHalf + i] = opr.off[i];
+  }
+  opc.init(tid, a.ldc, a.nc - c0);
+  // steps: kInputGrad runs over the features of dg and then over those of du
+  const long seg_steps = (a.nk + KS - 1) / KS;
+  const long all_steps = MODE == kInputGrad ? 2 * seg_steps : seg_steps;
+  const long first = (long)split * a.steps_per_split;
+  const long last = first + a.steps_per_split < all_steps ? first + a.steps_per_split : all_steps;
+
+  u32x4 rv[OpR::UNITS], cv[OpC::UNITS];
+  auto load_step = [&](long s) {
+    const int seg = MODE == kInputGrad && s >= seg_steps ? 1 : 0;
+    const long k0 = (s - seg * seg_steps) * KS, k_left = a.nk - k0;
+    if constexpr (kPair) {
+      u32x4 half[kHalf];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const T* origin = static_cast<const T*>(a.r[h]) + r0 * a.ldr + k0;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(origin), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+          half[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+              rs, (int)((long)opr.unit * OpR::EC < k_left ? opr.off[i] : kOutside), 0, 0));
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i) rv[h * kHalf + i] = half[i];
+      }
+    } else {
+      opr.load(static_cast<const T*>(a.r[seg]) + k0 * a.ldr + r0, k_left, rv);
+    }
+    const T* cm = static_cast<const T*>(a.c[MODE == kWeightGrad ? which : seg]);
+    opc.load(kCAcross ? cm + k0 * a.ldc + c0 : cm + c0 * a.ldc + k0, k_left, cv);
+  };
+  auto stage_step = [&](int buf) {
+    char* base = lds + buf * ((BR + BC) * 128);
+    opr.stage(base, rv);
+    opc.stage(base + BR * 128, cv);
+  };
+
+  f32x4 acc[RM][CN];
+#pragma unroll
+  for (int i = 0; i < RM; ++i)
+#pragma unroll
+    for (int j = 0; j < CN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the tile's 16-row block that this wavefront's block i is (pair tiles: the same features of both halves)
+  auto r_block = [&](int i) {
+    if constexpr (kPair) return (i / (RM / 2)) * (BR / 32) + wr * (RM / 2) + i % (RM / 2);
+    else return wr * RM + i;
+  };
+
+  if (first < last) {
+    load_step(first);
+    stage_step(0);
+  }
+  __syncthreads();
+  int buf = 0;
+  for (long s = first; s < last; ++s, buf ^= 1) {
+    if (s + 1 < last) load_step(s + 1);
+    const char* rs = lds + buf * ((BR + BC) * 128);
+    const char* cs = rs + BR * 128;
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      u32x4 cf[CN];
+#pragma unroll
+      for (int j = 0; j < CN; ++j) cf[j] = OpC::fragment(cs, wc * CN + j, sub, lane);
+#pragma unroll
+      for (int i = 0; i < RM; ++i) {
+        const u32x4 rf = OpR::fragment(rs, r_block(i), sub, lane);
+#pragma unroll
+        for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf, cf[j], acc[i][j], T{});
+      }
+    }
+    if (s + 1 < last) stage_step(buf ^ 1);
+    __syncthreads();
+  }
+
+  // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
+  const int lr = (lane >> 4) * 4, lc = lane & 15;
+  if constexpr (kPair) {
+    T* out0 = static_cast<T*>(a.out[0]);
+    T* out1 = static_cast<T*>(a.out[1]);
+    const bool vec_out = (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
+    const bool vec_dh = (a.lddh & 3) == 0 && ((size_t)a.dh & (4 * sizeof(T) - 1)) == 0;
+    float* colsum = reinterpret_cast<float*>(lds);                    // kGateGrad: [WC][2][TR]
+#pragma unroll
+    for (int i = 0; i < RM / 2; ++i) {
+      const int fr = (wr * (RM / 2) + i) * 16 + lr;                   // feature within the tile
+      const long f = r0 + fr;
+      const int nf = (int)(a.nr - f < 4 ? a.nr - f : 4);              // features that exist (may be <= 0)
+      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+      if (a.bias[0]) load4(static_cast<const T*>(a.bias[0]) + f, nf, false, bg);
+      if (a.bias[1]) load4(static_cast<const T*>(a.bias[1]) + f, nf, false, bu);
+      float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < CN; ++j) {
+        const long c = c0 + (wc * CN + j) * 16 + lc;
+        if (c >= a.nc) continue;
+        const f32x4 g = acc[i][j], u = acc[i + RM / 2][j];
+        if constexpr (MODE == kForward) {
+          float o[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) o[q] = activate<T>(a.activation, g[q] + bg[q]) * (u[q] + bu[q]);
+          store4(out0 + c * a.ldo + f, nf, vec_out && nf == 4, o);
+        } else {
+          float d[4], og[4], ou[4];
+          load4(static_cast<const T*>(a.dh) + c * a.lddh + f, nf, vec_dh && nf == 4, d);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float act, slope;
+            activate_grad<T>(a.activation, g[q] + bg[q], act, slope);
+            og[q] = q < nf ? d[q] * (u[q] + bu[q]) * slope : 0.f;
+            ou[q] = q < nf ? d[q] * act : 0.f;
+            sg[q] += og[q];
+            su[q] += ou[q];
+          }
+          // columns up to nr_pad exist and are read as k of the input gradient: zeros there
+          const int np = (int)(a.nr_pad - f < 4 ? a.nr_pad - f : 4);
+          store4(out0 + c * a.ldo + f, np, np == 4, og);
+          store4(out1 + c * a.ldo + f, np, np == 4, ou);
+        }
+      }
+      if constexpr (MODE == kGateGrad) {
+        if (a.col_partial) {       // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            sg[q] = lanes_sum<16>(sg[q]);
+            su[q] = lanes_sum<16>(su[q]);
+          }
+          if (lc == 0)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              colsum[(wc * 2 + 0) * TR + fr + q] = sg[q];
+              colsum[(wc * 2 + 1) * TR + fr + q] = su[q];
+            }
+        }
+      }
+    }
+    if constexpr (MODE == kGateGrad) {
+      if (a.col_partial) {
+        __syncthreads();
+        for (int i = tid; i < 2 * TR; i += NT) {
+          const int side = i / TR, f = i % TR;
+          if (r0 + f >= a.nr) continue;
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < WC; ++w) v += colsum[(w * 2 + side) * TR + f];
+          a.col_partial[((c0 / BC) * 2 + side) * a.nr + r0 + f] = v;
+        }
+      }
+    }
+  } else {
+    const bool whole = a.splits == 1;
+    T* out = static_cast<T*>(a.out[which]);
+    float* part = whole ? nullptr : a.partial + ((long)split * problems + which) * a.nc * a.nr;
+    const bool vec_out = (a.ldo & 3) == 0 && ((size_t)out & (4 * sizeof(T) - 1)) == 0;
+    const bool vec_part = (a.nr & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      const long r = r0 + (wr * RM + i) * 16 + lr;
+      const int n = (int)(a.nr - r < 4 ? a.nr - r : 4);
+#pragma unroll
+      for (int j = 0; j < CN; ++j) {
+        const long c = c0 + (wc * CN + j) * 16 + lc;
+        if (c >= a.nc) continue;
+        const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (whole) store4(out + c * a.ldo + r, n, vec_out && n == 4, o);
+        else store4(part + c * a.nr + r, n, vec_part && n == 4, o);
+      }
+    }
+  }
+}
+
+template <typename T, int MODE, int BR, int BC, int WR, int WC> int launch_one(const Args& a, hipStream_t s) {
+  constexpr int TR = MODE <= mz_gff::kGateGrad ? BR / 2 : BR, kLds = 2 * (BR + BC) * 128;
+  static bool done[mz::kMaxDevices] = {false};
+  const auto kernel = gff_gemm_kernel<T, MODE, BR, BC, WR, WC>;
+  if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
+  const long total = ((a.nr + TR - 1) / TR) * ((a.nc + BC - 1) / BC) * (MODE == mz_gff::kWeightGrad ? 2 : 1) * a.splits;
+  if (total > 0x7ffffff0l) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 7) / 8 * 8)), dim3(WR * WC * 64), kLds, s, a);
+  return MZ_OK;
+}
+
+template <typename T, int MODE> int launch_mode(const Args& a, int tile, hipStream_t s) {
+  if (tile == 0) return launch_one<T, MODE, 256, 256, 2, 4>(a, s);
+  if (tile == 1) return launch_one<T, MODE, 128, 128, 2, 2>(a, s);
+  return launch_one<T, MODE, 64, 64, 2, 2>(a, s);
+}
+template <typename T> int launch_any(const Args& a, int mode, int tile, hipStream_t s) {
+  switch (mode) {
+    case mz_gff::kForward: return launch_mode<T, mz_gff::kForward>(a, tile, s);
+    case mz_gff::kGateGrad: return launch_mode<T, mz_gff::kGateGrad>(a, tile, s);
+    case mz_gff::kInputGrad: return launch_mode<T, mz_gff::kInputGrad>(a, tile, s);
+    default: return launch_mode<T, mz_gff::kWeightGrad>(a, tile, s);
+  }
+}
+
+// ---- a few tokens (at most 64): the weights are read once, straight into the matrix instructions' registers; 16
+// features (their gate and up rows) a workgroup, its four wavefronts split k and add up through LDS.
+template <typename T, int CN> __global__ __launch_bounds__(256) void gff_few_kernel(Args a) {
+  constexpr int EC = 16 / (int)sizeof(T), KB = 4 * EC;     // k of one round of a wavefront's lanes
+  constexpr int kUnroll = CN == 1 ? 4 : 2;
+  __shared__ f32x4 red[3][2][CN][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l = lane & 15;
+  const long f0 = (long)blockIdx.x * 16;
+  // rows and tokens past the end read the last one's: their results are not stored
+  const long f_row = f0 + l < a.nr ? f0 + l : a.nr - 1;
+  const T* wg = static_cast<const T*>(a.r[0]) + f_row * a.ldr;
+  const T* wu = static_cast<const T*>(a.r[1]) + f_row * a.ldr;
+  const T* x[CN];
+#pragma unroll
+  for (int j = 0; j < CN; ++j) x[j] = static_cast<const T*>(a.c[0]) + (j * 16 + l < a.nc ? j * 16 + l : a.nc - 1) * a.ldc;
+  f32x4 acc[2][CN];
+#pragma unroll
+  for (int j = 0; j < CN; ++j) acc[0][j] = acc[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int rounds = (int)((a.nk + KB - 1) / KB);
+  for (int q0 = wave * kUnroll; q0 < rounds; q0 += 4 * kUnroll) {
+    Vec16<T> rg[kUnroll], ru[kUnroll], cf[kUnroll][CN];
+    if ((long)(q0 + kUnroll) * KB <= a.nk) {        // all of it inside: loads without conditions, all in flight
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const long k = (long)(q0 + q) * KB + g * EC;
+        rg[q].load(wg + k);
+        ru[q].load(wu + k);
+#pragma unroll
+        for (int j = 0; j < CN; ++j) cf[q][j].load(x[j] + k);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kUnroll; ++q) {
+        const long k = (long)(q0 + q) * KB + g * EC;
+        rg[q].load_upto(wg + k, a.nk - k);
+        ru[q].load_upto(wu + k, a.nk - k);
+#pragma unroll
+        for (int j = 0; j < CN; ++j) cf[q][j].load_upto(x[j] + k, a.nk - k);
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kUnroll; ++q)
+#pragma unroll
+      for (int j = 0; j < CN; ++j) {
+        const u32x4 c = __builtin_bit_cast(u32x4, cf[q][j].v);
+        acc[0][j] = mma(__builtin_bit_cast(u32x4, rg[q].v), c, acc[0][j], T{});
+        acc[1][j] = mma(__builtin_bit_cast(u32x4, ru[q].v), c, acc[1][j], T{});
+      }
+  }
+  if (wave > 0) {
+#pragma unroll
+    for (int j = 0; j < CN; ++j) {
+      red[wave - 1][0][j][lane] = acc[0][j];
+      red[wave - 1][1][j][lane] = acc[1][j];
+    }
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  const long f = f0 + g * 4;
+  const int nf = (int)(a.nr - f < 4 ? a.nr - f : 4);
+  float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
+  if (a.bias[0]) load4(static_cast<const T*>(a.bias[0]) + f, nf, false, bg);
+  if (a.bias[1]) load4(static_cast<const T*>(a.bias[1]) + f, nf, false, bu);
+  const bool vec = nf == 4 && (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll
+  for (int j = 0; j < CN; ++j) {
+    f32x4 s0 = acc[0][j], s1 = acc[1][j];
+#pragma unroll
+    for (int w = 0; w < 3; ++w) {
+      s0 += red[w][0][j][lane];
+      s1 += red[w][1][j][lane];
+    }
+    const long c = j * 16 + l;
+    if (c >= a.nc) continue;
+    float o[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = activate<T>(a.activation, s0[q] + bg[q]) * (s1[q] + bu[q]);
+    store4(static_cast<T*>(a.out[0]) + c * a.ldo + f, nf, vec, o);
+  }
+}
+
+template <typename T> int launch_few(const Args& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.nr + 15) / 16)), block(256);
+  if (a.nc <= 16) hipLaunchKernelGGL((gff_few_kernel<T, 1>), grid, block, 0, s, a);
+  else if (a.nc <= 32) hipLaunchKernelGGL((gff_few_kernel<T, 2>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((gff_few_kernel<T, 4>), grid, block, 0, s, a);
+  return MZ_OK;
+}
+
+}  // namespace
+#endif  // MZ_GFF_KERNELS

@@ -1,0 +1,324 @@
+// Gated feed-forward projection, forward and backward:
+//     g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) * u                    x [M][K], Wg, Wu [F][K], h [M][F]
+//     dg = dh u act'(g),  du = dh act(g)
+//     dx = dg Wg + du Wu,   dWg = dg^T x,  dWu = du^T x,   dbg = sum_rows dg,  dbu = sum_rows du
+// Forward is one kernel: a wavefront owns the gate and the up product of the same features, so activation and product
+// happen in its registers and only h is written.  Nothing else is kept for the backward pass: it computes g and u again
+// (4 M K F operations against 8 M F bytes written and read back in 16 bits - and without rounding g and u), writes
+// dg and du in the operands' type - they are matrix operands next, and their rounding adds one half step to a sum's
+// terms - and runs the two products that need them.  Sums over few tiles are split along k into float32 partial
+// results that a second launch adds up in a fixed order: no atomics, the same bits on every run.
+#include "gated_ff.h"
+
+namespace {
+
+using mz_gff::Args;
+
+int elem_bytes(int dtype) { return dtype == MZ_F32 ? 4 : 2; }
+int unit_elems(int dtype) { return 16 / elem_bytes(dtype); }
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+int launch(const Args& a, int dtype, int mode, int tile, hipStream_t s) {
+  return dtype == MZ_F32 ? mz_gff::launch_f32(a, mode, tile, s)
+         : dtype == MZ_BF16 ? mz_gff::launch_bf16(a, mode, tile, s)
+                            : mz_gff::launch_f16(a, mode, tile, s);
+}
+
+// a matrix whose rows are no whole 16-byte units (K odd for them), copied to rows that are, with zeros behind
+template <typename U>
+__global__ __launch_bounds__(256) void pad_rows_kernel(const U* __restrict__ in, long ld, U* __restrict__ out, long rows,
+                                                       int cols, int cols_pad) {
+  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * cols_pad; i += (long)gridDim.x * 256) {
+    const long r = i / cols_pad;
+    const int c = (int)(i - r * cols_pad);
+    out[i] = c < cols ? in[r * ld + c] : (U)0;
+  }
+}
+void pad_rows(const void* in, int64_t ld, void* out, int64_t rows, int64_t cols, int64_t cols_pad, int dtype, hipStream_t s) {
+  const long want = (rows * cols_pad + 255) / 256, cap = 16L * mz::compute_units();
+  const dim3 grid((unsigned)(want < cap ? want : cap));
+  if (elem_bytes(dtype) == 4)
+    hipLaunchKernelGGL((pad_rows_kernel<unsigned>), grid, dim3(256), 0, s, static_cast<const unsigned*>(in), ld,
+                       static_cast<unsigned*>(out), rows, (int)cols, (int)cols_pad);
+  else
+    hipLaunchKernelGGL((pad_rows_kernel<unsigned short>), grid, dim3(256), 0, s, static_cast<const unsigned short*>(in), ld,
+                       static_cast<unsigned short*>(out), rows, (int)cols, (int)cols_pad);
+}
+
+// out[p][c][r] = sum over the splits of partial[split][p][c][r]
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, long per_problem,
+                                                   int problems, T* out0, T* out1) {
+  const long n = per_problem * problems;
+  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long)gridDim.x * 1024) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const int m = (int)(n - i < 4 ? n - i : 4);
+    for (int s = 0; s < splits; ++s) {
+      const float* p = partial + s * n + i;
+      if (m == 4 && (n & 3) == 0) {
+        const float4 t = *reinterpret_cast<const float4*>(p);
+        v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+      } else {
+        for (int j = 0; j < m; ++j) v[j] += p[j];
+      }
+    }
+    for (int j = 0; j < m; ++j) {
+      const long e = i + j;
+      if (e < per_problem) out0[e] = (T)v[j];
+      else out1[e - per_problem] = (T)v[j];
+    }
+  }
+}
+template <typename T> void join_t(const Args& a, int problems, hipStream_t s) {
+  const long n = a.nr * a.nc * problems, want = (n + 1023) / 1024, cap = 8L * mz::compute_units();
+  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, s, a.partial, a.splits,
+                     a.nr * a.nc, problems, static_cast<T*>(a.out[0]), static_cast<T*>(a.out[1]));
+}
+void join(const Args& a, int problems, int dtype, hipStream_t s) {
+  if (dtype == MZ_F32) join_t<float>(a, problems, s);
+  else if (dtype == MZ_BF16) join_t<__bf16>(a, problems, s);
+  else join_t<_Float16>(a, problems, s);
+}
+
+// bias gradients: dbias[side][f] = sum over the token tiles of col_partial[tile][side][f]; 32 features x 32 tile lanes
+template <typename T>
+__global__ __launch_bounds__(1024) void bias_grad_kernel(const float* __restrict__ partial, long tiles, long F, T* dbg, T* dbu) {
+  __shared__ float red[2][32][33];
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
+  const long f = (long)blockIdx.x * 32 + col;
+  float g = 0.f, u = 0.f;
+  if (f < F)
+    for (long t = lane; t < tiles; t += 32) {
+      g += partial[(t * 2 + 0) * F + f];
+      u += partial[(t * 2 + 1) * F + f];
+    }
+  red[0][lane][col] = g;
+  red[1][lane][col] = u;
+  __syncthreads();
+  if (lane >= 2 || f >= F) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v += red[lane][k][col];
+  T* out = lane == 0 ? dbg : dbu;
+  if (out) out[f] = (T)v;
+}
+template <typename T> void bias_grad_t(const float* p, long tiles, long F, void* g, void* u, hipStream_t s) {
+  hipLaunchKernelGGL((bias_grad_kernel<T>), dim3((unsigned)((F + 31) / 32)), dim3(1024), 0, s, p, tiles, F,
+                     static_cast<T*>(g), static_cast<T*>(u));
+}
+
+int64_t tiles(int64_t nr, int64_t nc, int tr, int bc) { return ((nr + tr - 1) / tr) * ((nc + bc - 1) / bc); }
+
+// the largest tile that still gives every compute unit one
+int pick_tile(int64_t nr, int64_t nc, bool pair, int problems) {
+  for (int t = 0; t < 2; ++t) {
+    const int side = mz_gff::tile_side(t);
+    if (tiles(nr, nc, pair ? side / 2 : side, side) * problems >= 256) return t;
+  }
+  return 2;
+}
+
+struct Split { int tile, splits, steps; };
+constexpr int kMaxSplits = 32;
+// tile and split of a product whose sum may be cut: prefer whole sums in the largest tile that fills the chip; else
+// 128 x 128 tiles (64 x 64 where the outputs are few) with the sum cut into enough parts for one tile per compute unit,
+// at least four steps each
+Split pick_split(int64_t nr, int64_t nc, int problems, int64_t steps) {
+  const int whole = pick_tile(nr, nc, false, problems);
+  Split p = {whole, 1, (int)steps};
+  if (whole < 2) return p;
+  p.tile = nr > 64 && nc > 64 ? 1 : 2;
+  const int side = mz_gff::tile_side(p.tile);
+  const int64_t have = tiles(nr, nc, side, side) * problems;
+  int64_t splits = (256 + have - 1) / have;
+  if (splits > steps / 4) splits = steps / 4;
+  if (splits > kMaxSplits) splits = kMaxSplits;
+  if (splits < 1) splits = 1;
+  p.steps = (int)((steps + splits - 1) / splits);
+  p.splits = (int)((steps + p.steps - 1) / p.steps);
+  return p;
+}
+
+struct Shape {
+  int64_t M, K, F, Kp, Fp;
+  int dtype;
+  bool pads;                 // K is no whole number of 16-byte units: x, Wg, Wu are copied to padded rows
+  int64_t pad_bytes() const { return pads ? round_up(M * Kp * elem_bytes(dtype), 256) + 2 * round_up(F * Kp * elem_bytes(dtype), 256) : 0; }
+  int k_step() const { return 128 / elem_bytes(dtype); }
+};
+Shape make_shape(int64_t M, int64_t K, int64_t F, int dtype) {
+  const int e = unit_elems(dtype);
+  return {M, K, F, round_up(K, e), round_up(F, e), dtype, K % e != 0};
+}
+constexpr int64_t kFew = 64;   // tokens the streaming kernel takes
+
+struct Backward {
+  Split dx, dw;
+  int gate_tile;
+  int64_t dgu_bytes, col_bytes, partial_bytes;
+};
+Backward plan_backward(const Shape& h) {
+  Backward b;
+  const int64_t f_steps = 2 * ((h.F + h.k_step() - 1) / h.k_step()), m_steps = (h.M + h.k_step() - 1) / h.k_step();
+  b.gate_tile = pick_tile(h.F, h.M, true, 1);
+  b.dx = pick_split(h.K, h.M, 1, f_steps);
+  b.dw = pick_split(h.K, h.F, 2, m_steps);
+  b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
+  const int side = mz_gff::tile_side(b.gate_tile);
+  b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
+  const int64_t px = b.dx.splits > 1 ? b.dx.splits * h.M * h.K * 4 : 0, pw = b.dw.splits > 1 ? b.dw.splits * 2 * h.F * h.K * 4 : 0;
+  b.partial_bytes = round_up(px > pw ? px : pw, 256);
+  return b;
+}
+
+int check_shape(const char* who, int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation) {
+  MZ_REQUIRE(dtype == MZ_F32 || dtype == MZ_BF16 || dtype == MZ_F16, "%s: unknown element type %d", who, dtype);
+  MZ_REQUIRE(M > 0 && K > 0 && F > 0 && K <= (1 << 20) && F <= (1 << 20) && M <= (1ll << 40),
+             "%s: sizes out of range (M = %lld, K = %lld, F = %lld; K and F up to 2^20)", who, (long long)M, (long long)K,
+             (long long)F);
+  MZ_REQUIRE(activation >= 0 && activation <= mz_gff::kSigmoid, "%s: unknown activation %d", who, activation);
+  return MZ_OK;
+}
+int check_operands(const char* who, const Shape& h, const void* x, int64_t ldx, const void* wg, const void* wu) {
+  MZ_REQUIRE(ldx >= h.K && ldx * elem_bytes(h.dtype) <= (1 << 22),
+             "%s: stride of x out of range (%lld, K = %lld; rows up to 4 MiB apart)", who, (long long)ldx, (long long)h.K);
+  MZ_REQUIRE(h.pads || (((size_t)x | (size_t)wg | (size_t)wu) % 16 == 0 && ldx % unit_elems(h.dtype) == 0),
+             "%s: x, w_gate, w_up and the rows of x must start on 16 bytes", who);
+  return MZ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward) {
+  if (check_shape("mz_gated_ff_workspace_bytes", M, K, F, dtype, 0)) return -1;
+  const Shape h = make_shape(M, K, F, dtype);
+  if (!backward) return M <= kFew ? 0 : h.pad_bytes();
+  const Backward b = plan_backward(h);
+  return h.pad_bytes() + 2 * b.dgu_bytes + b.col_bytes + b.partial_bytes;
+}
+
+int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                    int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation, void* h, void* workspace,
+                    int64_t workspace_bytes, mz_stream_t stream) {
+  MZ_REQUIRE(x && w_gate && w_up && h, "mz_gated_ff_fwd: null tensor");
+  if (int rc = check_shape("mz_gated_ff_fwd", M, K, F, dtype, activation)) return rc;
+  Shape sh = make_shape(M, K, F, dtype);
+  if (int rc = check_operands("mz_gated_ff_fwd", sh, x, ldx, w_gate, w_up)) return rc;
+  hipStream_t s = mz::as_stream(stream);
+  Args a = {};
+  a.r[0] = w_gate; a.r[1] = w_up;
+  a.c[0] = a.c[1] = x;
+  a.ldr = K; a.ldc = ldx;
+  a.nr = F; a.nc = M; a.nk = K;
+  a.out[0] = h; a.ldo = F;
+  a.bias[0] = b_gate; a.bias[1] = b_up;
+  a.activation = activation;
+  a.splits = 1;
+  if (M <= kFew) {
+    if (int rc = dtype == MZ_F32 ? mz_gff::launch_few_f32(a, s) : dtype == MZ_BF16 ? mz_gff::launch_few_bf16(a, s) : mz_gff::launch_few_f16(a, s))
+      return rc;
+    return mz::check_launch("mz_gated_ff_fwd");
+  }
+  const int64_t need = sh.pad_bytes();
+  MZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (size_t)workspace % 16 == 0),
+             "mz_gated_ff_fwd: workspace too small or not 16-byte aligned");
+  if (sh.pads) {
+    char* w = static_cast<char*>(workspace);
+    const int64_t xb = round_up(M * sh.Kp * elem_bytes(dtype), 256), wb = round_up(F * sh.Kp * elem_bytes(dtype), 256);
+    pad_rows(x, ldx, w, M, K, sh.Kp, dtype, s);
+    pad_rows(w_gate, K, w + xb, F, K, sh.Kp, dtype, s);
+    pad_rows(w_up, K, w + xb + wb, F, K, sh.Kp, dtype, s);
+    a.c[0] = a.c[1] = w;
+    a.r[0] = w + xb; a.r[1] = w + xb + wb;
+    a.ldr = a.ldc = a.nk = sh.Kp;
+  }
+  a.steps_per_split = (int)((a.nk + sh.k_step() - 1) / sh.k_step());
+  if (int rc = launch(a, dtype, mz_gff::kForward, pick_tile(F, M, true, 1), s)) return rc;
+  return mz::check_launch("mz_gated_ff_fwd");
+}
+
+int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
+                    const void* dh, int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation, void* dx,
+                    void* dw_gate, void* dw_up, void* db_gate, void* db_up, void* workspace, int64_t workspace_bytes,
+                    mz_stream_t stream) {
+  MZ_REQUIRE(x && w_gate && w_up && dh, "mz_gated_ff_bwd: null tensor");
+  MZ_REQUIRE((dw_gate == nullptr) == (dw_up == nullptr), "mz_gated_ff_bwd: dw_gate and dw_up go together");
+  MZ_REQUIRE(dx || dw_gate || db_gate || db_up, "mz_gated_ff_bwd: no gradient asked for");
+  if (int rc = check_shape("mz_gated_ff_bwd", M, K, F, dtype, activation)) return rc;
+  Shape sh = make_shape(M, K, F, dtype);
+  if (int rc = check_operands("mz_gated_ff_bwd", sh, x, ldx, w_gate, w_up)) return rc;
+  const Backward plan = plan_backward(sh);
+  const int64_t need = mz_gated_ff_workspace_bytes(M, K, F, dtype, 1);
+  MZ_REQUIRE(workspace && workspace_bytes >= need && (size_t)workspace % 16 == 0,
+             "mz_gated_ff_bwd: workspace too small (%lld of %lld bytes) or not 16-byte aligned", (long long)workspace_bytes,
+             (long long)need);
+  hipStream_t s = mz::as_stream(stream);
+  char* w = static_cast<char*>(workspace);
+  const void *xm = x, *wg = w_gate, *wu = w_up;
+  int64_t ldxm = ldx, kk = K;
+  if (sh.pads) {
+    const int64_t xb = round_up(M * sh.Kp * elem_bytes(dtype), 256), wb = round_up(F * sh.Kp * elem_bytes(dtype), 256);
+    pad_rows(x, ldx, w, M, K, sh.Kp, dtype, s);
+    pad_rows(w_gate, K, w + xb, F, K, sh.Kp, dtype, s);
+    pad_rows(w_up, K, w + xb + wb, F, K, sh.Kp, dtype, s);
+    xm = w; wg = w + xb; wu = w + xb + wb;
+    ldxm = kk = sh.Kp;
+    w += sh.pad_bytes();
+  }
+  char* dg = w;
+  char* du = dg + plan.dgu_bytes;
+  float* cols = reinterpret_cast<float*>(du + plan.dgu_bytes);
+  float* partial = reinterpret_cast<float*>(du + plan.dgu_bytes + plan.col_bytes);
+  const bool biases = db_gate || db_up;
+
+  Args a = {};                                     // dg, du
+  a.r[0] = wg; a.r[1] = wu;
+  a.c[0] = a.c[1] = xm;
+  a.ldr = kk; a.ldc = ldxm;
+  a.nr = F; a.nc = M; a.nk = kk;
+  a.out[0] = dg; a.out[1] = du; a.ldo = sh.Fp;
+  a.bias[0] = b_gate; a.bias[1] = b_up;
+  a.dh = dh; a.lddh = F;
+  a.col_partial = biases ? cols : nullptr;
+  a.nr_pad = sh.Fp;
+  a.activation = activation;
+  a.splits = 1;
+  a.steps_per_split = (int)((kk + sh.k_step() - 1) / sh.k_step());
+  if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
+  if (biases) {
+    const int side = mz_gff::tile_side(plan.gate_tile);
+    const long n = (long)((M + side - 1) / side);
+    if (dtype == MZ_F32) bias_grad_t<float>(cols, n, F, db_gate, db_up, s);
+    else if (dtype == MZ_BF16) bias_grad_t<__bf16>(cols, n, F, db_gate, db_up, s);
+    else bias_grad_t<_Float16>(cols, n, F, db_gate, db_up, s);
+  }
+  if (dx) {
+    Args p = {};
+    p.r[0] = wg; p.r[1] = wu;
+    p.c[0] = dg; p.c[1] = du;
+    p.ldr = kk; p.ldc = sh.Fp;
+    p.nr = K; p.nc = M; p.nk = F;
+    p.out[0] = p.out[1] = dx; p.ldo = K;
+    p.partial = partial;
+    p.splits = plan.dx.splits; p.steps_per_split = plan.dx.steps;
+    if (int rc = launch(p, dtype, mz_gff::kInputGrad, plan.dx.tile, s)) return rc;
+    if (p.splits > 1) join(p, 1, dtype, s);
+  }
+  if (dw_gate) {
+    Args p = {};
+    p.r[0] = p.r[1] = xm;
+    p.c[0] = dg; p.c[1] = du;
+    p.ldr = ldxm; p.ldc = sh.Fp;
+    p.nr = K; p.nc = F; p.nk = M;
+    p.out[0] = dw_gate; p.out[1] = dw_up; p.ldo = K;
+    p.partial = partial;
+    p.splits = plan.dw.splits; p.steps_per_split = plan.dw.steps;
+    if (int rc = launch(p, dtype, mz_gff::kWeightGrad, plan.dw.tile, s)) return rc;
+    if (p.splits > 1) join(p, 2, dtype, s);
+  }
+  return mz::check_launch("mz_gated_ff_bwd");
+}
+
+}  // extern "C"

@@ -1,0 +1,461 @@
+// Layer norm over the last dimension, forward and backward (the training-block counterpart of bn_train.hip for batches
+// that batch statistics do not suit: single states, unequal games):
+//     y = (x - m) r w + b,   m = mean(x),  r = 1 / sqrt(mean((x - m)^2) + eps)          per row
+//     dx = r (w dy - mean(w dy) - xh mean(w dy xh)),  dw = sum_rows dy xh,  db = sum_rows dy,   xh = (x - m) r
+// All sums in float32; the variance is the mean of squared deviations from the mean already known (a second pass over
+// registers), so a large common offset costs no digits.
+//
+// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx, each once.  A row lives in the
+// registers of a group of TPR threads (16, 32 or 64 lanes, or a workgroup), NV 16-byte vectors a thread; groups walk
+// down the rows with the parameters of their columns - and, backward, the columns' running dw and db - in registers.
+// Every workgroup leaves its dw and db in a float32 partial row and a second launch adds those up: no atomics, the
+// same bits on every run.
+#include "block_common.h"
+
+namespace {
+
+constexpr int kMaxRegisterCols = 16384;     // 1024 threads x 16 columns; wider rows take the looping kernels
+constexpr int kMaxPartials = 1024;
+
+struct LnArgs {
+  const void* x;
+  const void* dy;
+  const void* weight;
+  const void* bias;
+  void* out;               // y or dx
+  float* mean;
+  float* rstd;
+  float* partial;          // [blocks][2][C]
+  long ldx, lddy, rows;
+  int C, affine_f32;
+  float eps;
+};
+
+// sum of `v` over the TPR threads of a row; `red` holds one float per wavefront of the workgroup.  Rows wider than a
+// wavefront have the workgroup to themselves, and every thread of it gets here.
+template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
+  if constexpr (TPR <= 64) {
+    return lanes_sum<TPR>(v);
+  } else {
+    v = lanes_sum<64>(v);
+    __syncthreads();                        // the previous sum has been read
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) s += red[i];
+    return s;
+  }
+}
+
+template <int TPR> constexpr int block_threads() { return TPR < 256 ? 256 : TPR; }
+
+// ------------------------------------------------------------------------------------------------------------ forward
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(block_threads<TPR>()) void ln_fwd_kernel(LnArgs a) {
+  constexpr int N = Vec16<T>::N, RPB = block_threads<TPR>() / TPR;
+  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const T* x = static_cast<const T*>(a.x);
+  T* y = static_cast<T*>(a.out);
+  const float inv_c = 1.f / (float)a.C;
+  float w[NV][N], b[NV][N];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (k * TPR + lane) * N + j;
+      w[k][j] = a.weight && c < a.C ? load_param<T>(a.weight, a.affine_f32, c) : 1.f;
+      b[k][j] = a.bias && c < a.C ? load_param<T>(a.bias, a.affine_f32, c) : 0.f;
+    }
+  for (long r0 = (long)blockIdx.x * RPB; r0 < a.rows; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + sub;
+    const bool live = r < a.rows;           // TPR > 64: one row a workgroup, always live
+    Vec16<T> v[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lane) * N;
+      v[k].load_upto(x + r * a.ldx + c, live ? a.C - c : 0);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += (float)v[k].v[j];
+    const float mean = row_sum<TPR>(s, red) * inv_c;
+    float q = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = (float)v[k].v[j] - mean;
+        q += (k * TPR + lane) * N + j < a.C ? d * d : 0.f;
+      }
+    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) * inv_c + a.eps);
+    if (!live) continue;
+    if (a.mean && lane == 0) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lane) * N;
+      Vec16<T> o;
+#pragma unroll
+      for (int j = 0; j < N; ++j) o.v[j] = (T)(((float)v[k].v[j] - mean) * rstd * w[k][j] + b[k][j]);
+      o.store_upto(y + r * (long)a.C + c, a.C - c);
+    }
+  }
+}
+
+// rows wider than the registers of a workgroup: three passes over the row, the later two out of the caches
+template <typename T> __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(LnArgs a) {
+  constexpr int N = Vec16<T>::N;
+  __shared__ float red[16];
+  const float inv_c = 1.f / (float)a.C;
+  for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+    T* y = static_cast<T*>(a.out) + r * (long)a.C;
+    float s = 0.f;
+    for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
+      Vec16<T> v;
+      v.load_upto(x + c, a.C - c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s += (float)v.v[j];
+    }
+    const float mean = row_sum<1024>(s, red) * inv_c;
+    float q = 0.f;
+    for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
+      Vec16<T> v;
+      v.load_upto(x + c, a.C - c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float d = (float)v.v[j] - mean;
+        q += c + j < a.C ? d * d : 0.f;
+      }
+    }
+    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red) * inv_c + a.eps);
+    if (a.mean && threadIdx.x == 0) {
+      a.mean[r] = mean;
+      a.rstd[r] = rstd;
+    }
+    for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
+      Vec16<T> v;
+      v.load_upto(x + c, a.C - c);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c + j < a.C) {
+          const float w = a.weight ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
+          const float b = a.bias ? load_param<T>(a.bias, a.affine_f32, c + j) : 0.f;
+          v.v[j] = (T)(((float)v.v[j] - mean) * rstd * w + b);
+        }
+      v.store_upto(y + c, a.C - c);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------------------------- backward
+template <typename T, int TPR, int NV>
+__global__ __launch_bounds__(block_threads<TPR>()) void ln_bwd_kernel(LnArgs a) {
+  constexpr int N = Vec16<T>::N, RPB = block_threads<TPR>() / TPR;
+  constexpr int kCols = TPR * NV * N;
+  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  __shared__ float cols[RPB > 1 ? RPB * 2 * kCols : 1];
+  const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  T* dx = static_cast<T*>(a.out);
+  const float inv_c = 1.f / (float)a.C;
+  float w[NV][N], dw[NV][N], db[NV][N];
+#pragma unroll
+  for (int k = 0; k < NV; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = (k * TPR + lane) * N + j;
+      w[k][j] = a.weight && c < a.C ? load_param<T>(a.weight, a.affine_f32, c) : 1.f;
+      dw[k][j] = db[k][j] = 0.f;
+    }
+  for (long r0 = (long)blockIdx.x * RPB; r0 < a.rows; r0 += (long)gridDim.x * RPB) {
+    const long r = r0 + sub;
+    const bool live = r < a.rows;
+    Vec16<T> xv[NV], gv[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lane) * N;
+      xv[k].load_upto(x + r * a.ldx + c, live ? a.C - c : 0);
+      gv[k].load_upto(dy + r * a.lddy + c, live ? a.C - c : 0);
+    }
+    const float mean = live ? a.mean[r] : 0.f, rstd = live ? a.rstd[r] : 0.f;
+    float s1 = 0.f, s2 = 0.f;               // sums of w dy and of w dy xh; columns past the end have dy = 0
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float g = (float)gv[k].v[j], xh = ((float)xv[k].v[j] - mean) * rstd;
+        dw[k][j] += g * xh;
+        db[k][j] += g;
+        s1 += g * w[k][j];
+        s2 += g * w[k][j] * xh;
+      }
+    if (!a.out) continue;                   // only the parameters' gradients are wanted
+    const float m1 = row_sum<TPR>(s1, red) * inv_c, m2 = row_sum<TPR>(s2, red) * inv_c;
+    if (!live) continue;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * TPR + lane) * N;
+      Vec16<T> o;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float xh = ((float)xv[k].v[j] - mean) * rstd;
+        o.v[j] = (T)(rstd * ((float)gv[k].v[j] * w[k][j] - m1 - xh * m2));
+      }
+      o.store_upto(dx + r * (long)a.C + c, a.C - c);
+    }
+  }
+  if (!a.partial) return;
+  float* mine = a.partial + (long)blockIdx.x * 2 * a.C;
+  if constexpr (RPB == 1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = (k * TPR + lane) * N + j;
+        if (c < a.C) {
+          mine[c] = dw[k][j];
+          mine[a.C + c] = db[k][j];
+        }
+      }
+  } else {                                  // several rows a workgroup: add its row groups' sums up first
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = (k * TPR + lane) * N + j;
+        cols[(sub * 2 + 0) * kCols + c] = dw[k][j];
+        cols[(sub * 2 + 1) * kCols + c] = db[k][j];
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * kCols; i += block_threads<TPR>()) {
+      const int which = i / kCols, c = i - which * kCols;
+      if (c >= a.C) continue;
+      float s = 0.f;
+#pragma unroll
+      for (int g = 0; g < RPB; ++g) s += cols[(g * 2 + which) * kCols + c];
+      mine[which * (long)a.C + c] = s;
+    }
+  }
+}
+
+template <typename T> __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(LnArgs a) {
+  constexpr int N = Vec16<T>::N;
+  __shared__ float red[16];
+  const float inv_c = 1.f / (float)a.C;
+  for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + r * a.ldx;
+    const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
+    T* dx = static_cast<T*>(a.out) + r * (long)a.C;
+    const float mean = a.mean[r], rstd = a.rstd[r];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
+      Vec16<T> xv, gv;
+      xv.load_upto(x + c, a.C - c);
+      gv.load_upto(dy + c, a.C - c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float w = a.weight && c + j < a.C ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
+        const float g = (float)gv.v[j] * w;
+        s1 += g;
+        s2 += g * ((float)xv.v[j] - mean) * rstd;
+      }
+    }
+    const float m1 = row_sum<1024>(s1, red) * inv_c, m2 = row_sum<1024>(s2, red) * inv_c;
+    for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
+      Vec16<T> xv, gv;
+      xv.load_upto(x + c, a.C - c);
+      gv.load_upto(dy + c, a.C - c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float w = a.weight && c + j < a.C ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
+        const float xh = ((float)xv.v[j] - mean) * rstd;
+        gv.v[j] = (T)(rstd * ((float)gv.v[j] * w - m1 - xh * m2));
+      }
+      gv.store_upto(dx + c, a.C - c);
+    }
+  }
+}
+
+// column sums for the wide rows: workgroup (bx, by) owns 256 vectors of columns and every gridDim.y-th row
+template <typename T> __global__ __launch_bounds__(256) void ln_bwd_wide_cols_kernel(LnArgs a) {
+  constexpr int N = Vec16<T>::N;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * N;
+  if (c >= a.C) return;
+  float dw[N], db[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) dw[j] = db[j] = 0.f;
+  for (long r = blockIdx.y; r < a.rows; r += gridDim.y) {
+    Vec16<T> xv, gv;
+    xv.load_upto(static_cast<const T*>(a.x) + r * a.ldx + c, a.C - c);
+    gv.load_upto(static_cast<const T*>(a.dy) + r * a.lddy + c, a.C - c);
+    const float mean = a.mean[r], rstd = a.rstd[r];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float g = (float)gv.v[j];
+      dw[j] += g * ((float)xv.v[j] - mean) * rstd;
+      db[j] += g;
+    }
+  }
+  float* mine = a.partial + (long)blockIdx.y * 2 * a.C;
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (c + j < a.C) {
+      mine[c + j] = dw[j];
+      mine[a.C + c + j] = db[j];
+    }
+}
+
+// dw and db from the workgroups' partial rows: 32 columns x 32 row lanes a workgroup
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd_finish_kernel(const float* __restrict__ partial, int blocks, int C,
+                                                             void* dweight, void* dbias, int affine_f32) {
+  __shared__ float red[2][32][33];
+  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
+  float s = 0.f, q = 0.f;
+  if (c < C)
+    for (int k = lane; k < blocks; k += 32) {
+      s += partial[(long)k * 2 * C + c];
+      q += partial[(long)k * 2 * C + C + c];
+    }
+  red[0][lane][col] = s;
+  red[1][lane][col] = q;
+  __syncthreads();
+  if (lane >= 2 || c >= C) return;
+  float t = 0.f;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) t += red[lane][k][col];
+  void* out = lane == 0 ? dweight : dbias;
+  if (out) store_param<T>(out, affine_f32, c, t);
+}
+
+// ------------------------------------------------------------------------------------------------------------- launch
+// How a row is laid over threads: the fewest threads that hold it at up to two vectors each (up to 16 columns a thread
+// for workgroup rows).
+template <typename T, typename Fwd> int with_shape(int C, Fwd&& f) {
+  constexpr int N = Vec16<T>::N;
+  const int units = (C + N - 1) / N;
+#define MZ_SHAPE(tpr, nv) if (units <= (tpr) * (nv)) return f(std::integral_constant<int, tpr>{}, std::integral_constant<int, nv>{})
+  MZ_SHAPE(16, 1);
+  MZ_SHAPE(32, 1);
+  MZ_SHAPE(64, 1);
+  MZ_SHAPE(64, 2);
+  MZ_SHAPE(256, 1);
+  MZ_SHAPE(256, 2);
+  if constexpr (N == 4) MZ_SHAPE(256, 4);
+  MZ_SHAPE(512, 16 / N);
+  MZ_SHAPE(1024, 16 / N);
+#undef MZ_SHAPE
+  return -1;
+}
+
+int row_blocks(long rows, int rows_per_block, int cap) {
+  const long want = (rows + rows_per_block - 1) / rows_per_block;
+  return (int)(want < cap ? want : cap);
+}
+
+int bwd_blocks(long rows, int rows_per_block, int threads) {
+  int cap = mz::compute_units() * (threads >= 1024 ? 1 : threads >= 512 ? 2 : 3);
+  if (cap > kMaxPartials) cap = kMaxPartials;
+  return row_blocks(rows, rows_per_block, cap);
+}
+
+template <typename T> int ln_fwd(const LnArgs& a, hipStream_t s) {
+  if (a.C > kMaxRegisterCols) {
+    hipLaunchKernelGGL((ln_fwd_wide_kernel<T>), dim3(row_blocks(a.rows, 1, 4 * mz::compute_units())), dim3(1024), 0, s, a);
+    return MZ_OK;
+  }
+  return with_shape<T>(a.C, [&](auto tpr, auto nv) {
+    constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, NT = block_threads<TPR>();
+    const int blocks = row_blocks(a.rows, NT / TPR, mz::compute_units() * (2048 / NT));
+    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV>), dim3(blocks), dim3(NT), 0, s, a);
+    return MZ_OK;
+  });
+}
+
+template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hipStream_t s) {
+  int blocks = 0;
+  if (a.C > kMaxRegisterCols) {
+    if (a.out)
+      hipLaunchKernelGGL((ln_bwd_wide_kernel<T>), dim3(row_blocks(a.rows, 1, 2 * mz::compute_units())), dim3(1024), 0, s, a);
+    if (a.partial) {
+      constexpr int kCols = 256 * Vec16<T>::N;
+      const int bx = (a.C + kCols - 1) / kCols;
+      int by = (4 * mz::compute_units() + bx - 1) / bx;
+      by = row_blocks(a.rows, 1, by < kMaxPartials ? by : kMaxPartials);
+      blocks = by;
+      hipLaunchKernelGGL((ln_bwd_wide_cols_kernel<T>), dim3(bx, by), dim3(256), 0, s, a);
+    }
+  } else {
+    with_shape<T>(a.C, [&](auto tpr, auto nv) {
+      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, NT = block_threads<TPR>();
+      blocks = bwd_blocks(a.rows, NT / TPR, NT);
+      hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV>), dim3(blocks), dim3(NT), 0, s, a);
+      return MZ_OK;
+    });
+  }
+  if (a.partial)
+    hipLaunchKernelGGL((ln_bwd_finish_kernel<T>), dim3((a.C + 31) / 32), dim3(1024), 0, s, a.partial, blocks, a.C, dweight,
+                       dbias, a.affine_f32);
+  return MZ_OK;
+}
+
+int check(const char* who, int64_t rows, int32_t C, int64_t ld, int32_t dtype, int32_t affine_dtype) {
+  MZ_REQUIRE(rows > 0 && C > 0 && C <= (1 << 24), "%s: rows > 0 and 0 < C <= 2^24 expected (rows = %lld, C = %d)", who,
+             (long long)rows, C);
+  MZ_REQUIRE(ld >= C || rows == 1, "%s: rows overlap (stride %lld < C = %d)", who, (long long)ld, C);
+  MZ_REQUIRE(dtype == MZ_F32 || dtype == MZ_BF16 || dtype == MZ_F16, "%s: unknown element type %d", who, dtype);
+  MZ_REQUIRE(affine_dtype == MZ_F32 || affine_dtype == dtype, "%s: parameters are float32 or of the activations' type", who);
+  return MZ_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mz_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, int32_t affine_dtype, double eps,
+                      int64_t rows, int32_t C, int32_t dtype, void* y, float* mean, float* rstd, mz_stream_t stream) {
+  MZ_REQUIRE(x && y, "mz_layer_norm_fwd: null tensor");
+  MZ_REQUIRE((mean == nullptr) == (rstd == nullptr), "mz_layer_norm_fwd: mean and rstd go together");
+  if (int rc = check("mz_layer_norm_fwd", rows, C, ldx, dtype, affine_dtype)) return rc;
+  MZ_REQUIRE(eps >= 0.0, "mz_layer_norm_fwd: eps must not be negative");
+  const LnArgs a = {x, nullptr, weight, bias, y, mean, rstd, nullptr, ldx, 0, rows, C, affine_dtype == MZ_F32, (float)eps};
+  hipStream_t s = mz::as_stream(stream);
+  if (dtype == MZ_F32) ln_fwd<float>(a, s);
+  else if (dtype == MZ_BF16) ln_fwd<__bf16>(a, s);
+  else ln_fwd<_Float16>(a, s);
+  return mz::check_launch("mz_layer_norm_fwd");
+}
+
+int64_t mz_layer_norm_workspace_bytes(int64_t rows, int32_t C) {
+  if (rows <= 0 || C <= 0) return 0;
+  return (rows < kMaxPartials ? rows : kMaxPartials) * 2 * (int64_t)C * 4;
+}
+
+int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const void* weight, int32_t affine_dtype,
+                      const float* mean, const float* rstd, int64_t rows, int32_t C, int32_t dtype, void* dx, void* dweight,
+                      void* dbias, void* workspace, int64_t workspace_bytes, mz_stream_t stream) {
+  MZ_REQUIRE(x && dy && mean && rstd, "mz_layer_norm_bwd: null tensor");
+  MZ_REQUIRE(dx || dweight || dbias, "mz_layer_norm_bwd: no gradient asked for");
+  if (int rc = check("mz_layer_norm_bwd", rows, C, ldx, dtype, affine_dtype)) return rc;
+  MZ_REQUIRE(lddy >= C || rows == 1, "mz_layer_norm_bwd: rows of dy overlap (stride %lld < C = %d)", (long long)lddy, C);
+  const bool params = dweight || dbias;
+  MZ_REQUIRE(!params || (workspace && workspace_bytes >= mz_layer_norm_workspace_bytes(rows, C)),
+             "mz_layer_norm_bwd: workspace too small");
+  const LnArgs a = {x, dy, weight, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd),
+                    params ? static_cast<float*>(workspace) : nullptr, ldx, lddy, rows, C, affine_dtype == MZ_F32, 0.f};
+  hipStream_t s = mz::as_stream(stream);
+  if (dtype == MZ_F32) ln_bwd<float>(a, dweight, dbias, s);
+  else if (dtype == MZ_BF16) ln_bwd<__bf16>(a, dweight, dbias, s);
+  else ln_bwd<_Float16>(a, dweight, dbias, s);
+  return mz::check_launch("mz_layer_norm_bwd");
+}
+
+}  // extern "C"

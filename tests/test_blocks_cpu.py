@@ -1,0 +1,93 @@
+"""The training-block operators' refusals and size queries, without a GPU: the Python checks raise ValueError before any
+launch, the C ABI returns MZ_E_ARG with a message."""
+import ctypes as C
+
+import pytest
+import torch
+
+from muzero_amd import _lib, blocks
+
+ONE = C.c_void_p(16)      # a non-null, 16-byte aligned address that is never dereferenced
+
+
+def _fails(name, *args, match):
+    with pytest.raises(_lib.MuZeroAmdError, match=match) as e:
+        _lib.call(name, *args)
+    assert name in str(e.value)
+
+
+def test_tensors_have_to_live_on_the_gpu():
+    x, w = torch.zeros(2, 8), torch.zeros(4, 8)
+    for call in (lambda: blocks.layer_norm(x), lambda: blocks.gated_ff(x, w, w),
+                 lambda: blocks.dropout(x, 0.1, torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(ValueError, match="GPU"):
+            call()
+    for call in (lambda: blocks.layer_norm(None), lambda: blocks.dropout([1.0], 0.1, None)):
+        with pytest.raises(ValueError, match="tensor required"):
+            call()
+
+
+def test_layer_norm_entry_points_refuse():
+    fwd = lambda **k: [k.get(n, d) for n, d in dict(x=ONE, ldx=8, w=ONE, b=ONE, affine=0, eps=1e-5, rows=4, c=8, dt=1, y=ONE,  # noqa: E731
+                                                    mean=ONE, rstd=ONE, s=None).items()]
+    _fails("mz_layer_norm_fwd", *fwd(x=None), match="null")
+    _fails("mz_layer_norm_fwd", *fwd(rstd=None), match="go together")
+    _fails("mz_layer_norm_fwd", *fwd(rows=0), match="rows > 0")
+    _fails("mz_layer_norm_fwd", *fwd(c=(1 << 24) + 1, ldx=1 << 25), match="rows > 0")
+    _fails("mz_layer_norm_fwd", *fwd(ldx=7), match="overlap")
+    _fails("mz_layer_norm_fwd", *fwd(dt=3), match="element type")
+    _fails("mz_layer_norm_fwd", *fwd(affine=2), match="parameters")
+    _fails("mz_layer_norm_fwd", *fwd(eps=-1.0), match="eps")
+    _fails("mz_layer_norm_fwd", *fwd(eps=float("nan")), match="eps")
+    bwd = lambda **k: [k.get(n, d) for n, d in dict(x=ONE, ldx=8, dy=ONE, lddy=8, w=ONE, affine=0, mean=ONE, rstd=ONE, rows=4,  # noqa: E731
+                                                    c=8, dt=1, dx=ONE, dw=ONE, db=ONE, ws=ONE, nb=1 << 20, s=None).items()]
+    _fails("mz_layer_norm_bwd", *bwd(mean=None), match="null")
+    _fails("mz_layer_norm_bwd", *bwd(dx=None, dw=None, db=None), match="no gradient")
+    _fails("mz_layer_norm_bwd", *bwd(lddy=4), match="overlap")
+    _fails("mz_layer_norm_bwd", *bwd(nb=4 * 2 * 8 * 4 - 1), match="workspace")
+    _fails("mz_layer_norm_bwd", *bwd(ws=None), match="workspace")
+    lib = _lib.lib()
+    assert lib.mz_layer_norm_workspace_bytes(4, 8) == 4 * 2 * 8 * 4
+    assert lib.mz_layer_norm_workspace_bytes(1 << 20, 8) == 1024 * 2 * 8 * 4
+    assert lib.mz_layer_norm_workspace_bytes(0, 8) == 0
+
+
+def test_gated_ff_entry_points_refuse():
+    fwd = lambda **k: [k.get(n, d) for n, d in dict(x=ONE, ldx=64, wg=ONE, wu=ONE, bg=None, bu=None, m=100, kk=64, f=32, dt=1,  # noqa: E731
+                                                    act=0, h=ONE, ws=None, nb=0, s=None).items()]
+    _fails("mz_gated_ff_fwd", *fwd(wu=None), match="null")
+    _fails("mz_gated_ff_fwd", *fwd(act=4), match="activation")
+    _fails("mz_gated_ff_fwd", *fwd(act=-1), match="activation")
+    _fails("mz_gated_ff_fwd", *fwd(dt=7), match="element type")
+    _fails("mz_gated_ff_fwd", *fwd(m=0), match="out of range")
+    _fails("mz_gated_ff_fwd", *fwd(f=(1 << 20) + 1), match="out of range")
+    _fails("mz_gated_ff_fwd", *fwd(ldx=63), match="stride")
+    _fails("mz_gated_ff_fwd", *fwd(ldx=1 << 22), match="stride")
+    _fails("mz_gated_ff_fwd", *fwd(x=C.c_void_p(18)), match="16 bytes")
+    _fails("mz_gated_ff_fwd", *fwd(ldx=66), match="16 bytes")
+    _fails("mz_gated_ff_fwd", *fwd(kk=63), match="workspace")
+    bwd = lambda **k: [k.get(n, d) for n, d in dict(x=ONE, ldx=64, wg=ONE, wu=ONE, bg=None, bu=None, dh=ONE, m=100, kk=64, f=32,  # noqa: E731
+                                                    dt=1, act=0, dx=ONE, dwg=ONE, dwu=ONE, dbg=None, dbu=None, ws=ONE,
+                                                    nb=1 << 30, s=None).items()]
+    _fails("mz_gated_ff_bwd", *bwd(dh=None), match="null")
+    _fails("mz_gated_ff_bwd", *bwd(dwu=None), match="go together")
+    _fails("mz_gated_ff_bwd", *bwd(dx=None, dwg=None, dwu=None), match="no gradient")
+    need = _lib.lib().mz_gated_ff_workspace_bytes(100, 64, 32, 1, 1)
+    assert need > 2 * 100 * 32 * 2
+    _fails("mz_gated_ff_bwd", *bwd(nb=need - 1), match="workspace")
+    _fails("mz_gated_ff_bwd", *bwd(ws=C.c_void_p(24)), match="16-byte aligned")
+    lib = _lib.lib()
+    assert lib.mz_gated_ff_workspace_bytes(100, 64, 32, 1, 0) == 0
+    assert lib.mz_gated_ff_workspace_bytes(100, 63, 32, 1, 0) >= 2 * 64 * (100 + 2 * 32)
+    assert lib.mz_gated_ff_workspace_bytes(1, 63, 32, 1, 0) == 0
+    assert lib.mz_gated_ff_workspace_bytes(0, 64, 32, 1, 0) == -1
+
+
+def test_dropout_entry_point_refuses():
+    call = lambda **k: [k.get(n, d) for n, d in dict(x=ONE, r=None, y=ONE, n=8, p=0.1, rng=ONE, c=0, dt=0, s=None).items()]  # noqa: E731
+    _fails("mz_dropout", *call(rng=None), match="null")
+    _fails("mz_dropout", *call(n=0), match="elements")
+    _fails("mz_dropout", *call(n=(1 << 35) + 1), match="elements")
+    _fails("mz_dropout", *call(p=1.5), match=r"p in")
+    _fails("mz_dropout", *call(p=float("nan")), match=r"p in")
+    _fails("mz_dropout", *call(dt=3), match="element type")
