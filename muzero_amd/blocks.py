@@ -16,6 +16,7 @@ shapes or devices raise ValueError; there is no CPU path.
 from typing import Optional
 
 import torch
+from torch._C import _cuda_getCurrentRawStream as _raw_stream
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -27,13 +28,45 @@ _MAX_WIDTH = 1 << 20         # input and hidden width of the gated projection
 _MAX_STRIDE_BYTES = 1 << 22  # between rows of its input
 
 
-def _run(device, name, *args):
-    """Call an entry point on the tensors' device and its current stream."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, _lib.C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+# The host's part of a call counts: a small training step is a handful of launches, and its backward pass runs on
+# autograd's own thread, where every Python operation costs several times what it does in a warm loop.  So entry points
+# are looked up once, the stream is read as a plain handle, and nothing is allocated, cast or copied that is there.
+_ENTRIES = {}
+
+
+def _entry(name):
+    f = _ENTRIES[name] = getattr(_lib.lib(), name)
+    return f
+
+
+def _run(index, name, *args):
+    """Call an entry point on device `index` and its current stream."""
+    f = _ENTRIES.get(name) or _entry(name)
+    if torch.cuda.current_device() == index:
+        rc = f(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, _lib.C.c_void_p(torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = f(*args, _raw_stream(index))
+    if rc:
+        _lib.fail(name, rc)
+
+
+def _bytes(name, *args):
+    return (_ENTRIES.get(name) or _entry(name))(*args)
+
+
+def _once(backward):
+    """once_differentiable, whose bookkeeping is only needed where a gradient's gradient may be asked for."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
+def _like(x):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _checked(x, name):
@@ -50,18 +83,15 @@ def _checked(x, name):
 
 
 def _param(t, name, shape, like, dtypes):
-    """A parameter (or None): the given shape, on the activations' device, of one of the types."""
-    if t is None:
-        return None
+    """Refuse a parameter that is not of the given shape, on the activations' device and of one of the types."""
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name}: tensor required")
     if t.device != like.device:
         raise ValueError(f"{name}: on {t.device}, expected {like.device}")
     if t.dtype not in dtypes:
         raise ValueError(f"{name}: dtype {t.dtype}, expected {' or '.join(str(d) for d in dict.fromkeys(dtypes))}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
-    return t
 
 
 def _rows(x):
@@ -76,7 +106,7 @@ def _rows(x):
 
 
 def _contiguous(t):
-    return None if t is None else t.detach().contiguous()
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def _address(t):
@@ -92,12 +122,13 @@ def _layer_norm_forward(x, weight, bias, eps, keep):
     xr, ld = _rows(x)
     c = x.shape[-1]
     rows = x.numel() // c
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
+    y = _like(x)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
     if rows:
+        weight, bias = _contiguous(weight), _contiguous(bias)
         affine = weight if weight is not None else bias
         mean = stats.data_ptr() if keep else None
-        _run(x.device, "mz_layer_norm_fwd", xr.data_ptr(), ld, _address(weight), _address(bias),
+        _run(x.device.index, "mz_layer_norm_fwd", xr.data_ptr(), ld, _address(weight), _address(bias),
              0 if affine is None else _DTYPES[affine.dtype], eps, rows, c, _DTYPES[x.dtype], y.data_ptr(), mean,
              mean + 4 * rows if keep else None)
     return y, stats
@@ -106,30 +137,34 @@ def _layer_norm_forward(x, weight, bias, eps, keep):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = _layer_norm_forward(x, _contiguous(weight), _contiguous(bias), eps, True)
+        y, stats = _layer_norm_forward(x, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.affine = None if weight is None and bias is None else (weight if weight is not None else bias).dtype
+        ctx.affine = torch.float32 if weight is None and bias is None else (weight if weight is not None else bias).dtype
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
-        want_x, want_w, want_b = ctx.needs_input_grad[:3]
+        want_x, want_w, want_b, _ = ctx.needs_input_grad
         c = x.shape[-1]
         rows = x.numel() // c
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
+        device, affine = x.device, ctx.affine
+        dx = _like(x) if want_x else None
         fresh = torch.empty if rows else torch.zeros
-        dw = fresh(c, dtype=ctx.affine, device=x.device) if want_w else None
-        db = fresh(c, dtype=ctx.affine, device=x.device) if want_b else None
+        dw = fresh(c, dtype=affine, device=device) if want_w else None
+        db = fresh(c, dtype=affine, device=device) if want_b else None
         if rows:
-            (xr, ldx), (gr, ldg) = _rows(x), _rows(dy.to(x.dtype))
-            need = _lib.lib().mz_layer_norm_workspace_bytes(rows, c) if want_w or want_b else 0
-            ws = torch.empty(need // 4, dtype=torch.float32, device=x.device) if need else None
+            if dy.dtype != x.dtype:
+                dy = dy.to(x.dtype)
+            (xr, ldx), (gr, ldg) = _rows(x), _rows(dy)
+            need = _bytes("mz_layer_norm_workspace_bytes", rows, c) if want_w or want_b else 0
+            ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+            mean = stats.data_ptr()
             weight = _contiguous(weight)
-            _run(x.device, "mz_layer_norm_bwd", xr.data_ptr(), ldx, gr.data_ptr(), ldg, _address(weight),
-                 0 if ctx.affine is None else _DTYPES[ctx.affine], stats.data_ptr(), stats.data_ptr() + 4 * rows, rows, c,
-                 _DTYPES[x.dtype], _address(dx), _address(dw), _address(db), _address(ws), need)
+            _run(device.index, "mz_layer_norm_bwd", xr.data_ptr(), ldx, gr.data_ptr(), ldg, _address(weight),
+                 _DTYPES[affine], mean, mean + 4 * rows, rows, c, _DTYPES[x.dtype], _address(dx), _address(dw), _address(db),
+                 _address(ws), need)
         return dx, dw, db, None
 
 
@@ -141,13 +176,15 @@ def layer_norm(x, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Te
     _checked(x, "layer_norm: x")
     if x.shape[-1] > _MAX_COLS:
         raise ValueError(f"layer_norm: x: at most {_MAX_COLS} columns")
-    _param(weight, "layer_norm: weight", x.shape[-1:], x, (torch.float32, x.dtype))
-    _param(bias, "layer_norm: bias", x.shape[-1:], x, (torch.float32, x.dtype) if weight is None else (weight.dtype,))
+    if weight is not None:
+        _param(weight, "layer_norm: weight", x.shape[-1:], x, (torch.float32, x.dtype))
+    if bias is not None:
+        _param(bias, "layer_norm: bias", x.shape[-1:], x, (torch.float32, x.dtype) if weight is None else (weight.dtype,))
     if not eps >= 0.0:
         raise ValueError(f"layer_norm: eps {eps}, expected at least 0")
     if _wants_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
-    return _layer_norm_forward(x, _contiguous(weight), _contiguous(bias), float(eps), False)[0]
+    return _layer_norm_forward(x, weight, bias, float(eps), False)[0]
 
 
 # ------------------------------------------------------------------------------------------- gated feed-forward
@@ -157,14 +194,14 @@ def _ff_rows(x):
     xr, ld = _rows(x)
     size = x.element_size()
     aligned = xr.data_ptr() % 16 == 0 and ld * size % 16 == 0
-    if ld * size > _MAX_STRIDE_BYTES or (x.shape[-1] * size % 16 == 0 and not aligned):
+    if ld * size > _MAX_STRIDE_BYTES or (not aligned and x.shape[-1] * size % 16 == 0):
         xr = xr.clone(memory_format=torch.contiguous_format)
         ld = x.shape[-1]
     return xr, ld
 
 
 def _ff_weight(w):
-    w = w.detach().contiguous()
+    w = _contiguous(w)
     return w.clone() if w.data_ptr() % 16 else w
 
 
@@ -176,13 +213,14 @@ def _gated_ff_forward(x, w_gate, w_up, b_gate, b_up, activation):
     xr, ld = _ff_rows(x)
     hidden, k = w_gate.shape
     rows = x.numel() // k
-    h = torch.empty(x.shape[:-1] + (hidden,), dtype=x.dtype, device=x.device)
+    device = x.device
+    h = torch.empty(x.shape[:-1] + (hidden,), dtype=x.dtype, device=device)
     if rows:
         w_gate, w_up, b_gate, b_up = _ff_weight(w_gate), _ff_weight(w_up), _contiguous(b_gate), _contiguous(b_up)
         dt = _DTYPES[x.dtype]
-        need = _lib.lib().mz_gated_ff_workspace_bytes(rows, k, hidden, dt, 0)
-        ws = _workspace(need, x.device)
-        _run(x.device, "mz_gated_ff_fwd", xr.data_ptr(), ld, w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate),
+        need = _bytes("mz_gated_ff_workspace_bytes", rows, k, hidden, dt, 0)
+        ws = _workspace(need, device)
+        _run(device.index, "mz_gated_ff_fwd", xr.data_ptr(), ld, w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate),
              _address(b_up), rows, k, hidden, dt, activation, h.data_ptr(), _address(ws), need)
     return h
 
@@ -195,32 +233,33 @@ class _GatedFF(torch.autograd.Function):
         return _gated_ff_forward(x, w_gate, w_up, b_gate, b_up, activation)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dh):
         x, w_gate, w_up, b_gate, b_up = ctx.saved_tensors
         hidden, k = w_gate.shape
         rows = x.numel() // k
-        want = ctx.needs_input_grad
+        want_x, want_g, want_u, want_bg, want_bu, _ = ctx.needs_input_grad
+        dtype, device = x.dtype, x.device
         make = torch.empty if rows else torch.zeros
-
-        def grad(shape, wanted):
-            return make(shape, dtype=x.dtype, device=x.device) if wanted else None
-
-        dx = grad(x.shape, want[0])
-        both = want[1] or want[2]            # one kernel makes the two weights' gradients
-        dwg, dwu = grad(w_gate.shape, both), grad(w_gate.shape, both)
-        dbg, dbu = grad((hidden,), want[3]), grad((hidden,), want[4])
+        both = want_g or want_u              # one kernel makes the two weights' gradients
+        dx = _like(x) if want_x else None
+        dwg = make((hidden, k), dtype=dtype, device=device) if both else None
+        dwu = make((hidden, k), dtype=dtype, device=device) if both else None
+        dbg = make(hidden, dtype=dtype, device=device) if want_bg else None
+        dbu = make(hidden, dtype=dtype, device=device) if want_bu else None
         if rows:
             xr, ld = _ff_rows(x)
             w_gate, w_up, b_gate, b_up = _ff_weight(w_gate), _ff_weight(w_up), _contiguous(b_gate), _contiguous(b_up)
-            dt = _DTYPES[x.dtype]
-            dh = dh.to(x.dtype).contiguous()
-            need = _lib.lib().mz_gated_ff_workspace_bytes(rows, k, hidden, dt, 1)
-            ws = _workspace(need, x.device)
-            _run(x.device, "mz_gated_ff_bwd", xr.data_ptr(), ld, w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate),
+            dt = _DTYPES[dtype]
+            if dh.dtype != dtype:
+                dh = dh.to(dtype)
+            dh = _contiguous(dh)
+            need = _bytes("mz_gated_ff_workspace_bytes", rows, k, hidden, dt, 1)
+            ws = _workspace(need, device)
+            _run(device.index, "mz_gated_ff_bwd", xr.data_ptr(), ld, w_gate.data_ptr(), w_up.data_ptr(), _address(b_gate),
                  _address(b_up), dh.data_ptr(), rows, k, hidden, dt, ctx.activation, _address(dx), _address(dwg),
                  _address(dwu), _address(dbg), _address(dbu), _address(ws), need)
-        return dx, dwg if want[1] else None, dwu if want[2] else None, dbg, dbu, None
+        return dx, dwg if want_g else None, dwu if want_u else None, dbg, dbu, None
 
 
 def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optional[torch.Tensor] = None,
@@ -245,11 +284,13 @@ def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optio
     hidden, k = w_gate.shape[0], x.shape[-1]
     if k > _MAX_WIDTH or hidden > _MAX_WIDTH:
         raise ValueError(f"gated_ff: widths {k} and {hidden}, expected at most {_MAX_WIDTH}")
-    if w_up is None:
-        raise ValueError("gated_ff: w_up: tensor required")
-    for t, name, shape in ((w_gate, "w_gate", (hidden, k)), (w_up, "w_up", (hidden, k)), (b_gate, "b_gate", (hidden,)),
-                           (b_up, "b_up", (hidden,))):
-        _param(t, f"gated_ff: {name}", shape, x, (x.dtype,))
+    types = (x.dtype,)
+    _param(w_gate, "gated_ff: w_gate", (hidden, k), x, types)
+    _param(w_up, "gated_ff: w_up", (hidden, k), x, types)
+    if b_gate is not None:
+        _param(b_gate, "gated_ff: b_gate", (hidden,), x, types)
+    if b_up is not None:
+        _param(b_up, "gated_ff: b_up", (hidden,), x, types)
     kind = _ACTIVATIONS[activation]
     if _wants_grad(x, w_gate, w_up, b_gate, b_up):
         return _GatedFF.apply(x, w_gate, w_up, b_gate, b_up, kind)
@@ -258,11 +299,11 @@ def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optio
 
 # ---------------------------------------------------------------------------------------------------------- dropout
 def _dropout_forward(x, residual, p, rng, call):
-    x = x.contiguous()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.numel():
-        residual = _contiguous(residual)
-        _run(x.device, "mz_dropout", x.data_ptr(), _address(residual), y.data_ptr(), x.numel(), p, rng.data_ptr(), call,
+    x, residual = _contiguous(x), _contiguous(residual)
+    y = torch.empty_like(x)
+    n = x.numel()
+    if n:
+        _run(x.device.index, "mz_dropout", x.data_ptr(), _address(residual), y.data_ptr(), n, p, rng.data_ptr(), call,
              _DTYPES[x.dtype])
     return y
 
@@ -275,11 +316,12 @@ class _Dropout(torch.autograd.Function):
         return _dropout_forward(x, residual, p, rng, call)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         (rng,) = ctx.saved_tensors
-        dx = _dropout_forward(dy, None, ctx.p, rng, ctx.call) if ctx.needs_input_grad[0] else None
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
+        want_x, want_residual, _, _, _ = ctx.needs_input_grad
+        dx = _dropout_forward(dy, None, ctx.p, rng, ctx.call) if want_x else None
+        return dx, dy if want_residual else None, None, None, None
 
 
 def dropout(x, p: float, rng: torch.Tensor, call: int = 0, residual: Optional[torch.Tensor] = None):
@@ -298,12 +340,11 @@ def dropout(x, p: float, rng: torch.Tensor, call: int = 0, residual: Optional[to
         raise ValueError(f"dropout: p {p}, expected 0 to 1")
     if not 0 <= call < 1 << 32:
         raise ValueError(f"dropout: call {call}, expected 0 to 2^32 - 1")
-    if rng is None:
-        raise ValueError("dropout: rng: tensor required")
     _param(rng, "dropout: rng", (2,), x, (torch.int64,))
     if not rng.is_contiguous():
         raise ValueError("dropout: rng: must be contiguous")
-    _param(residual, "dropout: residual", x.shape, x, (x.dtype,))
+    if residual is not None:
+        _param(residual, "dropout: residual", x.shape, x, (x.dtype,))
     if _wants_grad(x, residual):
         return _Dropout.apply(x, residual, float(p), rng, int(call))
-    return _dropout_forward(x.detach(), residual, float(p), rng, int(call))
+    return _dropout_forward(x, residual, float(p), rng, int(call))

@@ -17,6 +17,8 @@
 #pragma once
 #include "block_common.h"
 
+#include <type_traits>
+
 namespace mz_gff {
 
 enum Mode { kForward = 0, kGateGrad = 1, kInputGrad = 2, kWeightGrad = 3 };
@@ -87,26 +89,33 @@ template <> __device__ __forceinline__ float act_exp<float>(float v) { return ex
 template <typename T> __device__ __forceinline__ float act_rcp(float v) { return __builtin_amdgcn_rcpf(v); }
 template <> __device__ __forceinline__ float act_rcp<float>(float v) { return 1.f / v; }
 
-template <typename T> __device__ __forceinline__ float activate(int kind, float g) {
-  if (kind == mz_gff::kRelu) return g < 0.f ? 0.f : g;      // a NaN stays one
-  if (kind == mz_gff::kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+template <typename T, int KIND> __device__ __forceinline__ float activate(float g) {
+  if constexpr (KIND == mz_gff::kRelu) return g < 0.f ? 0.f : g;      // a NaN stays one
+  if constexpr (KIND == mz_gff::kGelu) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
   const float sig = act_rcp<T>(1.f + act_exp<T>(-g));
-  return kind == mz_gff::kSilu ? g * sig : sig;
+  return KIND == mz_gff::kSilu ? g * sig : sig;
 }
 // act(g) and act'(g)
-template <typename T> __device__ __forceinline__ void activate_grad(int kind, float g, float& act, float& slope) {
-  if (kind == mz_gff::kRelu) {
+template <typename T, int KIND> __device__ __forceinline__ void activate_grad(float g, float& act, float& slope) {
+  if constexpr (KIND == mz_gff::kRelu) {
     act = g < 0.f ? 0.f : g;
     slope = g > 0.f ? 1.f : 0.f;
-  } else if (kind == mz_gff::kGelu) {
+  } else if constexpr (KIND == mz_gff::kGelu) {
     const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     act = g * cdf;
     slope = cdf + g * act_exp<T>(-0.5f * g * g) * 0.39894228040143268f;
   } else {
     const float sig = act_rcp<T>(1.f + act_exp<T>(-g));
-    act = kind == mz_gff::kSilu ? g * sig : sig;
-    slope = kind == mz_gff::kSilu ? sig * (1.f + g * (1.f - sig)) : sig * (1.f - sig);
+    act = KIND == mz_gff::kSilu ? g * sig : sig;
+    slope = KIND == mz_gff::kSilu ? sig * (1.f + g * (1.f - sig)) : sig * (1.f - sig);
   }
+}
+// f(integral constant of the activation): the choice is made once, outside the loops over outputs
+template <typename F> __device__ __forceinline__ void with_activation(int kind, F&& f) {
+  if (kind == mz_gff::kSilu) f(std::integral_constant<int, mz_gff::kSilu>{});
+  else if (kind == mz_gff::kGelu) f(std::integral_constant<int, mz_gff::kGelu>{});
+  else if (kind == mz_gff::kRelu) f(std::integral_constant<int, mz_gff::kRelu>{});
+  else f(std::integral_constant<int, mz_gff::kSigmoid>{});
 }
 
 // four consecutive elements from / to memory; `vec`: all four exist and the address suits one access
@@ -227,7 +236,7 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   constexpr int KS = OpR::KS;
   constexpr int RM = BR / WR / 16, CN = BC / WC / 16;                 // 16 x 16 blocks of a wavefront
   constexpr int TR = kPair ? BR / 2 : BR;                             // output rows (r) of a tile
-  extern __shared__ __attribute__((aligned(16))) char lds[];          // 2 x (BR + BC) x 128 bytes
+  extern __shared__ __attribute__((aligned(16))) char lds[];          // 2 x (BR + BC) x 128 bytes, then biases
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / WC, wc = wave % WC;
@@ -306,14 +315,24 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
     else return wr * RM + i;
   };
 
-  if (first < last) {
-    load_step(first);
-    stage_step(0);
+  if constexpr (kPair) {          // the tile's biases as float32 behind the two buffers: [gate, up][TR]
+    float* bias = reinterpret_cast<float*>(lds + 2 * (BR + BC) * 128);
+    for (int i = tid; i < 2 * TR; i += NT) {
+      const T* b = static_cast<const T*>(a.bias[i / TR]);
+      const long f = r0 + i % TR;
+      bias[i] = b && f < a.nr ? (float)b[f] : 0.f;
+    }
   }
+
+  // Step s computes from one buffer; meanwhile the units of step s + 1, loaded a step ago, go to the other one and those
+  // of step s + 2 are on their way.  No branch in the loop: steps past the end load nothing (every offset is outside) and
+  // stage zeros that nobody reads.
+  load_step(first);
+  stage_step(0);
+  load_step(first + 1);
   __syncthreads();
   int buf = 0;
   for (long s = first; s < last; ++s, buf ^= 1) {
-    if (s + 1 < last) load_step(s + 1);
     const char* rs = lds + buf * ((BR + BC) * 128);
     const char* cs = rs + BR * 128;
 #pragma unroll
@@ -327,8 +346,11 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
 #pragma unroll
         for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf, cf[j], acc[i][j], T{});
       }
+      if (sub == 0) {
+        stage_step(buf ^ 1);
+        load_step(s + 2);
+      }
     }
-    if (s + 1 < last) stage_step(buf ^ 1);
     __syncthreads();
   }
 
@@ -337,62 +359,78 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   if constexpr (kPair) {
     T* out0 = static_cast<T*>(a.out[0]);
     T* out1 = static_cast<T*>(a.out[1]);
-    const bool vec_out = (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
-    const bool vec_dh = (a.lddh & 3) == 0 && ((size_t)a.dh & (4 * sizeof(T) - 1)) == 0;
+    const T* dh = static_cast<const T*>(a.dh);
+    const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
     float* colsum = reinterpret_cast<float*>(lds);                    // kGateGrad: [WC][2][TR]
+    // a tile without ragged edges in tensors that take four elements at a time has no conditions and all its loads in
+    // flight; any other goes element by element
+    bool whole = r0 + TR <= a.nr && c0 + BC <= a.nc && (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
+    if constexpr (MODE == kGateGrad) whole = whole && (a.lddh & 3) == 0 && ((size_t)a.dh & (4 * sizeof(T) - 1)) == 0;
+    auto finish = [&](auto kind, auto is_whole) __attribute__((always_inline)) {
+      constexpr int KIND = decltype(kind)::value;
+      constexpr bool W = decltype(is_whole)::value;
 #pragma unroll
-    for (int i = 0; i < RM / 2; ++i) {
-      const int fr = (wr * (RM / 2) + i) * 16 + lr;                   // feature within the tile
-      const long f = r0 + fr;
-      const int nf = (int)(a.nr - f < 4 ? a.nr - f : 4);              // features that exist (may be <= 0)
-      float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
-      if (a.bias[0]) load4(static_cast<const T*>(a.bias[0]) + f, nf, false, bg);
-      if (a.bias[1]) load4(static_cast<const T*>(a.bias[1]) + f, nf, false, bu);
-      float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < RM / 2; ++i) {
+        const int fr = (wr * (RM / 2) + i) * 16 + lr;                 // feature within the tile
+        const long f = r0 + fr;
+        const int nf = W ? 4 : (int)(a.nr - f < 4 ? a.nr - f : 4);    // features that exist (may be <= 0)
+        const f32x4 bg = *reinterpret_cast<const f32x4*>(bias + fr), bu = *reinterpret_cast<const f32x4*>(bias + TR + fr);
+        float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f}, d[CN][4];
+        if constexpr (MODE == kGateGrad) {
 #pragma unroll
-      for (int j = 0; j < CN; ++j) {
-        const long c = c0 + (wc * CN + j) * 16 + lc;
-        if (c >= a.nc) continue;
-        const f32x4 g = acc[i][j], u = acc[i + RM / 2][j];
-        if constexpr (MODE == kForward) {
-          float o[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) o[q] = activate<T>(a.activation, g[q] + bg[q]) * (u[q] + bu[q]);
-          store4(out0 + c * a.ldo + f, nf, vec_out && nf == 4, o);
-        } else {
-          float d[4], og[4], ou[4];
-          load4(static_cast<const T*>(a.dh) + c * a.lddh + f, nf, vec_dh && nf == 4, d);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float act, slope;
-            activate_grad<T>(a.activation, g[q] + bg[q], act, slope);
-            og[q] = q < nf ? d[q] * (u[q] + bu[q]) * slope : 0.f;
-            ou[q] = q < nf ? d[q] * act : 0.f;
-            sg[q] += og[q];
-            su[q] += ou[q];
+          for (int j = 0; j < CN; ++j) {
+            const long c = c0 + (wc * CN + j) * 16 + lc;
+            load4(dh + c * a.lddh + f, c < a.nc ? nf : 0, W, d[j]);
           }
-          // columns up to nr_pad exist and are read as k of the input gradient: zeros there
-          const int np = (int)(a.nr_pad - f < 4 ? a.nr_pad - f : 4);
-          store4(out0 + c * a.ldo + f, np, np == 4, og);
-          store4(out1 + c * a.ldo + f, np, np == 4, ou);
         }
-      }
-      if constexpr (MODE == kGateGrad) {
-        if (a.col_partial) {       // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            sg[q] = lanes_sum<16>(sg[q]);
-            su[q] = lanes_sum<16>(su[q]);
-          }
-          if (lc == 0)
+        for (int j = 0; j < CN; ++j) {
+          const long c = c0 + (wc * CN + j) * 16 + lc;
+          if (!W && c >= a.nc) continue;
+          const f32x4 g = acc[i][j], u = acc[i + RM / 2][j];
+          if constexpr (MODE == kForward) {
+            float o[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) o[q] = activate<T, KIND>(g[q] + bg[q]) * (u[q] + bu[q]);
+            store4(out0 + c * a.ldo + f, nf, W, o);
+          } else {
+            float og[4], ou[4];
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              colsum[(wc * 2 + 0) * TR + fr + q] = sg[q];
-              colsum[(wc * 2 + 1) * TR + fr + q] = su[q];
+              float act, slope;
+              activate_grad<T, KIND>(g[q] + bg[q], act, slope);
+              og[q] = W || q < nf ? d[j][q] * (u[q] + bu[q]) * slope : 0.f;
+              ou[q] = W || q < nf ? d[j][q] * act : 0.f;
+              sg[q] += og[q];
+              su[q] += ou[q];
             }
+            // columns up to nr_pad exist and are read as k of the input gradient: zeros there
+            const int np = W ? 4 : (int)(a.nr_pad - f < 4 ? a.nr_pad - f : 4);
+            store4(out0 + c * a.ldo + f, np, np == 4, og);
+            store4(out1 + c * a.ldo + f, np, np == 4, ou);
+          }
+        }
+        if constexpr (MODE == kGateGrad) {
+          if (a.col_partial) {     // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              sg[q] = lanes_sum<16>(sg[q]);
+              su[q] = lanes_sum<16>(su[q]);
+            }
+            if (lc == 0)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                colsum[(wc * 2 + 0) * TR + fr + q] = sg[q];
+                colsum[(wc * 2 + 1) * TR + fr + q] = su[q];
+              }
+          }
         }
       }
-    }
+    };
+    with_activation(a.activation, [&](auto kind) __attribute__((always_inline)) {
+      if (whole) finish(kind, std::true_type{});
+      else finish(kind, std::false_type{});
+    });
     if constexpr (MODE == kGateGrad) {
       if (a.col_partial) {
         __syncthreads();
@@ -407,29 +445,35 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
       }
     }
   } else {
-    const bool whole = a.splits == 1;
+    const bool joined = a.splits == 1;
     T* out = static_cast<T*>(a.out[which]);
-    float* part = whole ? nullptr : a.partial + ((long)split * problems + which) * a.nc * a.nr;
-    const bool vec_out = (a.ldo & 3) == 0 && ((size_t)out & (4 * sizeof(T) - 1)) == 0;
-    const bool vec_part = (a.nr & 3) == 0;
+    float* part = joined ? nullptr : a.partial + ((long)split * problems + which) * a.nc * a.nr;
+    const bool inside = r0 + BR <= a.nr && c0 + BC <= a.nc;
+    const bool vec = joined ? (a.ldo & 3) == 0 && ((size_t)out & (4 * sizeof(T) - 1)) == 0 : (a.nr & 3) == 0;
+    auto finish = [&](auto is_whole) __attribute__((always_inline)) {
+      constexpr bool W = decltype(is_whole)::value;
 #pragma unroll
-    for (int i = 0; i < RM; ++i) {
-      const long r = r0 + (wr * RM + i) * 16 + lr;
-      const int n = (int)(a.nr - r < 4 ? a.nr - r : 4);
+      for (int i = 0; i < RM; ++i) {
+        const long r = r0 + (wr * RM + i) * 16 + lr;
+        const int n = W ? 4 : (int)(a.nr - r < 4 ? a.nr - r : 4);
 #pragma unroll
-      for (int j = 0; j < CN; ++j) {
-        const long c = c0 + (wc * CN + j) * 16 + lc;
-        if (c >= a.nc) continue;
-        const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        if (whole) store4(out + c * a.ldo + r, n, vec_out && n == 4, o);
-        else store4(part + c * a.nr + r, n, vec_part && n == 4, o);
+        for (int j = 0; j < CN; ++j) {
+          const long c = c0 + (wc * CN + j) * 16 + lc;
+          if (!W && c >= a.nc) continue;
+          const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+          if (joined) store4(out + c * a.ldo + r, n, W || (vec && n == 4), o);
+          else store4(part + c * a.nr + r, n, W || (vec && n == 4), o);
+        }
       }
-    }
+    };
+    if (inside && vec) finish(std::true_type{});
+    else finish(std::false_type{});
   }
 }
 
 template <typename T, int MODE, int BR, int BC, int WR, int WC> int launch_one(const Args& a, hipStream_t s) {
-  constexpr int TR = MODE <= mz_gff::kGateGrad ? BR / 2 : BR, kLds = 2 * (BR + BC) * 128;
+  constexpr bool kPair = MODE <= mz_gff::kGateGrad;
+  constexpr int TR = kPair ? BR / 2 : BR, kLds = 2 * (BR + BC) * 128 + (kPair ? 2 * TR * 4 : 0);
   static bool done[mz::kMaxDevices] = {false};
   const auto kernel = gff_gemm_kernel<T, MODE, BR, BC, WR, WC>;
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
@@ -517,21 +561,24 @@ template <typename T, int CN> __global__ __launch_bounds__(256) void gff_few_ker
   if (a.bias[0]) load4(static_cast<const T*>(a.bias[0]) + f, nf, false, bg);
   if (a.bias[1]) load4(static_cast<const T*>(a.bias[1]) + f, nf, false, bu);
   const bool vec = nf == 4 && (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
+  with_activation(a.activation, [&](auto kind) __attribute__((always_inline)) {
+    constexpr int KIND = decltype(kind)::value;
 #pragma unroll
-  for (int j = 0; j < CN; ++j) {
-    f32x4 s0 = acc[0][j], s1 = acc[1][j];
+    for (int j = 0; j < CN; ++j) {
+      f32x4 s0 = acc[0][j], s1 = acc[1][j];
 #pragma unroll
-    for (int w = 0; w < 3; ++w) {
-      s0 += red[w][0][j][lane];
-      s1 += red[w][1][j][lane];
+      for (int w = 0; w < 3; ++w) {
+        s0 += red[w][0][j][lane];
+        s1 += red[w][1][j][lane];
+      }
+      const long c = j * 16 + l;
+      if (c >= a.nc) continue;
+      float o[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = activate<T, KIND>(s0[q] + bg[q]) * (s1[q] + bu[q]);
+      store4(static_cast<T*>(a.out[0]) + c * a.ldo + f, nf, vec, o);
     }
-    const long c = j * 16 + l;
-    if (c >= a.nc) continue;
-    float o[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = activate<T>(a.activation, s0[q] + bg[q]) * (s1[q] + bu[q]);
-    store4(static_cast<T*>(a.out[0]) + c * a.ldo + f, nf, vec, o);
-  }
+  });
 }
 
 template <typename T> int launch_few(const Args& a, hipStream_t s) {

@@ -61,13 +61,10 @@ __global__ __launch_bounds__(block_threads<TPR>()) void ln_fwd_kernel(LnArgs a) 
   const float inv_c = 1.f / (float)a.C;
   float w[NV][N], b[NV][N];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (k * TPR + lane) * N + j;
-      w[k][j] = a.weight && c < a.C ? load_param<T>(a.weight, a.affine_f32, c) : 1.f;
-      b[k][j] = a.bias && c < a.C ? load_param<T>(a.bias, a.affine_f32, c) : 0.f;
-    }
+  for (int k = 0; k < NV; ++k) {
+    load_params<T, N>(a.weight, a.affine_f32, (k * TPR + lane) * N, a.C, 1.f, w[k]);
+    load_params<T, N>(a.bias, a.affine_f32, (k * TPR + lane) * N, a.C, 0.f, b[k]);
+  }
   for (long r0 = (long)blockIdx.x * RPB; r0 < a.rows; r0 += (long)gridDim.x * RPB) {
     const long r = r0 + sub;
     const bool live = r < a.rows;           // TPR > 64: one row a workgroup, always live
@@ -168,13 +165,11 @@ __global__ __launch_bounds__(block_threads<TPR>()) void ln_bwd_kernel(LnArgs a) 
   const float inv_c = 1.f / (float)a.C;
   float w[NV][N], dw[NV][N], db[NV][N];
 #pragma unroll
-  for (int k = 0; k < NV; ++k)
+  for (int k = 0; k < NV; ++k) {
+    load_params<T, N>(a.weight, a.affine_f32, (k * TPR + lane) * N, a.C, 1.f, w[k]);
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = (k * TPR + lane) * N + j;
-      w[k][j] = a.weight && c < a.C ? load_param<T>(a.weight, a.affine_f32, c) : 1.f;
-      dw[k][j] = db[k][j] = 0.f;
-    }
+    for (int j = 0; j < N; ++j) dw[k][j] = db[k][j] = 0.f;
+  }
   for (long r0 = (long)blockIdx.x * RPB; r0 < a.rows; r0 += (long)gridDim.x * RPB) {
     const long r = r0 + sub;
     const bool live = r < a.rows;
@@ -321,9 +316,19 @@ __global__ __launch_bounds__(1024) void ln_bwd_finish_kernel(const float* __rest
   const int col = threadIdx.x & 31, lane = threadIdx.x >> 5, c = blockIdx.x * 32 + col;
   float s = 0.f, q = 0.f;
   if (c < C)
-    for (int k = lane; k < blocks; k += 32) {
-      s += partial[(long)k * 2 * C + c];
-      q += partial[(long)k * 2 * C + C + c];
+    for (int k0 = lane; k0 < blocks; k0 += 32 * 4) {      // eight loads in flight
+      float t[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + 32 * i;
+        t[0][i] = k < blocks ? partial[(long)k * 2 * C + c] : 0.f;
+        t[1][i] = k < blocks ? partial[(long)k * 2 * C + C + c] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s += t[0][i];
+        q += t[1][i];
+      }
     }
   red[0][lane][col] = s;
   red[1][lane][col] = q;
@@ -356,15 +361,22 @@ template <typename T, typename Fwd> int with_shape(int C, Fwd&& f) {
   return -1;
 }
 
+// workgroups for `rows`: as many as `cap`, fewer where that gives all of them the same number of rounds
 int row_blocks(long rows, int rows_per_block, int cap) {
-  const long want = (rows + rows_per_block - 1) / rows_per_block;
-  return (int)(want < cap ? want : cap);
+  const long groups = (rows + rows_per_block - 1) / rows_per_block, rounds = (groups + cap - 1) / cap;
+  return (int)((groups + rounds - 1) / rounds);
 }
 
+// Workgroups of the backward pass.  Each leaves 8 C bytes of partial sums that are written and read once more, so it
+// should walk at least eight rows (at 2000 x 8192 bf16: 34 us, with four rows 45 us), as long as every compute unit
+// has one (500 x 2048: 10.5 us with one each, 12.4 with one in four).
 int bwd_blocks(long rows, int rows_per_block, int threads) {
-  int cap = mz::compute_units() * (threads >= 1024 ? 1 : threads >= 512 ? 2 : 3);
+  const int cus = mz::compute_units();
+  long cap = threads >= 512 ? cus : 3 * cus;
+  const long few = rows / 8 > cus ? rows / 8 : cus;
+  if (cap > few) cap = few;
   if (cap > kMaxPartials) cap = kMaxPartials;
-  return row_blocks(rows, rows_per_block, cap);
+  return row_blocks(rows, rows_per_block, (int)cap);
 }
 
 template <typename T> int ln_fwd(const LnArgs& a, hipStream_t s) {
@@ -374,7 +386,7 @@ template <typename T> int ln_fwd(const LnArgs& a, hipStream_t s) {
   }
   return with_shape<T>(a.C, [&](auto tpr, auto nv) {
     constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, NT = block_threads<TPR>();
-    const int blocks = row_blocks(a.rows, NT / TPR, mz::compute_units() * (2048 / NT));
+    const int blocks = row_blocks(a.rows, NT / TPR, mz::compute_units() * 1024 / NT);
     hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV>), dim3(blocks), dim3(NT), 0, s, a);
     return MZ_OK;
   });
