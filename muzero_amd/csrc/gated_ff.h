@@ -150,6 +150,7 @@ template <typename T, bool ACROSS, int B, int NT> struct Operand {
   static constexpr int KS = 128 / (int)sizeof(T);       // k of a step
   static constexpr int UNITS = B * 8 / NT;              // 16-byte units a thread moves per step
   static constexpr int UPR = ACROSS ? B / EC : 8;       // units of a staged row
+  static constexpr int READS = !ACROSS ? 1 : sizeof(T) == 2 ? 2 : 4;   // LDS reads of a fragment
   static_assert(B * 8 % NT == 0 && NT % UPR == 0, "whole rows per round of threads");
   static constexpr int RPR = NT / UPR;                  // staged rows a round covers
   unsigned off[UNITS];                                  // byte offset from the step's origin
@@ -180,21 +181,15 @@ template <typename T, bool ACROSS, int B, int NT> struct Operand {
       else off[i] = row < rows_left ? (unsigned)(row * ld * (long)sizeof(T) + unit * 16) : kOutside;
     }
   }
-  // origin: the matrix element of (tile row 0, k = k0); k_left = nk - k0 > 0
-  __device__ __forceinline__ void load(const T* origin, long k_left, u32x4 (&v)[UNITS]) const {
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(origin), 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-      const bool inside = ACROSS ? row0 + i * RPR < k_left : (long)unit * EC < k_left;
-      v[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(inside ? off[i] : kOutside), 0, 0));
-    }
+  // unit i of the step whose origin - the matrix element of (tile row 0, k = k0) - `rs` starts at; k_left: how many of the
+  // step's k exist
+  __device__ __forceinline__ u32x4 load(__amdgpu_buffer_rsrc_t rs, int k_left, int i) const {
+    const bool inside = ACROSS ? row0 + i * RPR < k_left : unit * EC < k_left;
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)(inside ? off[i] : kOutside), 0, 0));
   }
-  __device__ __forceinline__ void stage(char* lds, const u32x4 (&v)[UNITS]) const {
-#pragma unroll
-    for (int i = 0; i < UNITS; ++i) {
-      const int row = row0 + i * RPR;
-      *reinterpret_cast<u32x4*>(lds + row * (UPR * 16) + place(row, unit) * 16) = v[i];
-    }
+  __device__ __forceinline__ void stage(char* lds, int i, u32x4 v) const {
+    const int row = row0 + i * RPR;
+    *reinterpret_cast<u32x4*>(lds + row * (UPR * 16) + place(row, unit) * 16) = v;
   }
   // lane's 16 bytes of block `blk` (rows 16 blk ..) at sub-step `sub` of the step's two
   static __device__ __forceinline__ u32x4 fragment(const char* lds, int blk, int sub, int lane) {
@@ -224,6 +219,26 @@ template <typename T, bool ACROSS, int B, int NT> struct Operand {
     }
   }
 };
+
+// How many of n things fall to the i-th of `parts` turns: turn i takes [i n / parts, (i + 1) n / parts).
+constexpr int turn_begin(int i, int n, int parts) { return i * n / parts; }
+constexpr int turn_count(int i, int n, int parts) { return (i + 1) * n / parts - i * n / parts; }
+// The order of a half step's instructions, which is the order they are written in: per 16-row block of R its matrix
+// instructions, then that turn's LDS reads, LDS writes and loads.  (Left to itself the compiler moves the reads to right
+// before their use and waits for each.)
+template <int I, int BLOCKS, int MMAS, int R_READS, int C_BLOCKS, int C_READS, int UNITS>
+__device__ __forceinline__ void half_step_order() {
+  if constexpr (I < BLOCKS) {
+    constexpr int units = turn_count(I, UNITS, BLOCKS);
+    __builtin_amdgcn_sched_group_barrier(0x008, MMAS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R_READS + C_READS * turn_count(I, C_BLOCKS, BLOCKS), 0);
+    if constexpr (units > 0) {
+      __builtin_amdgcn_sched_group_barrier(0x200, units, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, units, 0);
+    }
+    half_step_order<I + 1, BLOCKS, MMAS, R_READS, C_BLOCKS, C_READS, UNITS>();
+  }
+}
 
 template <typename T, int MODE, int BR, int BC, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) void gff_gemm_kernel(Args a) {
@@ -275,33 +290,35 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   const long first = (long)split * a.steps_per_split;
   const long last = first + a.steps_per_split < all_steps ? first + a.steps_per_split : all_steps;
 
-  u32x4 rv[OpR::UNITS], cv[OpC::UNITS];
-  auto load_step = [&](long s) {
-    const int seg = MODE == kInputGrad && s >= seg_steps ? 1 : 0;
-    const long k0 = (s - seg * seg_steps) * KS, k_left = a.nk - k0;
-    if constexpr (kPair) {
-      u32x4 half[kHalf];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const T* origin = static_cast<const T*>(a.r[h]) + r0 * a.ldr + k0;
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(origin), 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-          half[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-              rs, (int)((long)opr.unit * OpR::EC < k_left ? opr.off[i] : kOutside), 0, 0));
-#pragma unroll
-        for (int i = 0; i < kHalf; ++i) rv[h * kHalf + i] = half[i];
-      }
-    } else {
-      opr.load(static_cast<const T*>(a.r[seg]) + k0 * a.ldr + r0, k_left, rv);
-    }
-    const T* cm = static_cast<const T*>(a.c[MODE == kWeightGrad ? which : seg]);
-    opc.load(kCAcross ? cm + k0 * a.ldc + c0 : cm + c0 * a.ldc + k0, k_left, cv);
+  // a step's units, R's and then C's, travel in v; unit u of step s is loaded from source(s) and staged in a buffer
+  constexpr int kUnits = OpR::UNITS + OpC::UNITS;
+  u32x4 v[kUnits];
+  struct Source {
+    __amdgpu_buffer_rsrc_t r[2], c;
+    int k_left;
   };
-  auto stage_step = [&](int buf) {
+  auto source = [&](long s) __attribute__((always_inline)) {
+    const int seg = MODE == kInputGrad && s >= seg_steps ? 1 : 0;
+    const long k0 = (s - seg * seg_steps) * KS, left = a.nk - k0;
+    const T* cm = static_cast<const T*>(a.c[MODE == kWeightGrad ? which : seg]);
+    const T* rm0 = static_cast<const T*>(a.r[seg]);
+    const T* rm1 = static_cast<const T*>(a.r[kPair ? 1 : seg]);
+    const long ro = kPair ? r0 * a.ldr + k0 : k0 * a.ldr + r0, co = kCAcross ? k0 * a.ldc + c0 : c0 * a.ldc + k0;
+    Source src;
+    src.r[0] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(rm0) + ro, 0, 0x7fffffff, 0x00020000);
+    src.r[1] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(rm1) + ro, 0, 0x7fffffff, 0x00020000);
+    src.c = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(cm) + co, 0, 0x7fffffff, 0x00020000);
+    src.k_left = left < 0 ? 0 : left < KS ? (int)left : KS;
+    return src;
+  };
+  auto load_unit = [&](const Source& src, int u) __attribute__((always_inline)) {
+    if (u < OpR::UNITS) v[u] = opr.load(src.r[kPair && u >= kHalf ? 1 : 0], src.k_left, u);
+    else v[u] = opc.load(src.c, src.k_left, u - OpR::UNITS);
+  };
+  auto stage_unit = [&](int buf, int u) __attribute__((always_inline)) {
     char* base = lds + buf * ((BR + BC) * 128);
-    opr.stage(base, rv);
-    opc.stage(base + BR * 128, cv);
+    if (u < OpR::UNITS) opr.stage(base, u, v[u]);
+    else opc.stage(base + BR * 128, u - OpR::UNITS, v[u]);
   };
 
   f32x4 acc[RM][CN];
@@ -324,35 +341,59 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
     }
   }
 
-  // Step s computes from one buffer; meanwhile the units of step s + 1, loaded a step ago, go to the other one and those
-  // of step s + 2 are on their way.  No branch in the loop: steps past the end load nothing (every offset is outside) and
-  // stage zeros that nobody reads.
-  load_step(first);
-  stage_step(0);
-  load_step(first + 1);
+  // A step has two halves, 64 bytes of k each, whose operands are in registers when they begin: while the first half's
+  // matrix instructions run, the second half's operands are read from LDS, the next step's units (loaded a step ago) are
+  // staged in the other buffer and the ones after that are sent for; then the barrier; while the second half runs, the
+  // next step's first operands are read.  No branch in the loop: steps past the end load nothing (every offset is
+  // outside) and stage zeros.
+  constexpr int kMmas = sizeof(T) == 4 ? 4 : 1;
+  u32x4 rf[RM], cf[2][CN];
+  {
+    const Source src = source(first), after = source(first + 1);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) load_unit(src, u);
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      stage_unit(0, u);
+      load_unit(after, u);
+    }
+  }
   __syncthreads();
+#pragma unroll
+  for (int j = 0; j < CN; ++j) cf[0][j] = OpC::fragment(lds + BR * 128, wc * CN + j, 0, lane);
+#pragma unroll
+  for (int i = 0; i < RM; ++i) rf[i] = OpR::fragment(lds, r_block(i), 0, lane);
   int buf = 0;
   for (long s = first; s < last; ++s, buf ^= 1) {
-    const char* rs = lds + buf * ((BR + BC) * 128);
-    const char* cs = rs + BR * 128;
+    const char* here = lds + buf * ((BR + BC) * 128);
+    const char* next = lds + (buf ^ 1) * ((BR + BC) * 128);
+    const Source after = source(s + 2);
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-      u32x4 cf[CN];
+    for (int i = 0; i < RM; ++i) {
 #pragma unroll
-      for (int j = 0; j < CN; ++j) cf[j] = OpC::fragment(cs, wc * CN + j, sub, lane);
+      for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
 #pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        const u32x4 rf = OpR::fragment(rs, r_block(i), sub, lane);
+      for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[1][j] = OpC::fragment(here + BR * 128, wc * CN + j, 1, lane);
+      rf[i] = OpR::fragment(here, r_block(i), 1, lane);
 #pragma unroll
-        for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf, cf[j], acc[i][j], T{});
-      }
-      if (sub == 0) {
-        stage_step(buf ^ 1);
-        load_step(s + 2);
+      for (int u = turn_begin(i, kUnits, RM); u < turn_begin(i + 1, kUnits, RM); ++u) {
+        stage_unit(buf ^ 1, u);
+        load_unit(after, u);
       }
     }
+    half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, kUnits>();
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+#pragma unroll
+      for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[1][j], acc[i][j], T{});
+#pragma unroll
+      for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[0][j] = OpC::fragment(next + BR * 128, wc * CN + j, 0, lane);
+      rf[i] = OpR::fragment(next, r_block(i), 0, lane);
+    }
+    half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, 0>();
   }
+  __syncthreads();               // the epilogue uses the buffers
 
   // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
   const int lr = (lane >> 4) * 4, lc = lane & 15;
