@@ -41,7 +41,7 @@ struct Args {
   int activation, splits, steps_per_split;
 };
 
-// launchers, one translation unit per element type; tile: 0 = 256 x 256, 1 = 128 x 128, 2 = 64 x 64
+// launchers, one translation unit per element type; tile: 0 = 256 x 256 (16-bit types), 1 = 128 x 128, 2 = 64 x 64
 int launch_bf16(const Args& a, int mode, int tile, hipStream_t s);
 int launch_f16(const Args& a, int mode, int tile, hipStream_t s);
 int launch_f32(const Args& a, int mode, int tile, hipStream_t s);
@@ -110,8 +110,11 @@ template <typename T, int KIND> __device__ __forceinline__ void activate_grad(fl
     slope = KIND == mz_gff::kSilu ? sig * (1.f + g * (1.f - sig)) : sig * (1.f - sig);
   }
 }
-// f(integral constant of the activation): the choice is made once, outside the loops over outputs
-template <typename F> __device__ __forceinline__ void with_activation(int kind, F&& f) {
+// f(integral constant of the activation): the choice is made once, outside the loops over outputs.  FIXED >= 0: it is
+// that one (the kernels whose registers four copies of the epilogue in one function would cost).
+constexpr int kAnyActivation = -1;
+template <int FIXED, typename F> __device__ __forceinline__ void with_activation(int kind, F&& f) {
+  if constexpr (FIXED != kAnyActivation) return f(std::integral_constant<int, FIXED>{});
   if (kind == mz_gff::kSilu) f(std::integral_constant<int, mz_gff::kSilu>{});
   else if (kind == mz_gff::kGelu) f(std::integral_constant<int, mz_gff::kGelu>{});
   else if (kind == mz_gff::kRelu) f(std::integral_constant<int, mz_gff::kRelu>{});
@@ -240,7 +243,7 @@ __device__ __forceinline__ void half_step_order() {
   }
 }
 
-template <typename T, int MODE, int BR, int BC, int WR, int WC>
+template <typename T, int MODE, int BR, int BC, int WR, int WC, int ACT>
 __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) void gff_gemm_kernel(Args a) {
   using namespace mz_gff;
   constexpr int NT = WR * WC * 64;
@@ -363,11 +366,17 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   for (int j = 0; j < CN; ++j) cf[0][j] = OpC::fragment(lds + BR * 128, wc * CN + j, 0, lane);
 #pragma unroll
   for (int i = 0; i < RM; ++i) rf[i] = OpR::fragment(lds, r_block(i), 0, lane);
-  int buf = 0;
-  for (long s = first; s < last; ++s, buf ^= 1) {
-    const char* here = lds + buf * ((BR + BC) * 128);
-    const char* next = lds + (buf ^ 1) * ((BR + BC) * 128);
-    const Source after = source(s + 2);
+  // The epilogue goes over the tile in CN passes, each one 16-token block of every wavefront: values pass through LDS so
+  // that memory is read and written in whole 16-byte units of consecutive features, whatever the rows' alignment.
+  constexpr int PR = WC * 16;                                          // tokens of a pass
+  auto pass_row = [&](int q, int j) { return ((q >> 4) * CN + j) * 16 + (q & 15); };   // of the tile, for row q of pass j
+  const int lr = (lane >> 4) * 4, lc = lane & 15;
+  constexpr int EU = TR / OpR::EC, PU = (PR * EU + NT - 1) / NT;       // units of a pass's row; units a thread moves
+  // the last step has nothing to stage or to read ahead
+  auto step = [&](const char* here, const char* next, int next_buf, long s, auto is_last) __attribute__((always_inline)) {
+    constexpr bool LAST = decltype(is_last)::value;
+    Source after;
+    if constexpr (!LAST) after = source(s + 2);
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
 #pragma unroll
@@ -375,158 +384,220 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
 #pragma unroll
       for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[1][j] = OpC::fragment(here + BR * 128, wc * CN + j, 1, lane);
       rf[i] = OpR::fragment(here, r_block(i), 1, lane);
+      if constexpr (!LAST) {
 #pragma unroll
-      for (int u = turn_begin(i, kUnits, RM); u < turn_begin(i + 1, kUnits, RM); ++u) {
-        stage_unit(buf ^ 1, u);
-        load_unit(after, u);
+        for (int u = turn_begin(i, kUnits, RM); u < turn_begin(i + 1, kUnits, RM); ++u) {
+          stage_unit(next_buf, u);
+          load_unit(after, u);
+        }
       }
     }
-    half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, kUnits>();
+    half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, LAST ? 0 : kUnits>();
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
 #pragma unroll
       for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[1][j], acc[i][j], T{});
+      if constexpr (!LAST) {
 #pragma unroll
-      for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[0][j] = OpC::fragment(next + BR * 128, wc * CN + j, 0, lane);
-      rf[i] = OpR::fragment(next, r_block(i), 0, lane);
+        for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[0][j] = OpC::fragment(next + BR * 128, wc * CN + j, 0, lane);
+        rf[i] = OpR::fragment(next, r_block(i), 0, lane);
+      }
     }
-    half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, 0>();
-  }
+    if constexpr (!LAST) half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, 0>();
+  };
+  int buf = 0;
+  for (long s = first; s + 1 < last; ++s, buf ^= 1)
+    step(lds + buf * ((BR + BC) * 128), lds + (buf ^ 1) * ((BR + BC) * 128), buf ^ 1, s, std::false_type{});
+  if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
   __syncthreads();               // the epilogue uses the buffers
+  __builtin_amdgcn_sched_barrier(0);                                  // and none of its registers before
 
   // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
-  const int lr = (lane >> 4) * 4, lc = lane & 15;
   if constexpr (kPair) {
-    T* out0 = static_cast<T*>(a.out[0]);
-    T* out1 = static_cast<T*>(a.out[1]);
-    const T* dh = static_cast<const T*>(a.dh);
-    const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
-    float* colsum = reinterpret_cast<float*>(lds);                    // kGateGrad: [WC][2][TR]
-    // a tile without ragged edges in tensors that take four elements at a time has no conditions and all its loads in
-    // flight; any other goes element by element
-    bool whole = r0 + TR <= a.nr && c0 + BC <= a.nc && (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
-    if constexpr (MODE == kGateGrad) whole = whole && (a.lddh & 3) == 0 && ((size_t)a.dh & (4 * sizeof(T) - 1)) == 0;
-    auto finish = [&](auto kind, auto is_whole) __attribute__((always_inline)) {
-      constexpr int KIND = decltype(kind)::value;
-      constexpr bool W = decltype(is_whole)::value;
+    constexpr int kPitch = TR * (int)sizeof(T) + 16, kRegion = PR * kPitch;
+    // kGateGrad: the tile of dh, sent for as a whole where it has no ragged edge (16-bit types: 32 registers)
+    constexpr bool kDhAhead = MODE == kGateGrad && sizeof(T) == 2;
+    const bool full = r0 + TR <= a.nr && c0 + BC <= a.nc;
+    Vec16<T> dh_unit[kDhAhead ? CN : 1][PU];
+    if (kDhAhead && full) {
 #pragma unroll
-      for (int i = 0; i < RM / 2; ++i) {
-        const int fr = (wr * (RM / 2) + i) * 16 + lr;                 // feature within the tile
-        const long f = r0 + fr;
-        const int nf = W ? 4 : (int)(a.nr - f < 4 ? a.nr - f : 4);    // features that exist (may be <= 0)
-        const f32x4 bg = *reinterpret_cast<const f32x4*>(bias + fr), bu = *reinterpret_cast<const f32x4*>(bias + TR + fr);
-        float sg[4] = {0.f, 0.f, 0.f, 0.f}, su[4] = {0.f, 0.f, 0.f, 0.f}, d[CN][4];
-        if constexpr (MODE == kGateGrad) {
+      for (int j = 0; j < CN; ++j)
 #pragma unroll
-          for (int j = 0; j < CN; ++j) {
-            const long c = c0 + (wc * CN + j) * 16 + lc;
-            load4(dh + c * a.lddh + f, c < a.nc ? nf : 0, W, d[j]);
-          }
+        for (int n = 0; n < PU; ++n) {
+          const int e = tid + n * NT < PR * EU ? tid + n * NT : 0;
+          dh_unit[kDhAhead ? j : 0][n].load(static_cast<const T*>(a.dh) + (c0 + pass_row(e / EU, j)) * a.lddh + r0 + e % EU * OpR::EC);
         }
+    }
+    const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
+    float* colsum = reinterpret_cast<float*>(lds + 3 * kRegion);      // kGateGrad: [WC][2][TR]
+    const int my_row = (wc * 16 + lc) * kPitch;                       // of a pass's region
+    const long limit = (MODE == kGateGrad ? a.nr_pad : a.nr) - r0;    // columns of the outputs from r0 on
+    with_activation<ACT>(a.activation, [&](auto kind) __attribute__((always_inline)) {
+      constexpr int KIND = decltype(kind)::value;
+      float sg[RM / 2][4], su[RM / 2][4];
 #pragma unroll
-        for (int j = 0; j < CN; ++j) {
-          const long c = c0 + (wc * CN + j) * 16 + lc;
-          if (!W && c >= a.nc) continue;
-          const f32x4 g = acc[i][j], u = acc[i + RM / 2][j];
-          if constexpr (MODE == kForward) {
-            float o[4];
+      for (int i = 0; i < RM / 2; ++i)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) o[q] = activate<T, KIND>(g[q] + bg[q]) * (u[q] + bu[q]);
-            store4(out0 + c * a.ldo + f, nf, W, o);
+        for (int q = 0; q < 4; ++q) sg[i][q] = su[i][q] = 0.f;
+#pragma unroll
+      for (int j = 0; j < CN; ++j) {
+        char* region = lds + (MODE == kForward ? j & 1 : 1) * kRegion;  // kGateGrad: dh, dg, du
+        if constexpr (MODE == kGateGrad) {
+          if (kDhAhead && full) {
+#pragma unroll
+            for (int n = 0; n < PU; ++n) {
+              const int e = tid + n * NT;
+              if (e < PR * EU) dh_unit[kDhAhead ? j : 0][n].store(reinterpret_cast<T*>(lds + e / EU * kPitch + e % EU * 16));
+            }
           } else {
-            float og[4], ou[4];
+#pragma unroll 1
+            for (int e = tid; e < PR * EU; e += NT) {
+              const int q = e / EU, f = e % EU * OpR::EC;
+              const long c = c0 + pass_row(q, j);
+              Vec16<T> d;
+              d.load_upto(static_cast<const T*>(a.dh) + c * a.lddh + r0 + f, c < a.nc ? a.nr - r0 - f : 0);
+              d.store(reinterpret_cast<T*>(lds + q * kPitch + f * (int)sizeof(T)));
+            }
+          }
+          __syncthreads();
+        }
+        const bool token = c0 + pass_row(wc * 16 + lc, j) < a.nc;
+#pragma unroll
+        for (int i = 0; i < RM / 2; ++i) {
+          const int fr = (wr * (RM / 2) + i) * 16 + lr;               // feature within the tile
+          const f32x4 g = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + fr);
+          const f32x4 u = acc[i + RM / 2][j] + *reinterpret_cast<const f32x4*>(bias + TR + fr);
+          vec4<T> o0, o1;
+          if constexpr (MODE == kForward) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) o0[q] = (T)(activate<T, KIND>(g[q]) * u[q]);
+          } else {
+            const vec4<T> d = *reinterpret_cast<const vec4<T>*>(lds + my_row + fr * (int)sizeof(T));
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               float act, slope;
-              activate_grad<T, KIND>(g[q] + bg[q], act, slope);
-              og[q] = W || q < nf ? d[j][q] * (u[q] + bu[q]) * slope : 0.f;
-              ou[q] = W || q < nf ? d[j][q] * act : 0.f;
-              sg[q] += og[q];
-              su[q] += ou[q];
+              activate_grad<T, KIND>(g[q], act, slope);
+              // what lies past the last token or feature counts as zero, also as k of the input gradient (nr .. nr_pad)
+              const bool exists = token && r0 + fr + q < a.nr;
+              const float dg = exists ? (float)d[q] * u[q] * slope : 0.f, du = exists ? (float)d[q] * act : 0.f;
+              sg[i][q] += dg;
+              su[i][q] += du;
+              o0[q] = (T)dg;
+              o1[q] = (T)du;
             }
-            // columns up to nr_pad exist and are read as k of the input gradient: zeros there
-            const int np = W ? 4 : (int)(a.nr_pad - f < 4 ? a.nr_pad - f : 4);
-            store4(out0 + c * a.ldo + f, np, np == 4, og);
-            store4(out1 + c * a.ldo + f, np, np == 4, ou);
+            *reinterpret_cast<vec4<T>*>(region + kRegion + my_row + fr * (int)sizeof(T)) = o1;
+          }
+          *reinterpret_cast<vec4<T>*>(region + my_row + fr * (int)sizeof(T)) = o0;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < PU; ++n) {
+          const int e = tid + n * NT, q = e / EU, f = e % EU * OpR::EC;
+          const long c = c0 + pass_row(q, j), left = limit - f;
+          if (q >= PR || c >= a.nc || left <= 0) continue;
+#pragma unroll
+          for (int w = 0; w < (MODE == kGateGrad ? 2 : 1); ++w) {
+            Vec16<T> o;
+            o.load(reinterpret_cast<const T*>(region + w * kRegion + q * kPitch + f * (int)sizeof(T)));
+            o.store_upto(static_cast<T*>(a.out[w]) + c * a.ldo + r0 + f, left);
           }
         }
-        if constexpr (MODE == kGateGrad) {
-          if (a.col_partial) {     // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
+      }
+      if constexpr (MODE == kGateGrad) {
+        if (a.col_partial) {       // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
+#pragma unroll
+          for (int i = 0; i < RM / 2; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-              sg[q] = lanes_sum<16>(sg[q]);
-              su[q] = lanes_sum<16>(su[q]);
-            }
-            if (lc == 0)
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                colsum[(wc * 2 + 0) * TR + fr + q] = sg[q];
-                colsum[(wc * 2 + 1) * TR + fr + q] = su[q];
+              const int fr = (wr * (RM / 2) + i) * 16 + lr + q;
+              const float g = lanes_sum<16>(sg[i][q]), u = lanes_sum<16>(su[i][q]);
+              if (lc == 0) {
+                colsum[(wc * 2 + 0) * TR + fr] = g;
+                colsum[(wc * 2 + 1) * TR + fr] = u;
               }
+            }
+          __syncthreads();
+          for (int i = tid; i < 2 * TR; i += NT) {
+            const int side = i / TR, f = i % TR;
+            if (r0 + f >= a.nr) continue;
+            float v = 0.f;
+#pragma unroll
+            for (int w = 0; w < WC; ++w) v += colsum[(w * 2 + side) * TR + f];
+            a.col_partial[((c0 / BC) * 2 + side) * a.nr + r0 + f] = v;
           }
         }
       }
-    };
-    with_activation(a.activation, [&](auto kind) __attribute__((always_inline)) {
-      if (whole) finish(kind, std::true_type{});
-      else finish(kind, std::false_type{});
     });
-    if constexpr (MODE == kGateGrad) {
-      if (a.col_partial) {
-        __syncthreads();
-        for (int i = tid; i < 2 * TR; i += NT) {
-          const int side = i / TR, f = i % TR;
-          if (r0 + f >= a.nr) continue;
-          float v = 0.f;
-#pragma unroll
-          for (int w = 0; w < WC; ++w) v += colsum[(w * 2 + side) * TR + f];
-          a.col_partial[((c0 / BC) * 2 + side) * a.nr + r0 + f] = v;
-        }
-      }
-    }
   } else {
-    const bool joined = a.splits == 1;
-    T* out = static_cast<T*>(a.out[which]);
-    float* part = joined ? nullptr : a.partial + ((long)split * problems + which) * a.nc * a.nr;
-    const bool inside = r0 + BR <= a.nr && c0 + BC <= a.nc;
-    const bool vec = joined ? (a.ldo & 3) == 0 && ((size_t)out & (4 * sizeof(T) - 1)) == 0 : (a.nr & 3) == 0;
-    auto finish = [&](auto is_whole) __attribute__((always_inline)) {
-      constexpr bool W = decltype(is_whole)::value;
+    // out in elements of O: the result itself, or float32 partial results of a cut sum
+    auto finish = [&](auto* out, long ldo) __attribute__((always_inline)) {
+      using O = std::remove_pointer_t<decltype(out)>;
+      constexpr int EO = Vec16<O>::N, UO = BR / EO, kPitch = BR * (int)sizeof(O) + 16, kRegion = PR * kPitch;
 #pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        const long r = r0 + (wr * RM + i) * 16 + lr;
-        const int n = W ? 4 : (int)(a.nr - r < 4 ? a.nr - r : 4);
+      for (int j = 0; j < CN; ++j) {
+        char* region = lds + (j & 1) * kRegion;
 #pragma unroll
-        for (int j = 0; j < CN; ++j) {
-          const long c = c0 + (wc * CN + j) * 16 + lc;
-          if (!W && c >= a.nc) continue;
-          const float o[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-          if (joined) store4(out + c * a.ldo + r, n, W || (vec && n == 4), o);
-          else store4(part + c * a.nr + r, n, W || (vec && n == 4), o);
+        for (int i = 0; i < RM; ++i) {
+          vec4<O> o;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) o[q] = (O)acc[i][j][q];
+          *reinterpret_cast<vec4<O>*>(region + (wc * 16 + lc) * kPitch + ((wr * RM + i) * 16 + lr) * (int)sizeof(O)) = o;
+        }
+        __syncthreads();
+        for (int e = tid; e < PR * UO; e += NT) {
+          const int q = e / UO, r = e % UO * EO;
+          const long c = c0 + pass_row(q, j), left = a.nr - r0 - r;
+          if (c >= a.nc || left <= 0) continue;
+          Vec16<O> o;
+          o.load(reinterpret_cast<const O*>(region + q * kPitch + r * (int)sizeof(O)));
+          o.store_upto(out + c * ldo + r0 + r, left);
         }
       }
     };
-    if (inside && vec) finish(std::true_type{});
-    else finish(std::false_type{});
+    if (a.splits == 1) finish(static_cast<T*>(a.out[which]), a.ldo);
+    else finish(a.partial + ((long)split * problems + which) * a.nc * a.nr, a.nr);
   }
 }
 
-template <typename T, int MODE, int BR, int BC, int WR, int WC> int launch_one(const Args& a, hipStream_t s) {
+// LDS of a kernel: the two buffers and the biases, or what the epilogue's regions take
+template <typename T, int MODE, int BR, int BC, int WC> constexpr int lds_bytes() {
   constexpr bool kPair = MODE <= mz_gff::kGateGrad;
-  constexpr int TR = kPair ? BR / 2 : BR, kLds = 2 * (BR + BC) * 128 + (kPair ? 2 * TR * 4 : 0);
+  constexpr int TR = kPair ? BR / 2 : BR, PR = WC * 16, buffers = 2 * (BR + BC) * 128;
+  constexpr int regions = MODE == mz_gff::kForward    ? 2 * PR * (TR * (int)sizeof(T) + 16)
+                          : MODE == mz_gff::kGateGrad ? 3 * PR * (TR * (int)sizeof(T) + 16) + WC * 2 * TR * 4
+                                                      : 2 * PR * (BR * 4 + 16);
+  static_assert(!kPair || regions <= buffers, "the biases lie behind the buffers");
+  constexpr int bytes = (regions > buffers ? regions : buffers) + (kPair ? 2 * TR * 4 : 0);
+  static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
+  return bytes;
+}
+
+template <typename T, int MODE, int BR, int BC, int WR, int WC, int ACT = kAnyActivation> int launch_one(const Args& a, hipStream_t s) {
+  if constexpr (MODE == mz_gff::kGateGrad && ACT == kAnyActivation) {
+    switch (a.activation) {
+      case mz_gff::kSilu: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kSilu>(a, s);
+      case mz_gff::kGelu: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kGelu>(a, s);
+      case mz_gff::kRelu: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kRelu>(a, s);
+      default: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kSigmoid>(a, s);
+    }
+  } else {
+  constexpr int TR = MODE <= mz_gff::kGateGrad ? BR / 2 : BR, kLds = lds_bytes<T, MODE, BR, BC, WC>();
   static bool done[mz::kMaxDevices] = {false};
-  const auto kernel = gff_gemm_kernel<T, MODE, BR, BC, WR, WC>;
+  const auto kernel = gff_gemm_kernel<T, MODE, BR, BC, WR, WC, ACT>;
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
   const long total = ((a.nr + TR - 1) / TR) * ((a.nc + BC - 1) / BC) * (MODE == mz_gff::kWeightGrad ? 2 : 1) * a.splits;
   if (total > 0x7ffffff0l) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
   hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 7) / 8 * 8)), dim3(WR * WC * 64), kLds, s, a);
   return MZ_OK;
+  }
 }
 
 template <typename T, int MODE> int launch_mode(const Args& a, int tile, hipStream_t s) {
-  if (tile == 0) return launch_one<T, MODE, 256, 256, 2, 4>(a, s);
-  if (tile == 1) return launch_one<T, MODE, 128, 128, 2, 2>(a, s);
+  // float32's matrix instructions are slow enough for the smaller tiles to keep up with (18432 x 256 x 1024: 158 us, 209)
+  if constexpr (sizeof(T) == 2)
+    if (tile == 0) return launch_one<T, MODE, 256, 256, 2, 4>(a, s);
+  if (tile <= 1) return launch_one<T, MODE, 128, 128, 2, 2>(a, s);
   return launch_one<T, MODE, 64, 64, 2, 2>(a, s);
 }
 template <typename T> int launch_any(const Args& a, int mode, int tile, hipStream_t s) {
@@ -602,7 +673,7 @@ template <typename T, int CN> __global__ __launch_bounds__(256) void gff_few_ker
   if (a.bias[0]) load4(static_cast<const T*>(a.bias[0]) + f, nf, false, bg);
   if (a.bias[1]) load4(static_cast<const T*>(a.bias[1]) + f, nf, false, bu);
   const bool vec = nf == 4 && (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
-  with_activation(a.activation, [&](auto kind) __attribute__((always_inline)) {
+  with_activation<kAnyActivation>(a.activation, [&](auto kind) __attribute__((always_inline)) {
     constexpr int KIND = decltype(kind)::value;
 #pragma unroll
     for (int j = 0; j < CN; ++j) {

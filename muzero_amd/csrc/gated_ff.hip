@@ -109,34 +109,50 @@ template <typename T> void bias_grad_t(const float* p, long tiles, long F, void*
 
 int64_t tiles(int64_t nr, int64_t nc, int tr, int bc) { return ((nr + tr - 1) / tr) * ((nc + bc - 1) / bc); }
 
-// the largest tile that still gives every compute unit one
-int pick_tile(int64_t nr, int64_t nc, bool pair, int problems) {
-  for (int t = 0; t < 2; ++t) {
-    const int side = mz_gff::tile_side(t);
-    if (tiles(nr, nc, pair ? side / 2 : side, side) * problems >= 256) return t;
-  }
-  return 2;
-}
+// Tile and split of a product, by its estimated time (microseconds).  A tile's workgroups share a compute unit `at_once`
+// at a time; a step of one takes `alone`, and no less than `shared` times the workgroups there; `ends` is what a round
+// costs besides its steps (first loads, epilogue), by mode.  A sum cut into parts costs another launch and its partial
+// results' way through memory.  Measured per step (64 16-bit or 32 float32 values of k), one workgroup alone / the
+// compute unit full, on products of one to 4096 tiles; the estimate is within a fifth of what it was fitted to, and
+// choosing by it within a tenth of the best of all choices (18432 x 256 x 1024, dx: 128 x 128 tiles 33 us, 64 x 64 40,
+// 256 x 256 48; 1000 x 256 x 1000 float32, dx: 64 x 64 in 4 parts 18 us, 128 x 128 in 16 21, whole 137).
+struct TileCost {
+  int at_once;
+  float alone, shared, ends[3];                    // ends: kForward, kGateGrad, the plain products
+};
+constexpr TileCost kCost16[3] = {{1, 1.4f, 1.45f, {7.f, 14.f, 8.f}}, {2, .58f, .5f, {3.5f, 6.f, 4.5f}}, {5, .34f, .23f, {2.2f, 4.5f, 2.5f}}};
+constexpr TileCost kCost32[3] = {{}, {2, 2.1f, 1.95f, {4.f, 8.f, 5.f}}, {5, .72f, .53f, {2.5f, 4.f, 3.f}}};
 
 struct Split { int tile, splits, steps; };
 constexpr int kMaxSplits = 32;
-// tile and split of a product whose sum may be cut: prefer whole sums in the largest tile that fills the chip; else
-// 128 x 128 tiles (64 x 64 where the outputs are few) with the sum cut into enough parts for one tile per compute unit,
-// at least four steps each
-Split pick_split(int64_t nr, int64_t nc, int problems, int64_t steps) {
-  const int whole = pick_tile(nr, nc, false, problems);
-  Split p = {whole, 1, (int)steps};
-  if (whole < 2) return p;
-  p.tile = nr > 64 && nc > 64 ? 1 : 2;
-  const int side = mz_gff::tile_side(p.tile);
-  const int64_t have = tiles(nr, nc, side, side) * problems;
-  int64_t splits = (256 + have - 1) / have;
-  if (splits > steps / 4) splits = steps / 4;
-  if (splits > kMaxSplits) splits = kMaxSplits;
-  if (splits < 1) splits = 1;
-  p.steps = (int)((steps + splits - 1) / splits);
-  p.splits = (int)((steps + p.steps - 1) / p.steps);
-  return p;
+
+Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode) {
+  const bool pair = mode <= mz_gff::kGateGrad;
+  const int problems = mode == mz_gff::kWeightGrad ? 2 : 1;
+  const int cus = 256;                             // of an MI355X: the choice, and with it a sum's order, is the same everywhere
+  Split best = {2, 1, (int)steps};
+  float least = -1.f;
+  for (int t = dtype == MZ_F32 ? 1 : 0; t < 3; ++t) {
+    const TileCost& c = (dtype == MZ_F32 ? kCost32 : kCost16)[t];
+    const int side = mz_gff::tile_side(t);
+    const int64_t whole = tiles(nr, nc, pair ? side / 2 : side, side) * problems;
+    for (int want = 1; want <= (pair ? 1 : kMaxSplits); want += want < 4 ? 1 : want < 8 ? 2 : want < 16 ? 4 : 8) {
+      if (want > 1 && want > steps / 2) break;
+      const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+      const int64_t share = (whole * splits + cus - 1) / cus, rounds = share / c.at_once, rest = share % c.at_once;
+      auto round = [&](int64_t n) {
+        const float s = c.shared * n > c.alone ? c.shared * n : c.alone;
+        return per * s + c.ends[mode < 2 ? mode : 2];
+      };
+      float time = rounds * round(c.at_once) + (rest ? round(rest) : 0.f);
+      if (splits > 1) time += 3.f + (float)(nr * nc * problems) * splits * 8.f / 8e6f;
+      if (least < 0.f || time < least) {
+        least = time;
+        best = {t, (int)splits, (int)per};
+      }
+    }
+  }
+  return best;
 }
 
 struct Shape {
@@ -145,6 +161,7 @@ struct Shape {
   bool pads;                 // K is no whole number of 16-byte units: x, Wg, Wu are copied to padded rows
   int64_t pad_bytes() const { return pads ? round_up(M * Kp * elem_bytes(dtype), 256) + 2 * round_up(F * Kp * elem_bytes(dtype), 256) : 0; }
   int k_step() const { return 128 / elem_bytes(dtype); }
+  int64_t k_steps() const { return (Kp + k_step() - 1) / k_step(); }
 };
 Shape make_shape(int64_t M, int64_t K, int64_t F, int dtype) {
   const int e = unit_elems(dtype);
@@ -160,9 +177,9 @@ struct Backward {
 Backward plan_backward(const Shape& h) {
   Backward b;
   const int64_t f_steps = 2 * ((h.F + h.k_step() - 1) / h.k_step()), m_steps = (h.M + h.k_step() - 1) / h.k_step();
-  b.gate_tile = pick_tile(h.F, h.M, true, 1);
-  b.dx = pick_split(h.K, h.M, 1, f_steps);
-  b.dw = pick_split(h.K, h.F, 2, m_steps);
+  b.gate_tile = pick(h.F, h.M, h.k_steps(), h.dtype, mz_gff::kGateGrad).tile;
+  b.dx = pick(h.K, h.M, f_steps, h.dtype, mz_gff::kInputGrad);
+  b.dw = pick(h.K, h.F, m_steps, h.dtype, mz_gff::kWeightGrad);
   b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
   const int side = mz_gff::tile_side(b.gate_tile);
   b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
@@ -234,8 +251,8 @@ int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* 
     a.r[0] = w + xb; a.r[1] = w + xb + wb;
     a.ldr = a.ldc = a.nk = sh.Kp;
   }
-  a.steps_per_split = (int)((a.nk + sh.k_step() - 1) / sh.k_step());
-  if (int rc = launch(a, dtype, mz_gff::kForward, pick_tile(F, M, true, 1), s)) return rc;
+  a.steps_per_split = (int)sh.k_steps();
+  if (int rc = launch(a, dtype, mz_gff::kForward, pick(F, M, sh.k_steps(), dtype, mz_gff::kForward).tile, s)) return rc;
   return mz::check_launch("mz_gated_ff_fwd");
 }
 
@@ -285,7 +302,7 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   a.nr_pad = sh.Fp;
   a.activation = activation;
   a.splits = 1;
-  a.steps_per_split = (int)((kk + sh.k_step() - 1) / sh.k_step());
+  a.steps_per_split = (int)sh.k_steps();
   if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
   if (biases) {
     const int side = mz_gff::tile_side(plan.gate_tile);
