@@ -469,7 +469,7 @@ def test_outputs_and_workspaces_stay_inside_their_buffers(rows, k, f, t):
     written, nothing outside, and the results are those of the Python entry points."""
     from muzero_amd import _lib, blocks
     t = TYPES[t]
-    dt = blocks._DTYPES[t]
+    dt = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[t]          # MZ_F32, MZ_BF16, MZ_F16
     x, wg, wu, bg, bu, dh = ff_inputs(rows, rows, k, f, t)
     p, s = (lambda v: v.data_ptr()), _lib.current_stream()
     want = ff_run(x, wg, wu, bg, bu, dh, "silu")
