@@ -594,9 +594,8 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
 
 /* Gated feed-forward projection in one kernel: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up).  x: [M] rows of K
  * elements, ldx apart; w_gate, w_up: [F][K]; b_gate, b_up: [F] or NULL; h: [M][F]; all of `dtype`, float32
- * accumulation.  activation: 0 SiLU, 1 GELU (erf), 2 ReLU, 3 sigmoid.  K, F up to 2^20.  Where K is a whole number of
- * 16-byte units, x, w_gate, w_up and the rows of x start on 16 bytes; other K have no such condition (the operands are
- * copied to padded rows in the workspace).  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which may
+ * accumulation.  activation: 0 SiLU, 1 GELU (erf), 2 ReLU, 3 sigmoid.  K, F up to 2^20; rows of x up to 4 MiB apart.  No
+ * alignment beyond the elements' is needed.  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which may
  * be 0 (then NULL will do).
  * Backward: recomputes both products; dh [M][F] -> dx [M][K], dw_gate / dw_up [F][K] (both or neither), db_gate / db_up
  * [F]; NULL for what is not wanted.  The gradients of the two products are rounded to `dtype` between the launches.

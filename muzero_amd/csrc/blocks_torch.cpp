@@ -112,21 +112,11 @@ Rows rows_of(const Tensor& x) {
   if ((c > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < c)) r = r.contiguous();
   return {r, r.size(0) > 1 ? r.stride(0) : c};
 }
-// for the matrix kernels: where a row is whole 16-byte units, rows have to start on 16 bytes, and they lie at most 4 MiB
-// apart; what does not is copied
+// for the matrix kernels: rows at most 4 MiB apart
 Rows matrix_rows(const Tensor& x) {
   Rows r = rows_of(x);
-  const int64_t size = x.element_size();
-  const bool aligned = reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0 && r.ld * size % 16 == 0;
-  if (r.ld * size > kMaxStrideBytes || (!aligned && x.size(-1) * size % 16 == 0)) {
-    r.t = r.t.clone(at::MemoryFormat::Contiguous);
-    r.ld = x.size(-1);
-  }
+  if (r.ld * x.element_size() > kMaxStrideBytes) r = {r.t.clone(at::MemoryFormat::Contiguous), x.size(-1)};
   return r;
-}
-Tensor matrix_weight(const Tensor& w) {
-  Tensor c = contiguous(w);
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
 }
 
 // Gradients that a backward pass returns.  They are raw results: where somebody may ask for their own gradient, that has
@@ -235,7 +225,7 @@ Tensor gated_ff_forward(const Tensor& x, const Tensor& wg, const Tensor& wu, con
   Tensor h = at::empty(shape, x.options());
   if (rows == 0) return h;
   const Rows r = matrix_rows(x);
-  const Tensor wgc = matrix_weight(wg), wuc = matrix_weight(wu), bgc = contiguous(bg), buc = contiguous(bu);
+  const Tensor wgc = contiguous(wg), wuc = contiguous(wu), bgc = contiguous(bg), buc = contiguous(bu);
   const int type = type_code(x.scalar_type());
   const int64_t need = api.gated_ff_workspace_bytes(rows, k, hidden, type, 0);
   const Tensor ws = bytes(need, x);
@@ -274,7 +264,7 @@ struct GatedFF : torch::autograd::Function<GatedFF> {
       if (want[i]) out[i] = make({hidden});
     if (rows && (out[0].defined() || weights || out[3].defined() || out[4].defined())) {
       const Rows r = matrix_rows(x);
-      const Tensor wgc = matrix_weight(wg), wuc = matrix_weight(wu), bgc = contiguous(bg), buc = contiguous(bu);
+      const Tensor wgc = contiguous(wg), wuc = contiguous(wu), bgc = contiguous(bg), buc = contiguous(bu);
       const Tensor dh = contiguous(grad_as(grads[0], x.scalar_type()));
       const int type = type_code(x.scalar_type());
       const int64_t need = api.gated_ff_workspace_bytes(rows, k, hidden, type, 1);

@@ -22,6 +22,7 @@
 namespace mz_gff {
 
 enum Mode { kForward = 0, kGateGrad = 1, kInputGrad = 2, kWeightGrad = 3 };
+constexpr int tail_units(int mode) { return mode == kInputGrad ? 2 : 1; }
 enum Activation { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
 
 struct Args {
@@ -29,7 +30,8 @@ struct Args {
   const void* r[2];
   const void* c[2];
   long ldr, ldc;             // elements between rows of the matrices as they lie in memory
-  long nr, nc, nk;           // extents of r (kForward / kGateGrad: features), c and k
+  long nr, nc, nk;           // extents of r (kForward / kGateGrad: features), c and k - the k that the steps take
+  long nk_all;               // all k: nk .. nk_all - 1 are added element by element, at most tail_units(mode) 16-byte units of them
   void* out[2];
   long ldo;
   const void* bias[2];
@@ -173,7 +175,6 @@ template <typename T, bool ACROSS, int B, int NT> struct Operand {
     else return ((row >> 1) & 1) | (((row >> 3) & 1) << 1);   // four blocks a row, two rows to 256 bytes
   }
 
-  // row0_of(round) tells the matrix row of staged row 0 of the tile for `along`
   __device__ __forceinline__ void init(int tid, long ld, long rows_left) {
     row0 = tid / UPR;
     unit = tid % UPR;
@@ -254,7 +255,7 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   constexpr int KS = OpR::KS;
   constexpr int RM = BR / WR / 16, CN = BC / WC / 16;                 // 16 x 16 blocks of a wavefront
   constexpr int TR = kPair ? BR / 2 : BR;                             // output rows (r) of a tile
-  extern __shared__ __attribute__((aligned(16))) char lds[];          // 2 x (BR + BC) x 128 bytes, then biases
+  extern __shared__ __attribute__((aligned(16))) char lds[];          // two buffers of (BR + BC) x 128 bytes, then biases
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / WC, wc = wave % WC;
@@ -412,6 +413,56 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
   __syncthreads();               // the epilogue uses the buffers
   __builtin_amdgcn_sched_barrier(0);                                  // and none of its registers before
+
+  // ---- the k left out of the steps: staged as rows of one unit (kInputGrad: two of dg's and two of du's), one more half
+  // step
+  if (a.nk_all > a.nk && split == a.splits - 1) {
+    using TailR = Operand<T, false, BR, NT>;
+    using TailC = Operand<T, false, BC, NT>;
+    for (int row = tid; row < BR + BC; row += NT) {
+      const bool is_r = row < BR;
+      const int q = is_r ? row : row - BR;
+      char* base = lds + (is_r ? 0 : BR * 128) + q * 128;
+#pragma unroll
+      for (int unit = 0; unit < 4; ++unit) {
+        constexpr int kTail = tail_units(MODE);
+        const int seg = MODE == kInputGrad ? unit / kTail : 0;
+        const long k = a.nk + unit % kTail * OpR::EC;
+        Vec16<T> e;
+#pragma unroll
+        for (int t = 0; t < OpR::EC; ++t) e.v[t] = (T)0.f;
+        if (MODE == kInputGrad || unit < kTail) {
+          const T* p;
+          long along;              // elements between k's
+          bool exists;
+          if (is_r) {
+            const int r = kPair ? q % TR : q;
+            exists = r0 + r < a.nr;
+            p = static_cast<const T*>(a.r[kPair ? q / TR : seg]) + (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
+            along = kRAcross ? a.ldr : 1;
+          } else {
+            exists = c0 + q < a.nc;
+            p = static_cast<const T*>(a.c[MODE == kWeightGrad ? which : seg]) + (kCAcross ? k * a.ldc + c0 + q : (c0 + q) * a.ldc + k);
+            along = kCAcross ? a.ldc : 1;
+          }
+#pragma unroll
+          for (int t = 0; t < OpR::EC; ++t)
+            if (exists && k + t < a.nk_all) e.v[t] = p[t * along];
+        }
+        e.store(reinterpret_cast<T*>(base + TailR::place(q, unit) * 16));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < CN; ++j) cf[0][j] = TailC::fragment(lds + BR * 128, wc * CN + j, 0, lane);
+#pragma unroll
+    for (int i = 0; i < RM; ++i) {
+      rf[i] = TailR::fragment(lds, r_block(i), 0, lane);
+#pragma unroll
+      for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
+    }
+    __syncthreads();
+  }
 
   // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
   if constexpr (kPair) {

@@ -24,27 +24,6 @@ int launch(const Args& a, int dtype, int mode, int tile, hipStream_t s) {
                             : mz_gff::launch_f16(a, mode, tile, s);
 }
 
-// a matrix whose rows are no whole 16-byte units (K odd for them), copied to rows that are, with zeros behind
-template <typename U>
-__global__ __launch_bounds__(256) void pad_rows_kernel(const U* __restrict__ in, long ld, U* __restrict__ out, long rows,
-                                                       int cols, int cols_pad) {
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < rows * cols_pad; i += (long)gridDim.x * 256) {
-    const long r = i / cols_pad;
-    const int c = (int)(i - r * cols_pad);
-    out[i] = c < cols ? in[r * ld + c] : (U)0;
-  }
-}
-void pad_rows(const void* in, int64_t ld, void* out, int64_t rows, int64_t cols, int64_t cols_pad, int dtype, hipStream_t s) {
-  const long want = (rows * cols_pad + 255) / 256, cap = 16L * mz::compute_units();
-  const dim3 grid((unsigned)(want < cap ? want : cap));
-  if (elem_bytes(dtype) == 4)
-    hipLaunchKernelGGL((pad_rows_kernel<unsigned>), grid, dim3(256), 0, s, static_cast<const unsigned*>(in), ld,
-                       static_cast<unsigned*>(out), rows, (int)cols, (int)cols_pad);
-  else
-    hipLaunchKernelGGL((pad_rows_kernel<unsigned short>), grid, dim3(256), 0, s, static_cast<const unsigned short*>(in), ld,
-                       static_cast<unsigned short*>(out), rows, (int)cols, (int)cols_pad);
-}
-
 // out[p][c][r] = sum over the splits of partial[split][p][c][r]
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, long per_problem,
@@ -156,16 +135,23 @@ Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode) {
 }
 
 struct Shape {
-  int64_t M, K, F, Kp, Fp;
+  int64_t M, K, F, Fp;       // Fp: F in whole 16-byte units, the row length of dg and du
   int dtype;
-  bool pads;                 // K is no whole number of 16-byte units: x, Wg, Wu are copied to padded rows
-  int64_t pad_bytes() const { return pads ? round_up(M * Kp * elem_bytes(dtype), 256) + 2 * round_up(F * Kp * elem_bytes(dtype), 256) : 0; }
-  int k_step() const { return 128 / elem_bytes(dtype); }
-  int64_t k_steps() const { return (Kp + k_step() - 1) / k_step(); }
+  bool ragged;               // K is no whole number of units: a row's last unit reaches into the next row, the last row's
+                             // past the end (gated_ff.h: nk_all)
+  int step() const { return 128 / elem_bytes(dtype); }
+  int64_t steps(int64_t nk) const { return nk > 0 ? (nk + step() - 1) / step() : 1; }
+  // the rows at a matrix's end from which a unit that starts inside a row of K would reach past the last one
+  int64_t end_rows() const { return ragged ? (round_up(K, unit_elems(dtype)) - K + K - 1) / K : 0; }
+  // the k that the steps take: of K (forward), of F (input gradient) and of M (weight gradient); what is left is less
+  // than a unit of K, less than two of F (end_rows() and what makes whole units before it) and less than one of M
+  int64_t nk_K() const { return K / unit_elems(dtype) * unit_elems(dtype); }
+  int64_t nk_F() const { return !ragged ? F : F > end_rows() ? (F - end_rows()) / unit_elems(dtype) * unit_elems(dtype) : 0; }
+  int64_t nk_M() const { return M > end_rows() ? M - end_rows() : 0; }
 };
 Shape make_shape(int64_t M, int64_t K, int64_t F, int dtype) {
   const int e = unit_elems(dtype);
-  return {M, K, F, round_up(K, e), round_up(F, e), dtype, K % e != 0};
+  return {M, K, F, round_up(F, e), dtype, K % e != 0};
 }
 constexpr int64_t kFew = 64;   // tokens the streaming kernel takes
 
@@ -176,10 +162,9 @@ struct Backward {
 };
 Backward plan_backward(const Shape& h) {
   Backward b;
-  const int64_t f_steps = 2 * ((h.F + h.k_step() - 1) / h.k_step()), m_steps = (h.M + h.k_step() - 1) / h.k_step();
-  b.gate_tile = pick(h.F, h.M, h.k_steps(), h.dtype, mz_gff::kGateGrad).tile;
-  b.dx = pick(h.K, h.M, f_steps, h.dtype, mz_gff::kInputGrad);
-  b.dw = pick(h.K, h.F, m_steps, h.dtype, mz_gff::kWeightGrad);
+  b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad).tile;
+  b.dx = pick(h.K, h.M, 2 * h.steps(h.nk_F()), h.dtype, mz_gff::kInputGrad);
+  b.dw = pick(h.K, h.F, h.steps(h.nk_M()), h.dtype, mz_gff::kWeightGrad);
   b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
   const int side = mz_gff::tile_side(b.gate_tile);
   b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
@@ -196,11 +181,9 @@ int check_shape(const char* who, int64_t M, int64_t K, int64_t F, int32_t dtype,
   MZ_REQUIRE(activation >= 0 && activation <= mz_gff::kSigmoid, "%s: unknown activation %d", who, activation);
   return MZ_OK;
 }
-int check_operands(const char* who, const Shape& h, const void* x, int64_t ldx, const void* wg, const void* wu) {
+int check_stride(const char* who, const Shape& h, int64_t ldx) {
   MZ_REQUIRE(ldx >= h.K && ldx * elem_bytes(h.dtype) <= (1 << 22),
              "%s: stride of x out of range (%lld, K = %lld; rows up to 4 MiB apart)", who, (long long)ldx, (long long)h.K);
-  MZ_REQUIRE(h.pads || (((size_t)x | (size_t)wg | (size_t)wu) % 16 == 0 && ldx % unit_elems(h.dtype) == 0),
-             "%s: x, w_gate, w_up and the rows of x must start on 16 bytes", who);
   return MZ_OK;
 }
 
@@ -210,10 +193,9 @@ extern "C" {
 
 int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward) {
   if (check_shape("mz_gated_ff_workspace_bytes", M, K, F, dtype, 0)) return -1;
-  const Shape h = make_shape(M, K, F, dtype);
-  if (!backward) return M <= kFew ? 0 : h.pad_bytes();
-  const Backward b = plan_backward(h);
-  return h.pad_bytes() + 2 * b.dgu_bytes + b.col_bytes + b.partial_bytes;
+  if (!backward) return 0;
+  const Backward b = plan_backward(make_shape(M, K, F, dtype));
+  return 2 * b.dgu_bytes + b.col_bytes + b.partial_bytes;
 }
 
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
@@ -221,14 +203,14 @@ int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* 
                     int64_t workspace_bytes, mz_stream_t stream) {
   MZ_REQUIRE(x && w_gate && w_up && h, "mz_gated_ff_fwd: null tensor");
   if (int rc = check_shape("mz_gated_ff_fwd", M, K, F, dtype, activation)) return rc;
-  Shape sh = make_shape(M, K, F, dtype);
-  if (int rc = check_operands("mz_gated_ff_fwd", sh, x, ldx, w_gate, w_up)) return rc;
+  const Shape sh = make_shape(M, K, F, dtype);
+  if (int rc = check_stride("mz_gated_ff_fwd", sh, ldx)) return rc;
   hipStream_t s = mz::as_stream(stream);
   Args a = {};
   a.r[0] = w_gate; a.r[1] = w_up;
   a.c[0] = a.c[1] = x;
   a.ldr = K; a.ldc = ldx;
-  a.nr = F; a.nc = M; a.nk = K;
+  a.nr = F; a.nc = M; a.nk = M <= kFew ? K : sh.nk_K(); a.nk_all = K;
   a.out[0] = h; a.ldo = F;
   a.bias[0] = b_gate; a.bias[1] = b_up;
   a.activation = activation;
@@ -238,21 +220,8 @@ int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* 
       return rc;
     return mz::check_launch("mz_gated_ff_fwd");
   }
-  const int64_t need = sh.pad_bytes();
-  MZ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (size_t)workspace % 16 == 0),
-             "mz_gated_ff_fwd: workspace too small or not 16-byte aligned");
-  if (sh.pads) {
-    char* w = static_cast<char*>(workspace);
-    const int64_t xb = round_up(M * sh.Kp * elem_bytes(dtype), 256), wb = round_up(F * sh.Kp * elem_bytes(dtype), 256);
-    pad_rows(x, ldx, w, M, K, sh.Kp, dtype, s);
-    pad_rows(w_gate, K, w + xb, F, K, sh.Kp, dtype, s);
-    pad_rows(w_up, K, w + xb + wb, F, K, sh.Kp, dtype, s);
-    a.c[0] = a.c[1] = w;
-    a.r[0] = w + xb; a.r[1] = w + xb + wb;
-    a.ldr = a.ldc = a.nk = sh.Kp;
-  }
-  a.steps_per_split = (int)sh.k_steps();
-  if (int rc = launch(a, dtype, mz_gff::kForward, pick(F, M, sh.k_steps(), dtype, mz_gff::kForward).tile, s)) return rc;
+  a.steps_per_split = (int)sh.steps(a.nk);
+  if (int rc = launch(a, dtype, mz_gff::kForward, pick(F, M, sh.steps(a.nk), dtype, mz_gff::kForward).tile, s)) return rc;
   return mz::check_launch("mz_gated_ff_fwd");
 }
 
@@ -264,37 +233,25 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   MZ_REQUIRE((dw_gate == nullptr) == (dw_up == nullptr), "mz_gated_ff_bwd: dw_gate and dw_up go together");
   MZ_REQUIRE(dx || dw_gate || db_gate || db_up, "mz_gated_ff_bwd: no gradient asked for");
   if (int rc = check_shape("mz_gated_ff_bwd", M, K, F, dtype, activation)) return rc;
-  Shape sh = make_shape(M, K, F, dtype);
-  if (int rc = check_operands("mz_gated_ff_bwd", sh, x, ldx, w_gate, w_up)) return rc;
+  const Shape sh = make_shape(M, K, F, dtype);
+  if (int rc = check_stride("mz_gated_ff_bwd", sh, ldx)) return rc;
   const Backward plan = plan_backward(sh);
   const int64_t need = mz_gated_ff_workspace_bytes(M, K, F, dtype, 1);
   MZ_REQUIRE(workspace && workspace_bytes >= need && (size_t)workspace % 16 == 0,
              "mz_gated_ff_bwd: workspace too small (%lld of %lld bytes) or not 16-byte aligned", (long long)workspace_bytes,
              (long long)need);
   hipStream_t s = mz::as_stream(stream);
-  char* w = static_cast<char*>(workspace);
-  const void *xm = x, *wg = w_gate, *wu = w_up;
-  int64_t ldxm = ldx, kk = K;
-  if (sh.pads) {
-    const int64_t xb = round_up(M * sh.Kp * elem_bytes(dtype), 256), wb = round_up(F * sh.Kp * elem_bytes(dtype), 256);
-    pad_rows(x, ldx, w, M, K, sh.Kp, dtype, s);
-    pad_rows(w_gate, K, w + xb, F, K, sh.Kp, dtype, s);
-    pad_rows(w_up, K, w + xb + wb, F, K, sh.Kp, dtype, s);
-    xm = w; wg = w + xb; wu = w + xb + wb;
-    ldxm = kk = sh.Kp;
-    w += sh.pad_bytes();
-  }
-  char* dg = w;
+  char* dg = static_cast<char*>(workspace);
   char* du = dg + plan.dgu_bytes;
   float* cols = reinterpret_cast<float*>(du + plan.dgu_bytes);
   float* partial = reinterpret_cast<float*>(du + plan.dgu_bytes + plan.col_bytes);
   const bool biases = db_gate || db_up;
 
   Args a = {};                                     // dg, du
-  a.r[0] = wg; a.r[1] = wu;
-  a.c[0] = a.c[1] = xm;
-  a.ldr = kk; a.ldc = ldxm;
-  a.nr = F; a.nc = M; a.nk = kk;
+  a.r[0] = w_gate; a.r[1] = w_up;
+  a.c[0] = a.c[1] = x;
+  a.ldr = K; a.ldc = ldx;
+  a.nr = F; a.nc = M; a.nk = sh.nk_K(); a.nk_all = K;
   a.out[0] = dg; a.out[1] = du; a.ldo = sh.Fp;
   a.bias[0] = b_gate; a.bias[1] = b_up;
   a.dh = dh; a.lddh = F;
@@ -302,7 +259,7 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   a.nr_pad = sh.Fp;
   a.activation = activation;
   a.splits = 1;
-  a.steps_per_split = (int)sh.k_steps();
+  a.steps_per_split = (int)sh.steps(a.nk);
   if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
   if (biases) {
     const int side = mz_gff::tile_side(plan.gate_tile);
@@ -313,10 +270,10 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   }
   if (dx) {
     Args p = {};
-    p.r[0] = wg; p.r[1] = wu;
+    p.r[0] = w_gate; p.r[1] = w_up;
     p.c[0] = dg; p.c[1] = du;
-    p.ldr = kk; p.ldc = sh.Fp;
-    p.nr = K; p.nc = M; p.nk = F;
+    p.ldr = K; p.ldc = sh.Fp;
+    p.nr = K; p.nc = M; p.nk = sh.nk_F(); p.nk_all = F;
     p.out[0] = p.out[1] = dx; p.ldo = K;
     p.partial = partial;
     p.splits = plan.dx.splits; p.steps_per_split = plan.dx.steps;
@@ -325,10 +282,10 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   }
   if (dw_gate) {
     Args p = {};
-    p.r[0] = p.r[1] = xm;
+    p.r[0] = p.r[1] = x;
     p.c[0] = dg; p.c[1] = du;
-    p.ldr = ldxm; p.ldc = sh.Fp;
-    p.nr = K; p.nc = F; p.nk = M;
+    p.ldr = ldx; p.ldc = sh.Fp;
+    p.nr = K; p.nc = F; p.nk = sh.nk_M(); p.nk_all = M;
     p.out[0] = dw_gate; p.out[1] = dw_up; p.ldo = K;
     p.partial = partial;
     p.splits = plan.dw.splits; p.steps_per_split = plan.dw.steps;

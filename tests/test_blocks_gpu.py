@@ -230,7 +230,7 @@ def ff_run(x, wg, wu, bg, bu, dh, activation):
 # whole unit, whole steps and not; F likewise
 FF_SHAPES = [(1, 1, 1), (1, 256, 1024), (2, 7, 5), (16, 64, 33), (17, 96, 40), (33, 130, 48), (64, 257, 65), (65, 64, 64),
              (66, 33, 20), (128, 256, 128), (129, 264, 130), (300, 72, 1000), (1000, 257, 1001), (513, 520, 264), (4100, 64, 24),
-             (777, 8, 8), (2500, 512, 136)]
+             (777, 8, 8), (2500, 512, 136), (300, 1, 200), (300, 2, 101), (200, 3, 70), (129, 5, 9), (70, 6, 16), (66, 4, 7)]
 
 
 @pytest.mark.parametrize("t", TYPES)
