@@ -47,7 +47,11 @@ struct Args {
 int launch_bf16(const Args& a, int mode, int tile, hipStream_t s);
 int launch_f16(const Args& a, int mode, int tile, hipStream_t s);
 int launch_f32(const Args& a, int mode, int tile, hipStream_t s);
-// x in at most 64 rows: out = forward
+// kInputGrad and kWeightGrad in one launch, both in tiles 1 or 2
+int launch_both_bf16(const Args& x, const Args& w, int tile, hipStream_t s);
+int launch_both_f16(const Args& x, const Args& w, int tile, hipStream_t s);
+int launch_both_f32(const Args& x, const Args& w, int tile, hipStream_t s);
+// kForward of at most 16 tokens
 int launch_few_bf16(const Args& a, hipStream_t s);
 int launch_few_f16(const Args& a, hipStream_t s);
 int launch_few_f32(const Args& a, hipStream_t s);
@@ -121,30 +125,6 @@ template <int FIXED, typename F> __device__ __forceinline__ void with_activation
   else if (kind == mz_gff::kGelu) f(std::integral_constant<int, mz_gff::kGelu>{});
   else if (kind == mz_gff::kRelu) f(std::integral_constant<int, mz_gff::kRelu>{});
   else f(std::integral_constant<int, mz_gff::kSigmoid>{});
-}
-
-// four consecutive elements from / to memory; `vec`: all four exist and the address suits one access
-template <typename T> __device__ __forceinline__ void load4(const T* p, int n, bool vec, float (&v)[4]) {
-  if (vec) {
-    const vec4<T> t = *reinterpret_cast<const vec4<T>*>(p);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)t[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = j < n ? (float)p[j] : 0.f;
-  }
-}
-template <typename T> __device__ __forceinline__ void store4(T* p, int n, bool vec, const float (&v)[4]) {
-  if (vec) {
-    vec4<T> t;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = (T)v[j];
-    *reinterpret_cast<vec4<T>*>(p) = t;
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) p[j] = (T)v[j];
-  }
 }
 
 constexpr unsigned kOutside = 0x80000000u;   // a byte offset no descriptor below covers: the load returns zeros
@@ -245,7 +225,7 @@ __device__ __forceinline__ void half_step_order() {
 }
 
 template <typename T, int MODE, int BR, int BC, int WR, int WC, int ACT>
-__global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) void gff_gemm_kernel(Args a) {
+__device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
   using namespace mz_gff;
   constexpr int NT = WR * WC * 64;
   constexpr bool kPair = MODE == kForward || MODE == kGateGrad;       // a tile's R rows: half gate, half up features
@@ -255,7 +235,7 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   constexpr int KS = OpR::KS;
   constexpr int RM = BR / WR / 16, CN = BC / WC / 16;                 // 16 x 16 blocks of a wavefront
   constexpr int TR = kPair ? BR / 2 : BR;                             // output rows (r) of a tile
-  extern __shared__ __attribute__((aligned(16))) char lds[];          // two buffers of (BR + BC) x 128 bytes, then biases
+  // lds: two buffers of (BR + BC) x 128 bytes, then biases
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / WC, wc = wave % WC;
@@ -266,7 +246,7 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
   const unsigned problems = MODE == kWeightGrad ? 2 : 1;
   const unsigned per_problem = tiles_r * tiles_c, total = per_problem * problems * (unsigned)a.splits;
   const unsigned per_xcd = (total + 7) / 8;
-  const unsigned id = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  const unsigned id = (block & 7) * per_xcd + (block >> 3);
   if (id >= total) return;
   const unsigned job = id / per_problem, t = id - job * per_problem;
   const int which = MODE == kWeightGrad ? (int)(job % 2) : 0;
@@ -336,15 +316,6 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
     else return wr * RM + i;
   };
 
-  if constexpr (kPair) {          // the tile's biases as float32 behind the two buffers: [gate, up][TR]
-    float* bias = reinterpret_cast<float*>(lds + 2 * (BR + BC) * 128);
-    for (int i = tid; i < 2 * TR; i += NT) {
-      const T* b = static_cast<const T*>(a.bias[i / TR]);
-      const long f = r0 + i % TR;
-      bias[i] = b && f < a.nr ? (float)b[f] : 0.f;
-    }
-  }
-
   // A step has two halves, 64 bytes of k each, whose operands are in registers when they begin: while the first half's
   // matrix instructions run, the second half's operands are read from LDS, the next step's units (loaded a step ago) are
   // staged in the other buffer and the ones after that are sent for; then the barrier; while the second half runs, the
@@ -356,6 +327,14 @@ __global__ __launch_bounds__(WR * WC * 64, (BR == 256 ? 2 : BR == 128 ? 2 : 4)) 
     const Source src = source(first), after = source(first + 1);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) load_unit(src, u);
+    if constexpr (kPair) {        // meanwhile the tile's biases, as float32 behind the two buffers: [gate, up][TR]
+      float* bias = reinterpret_cast<float*>(lds + 2 * (BR + BC) * 128);
+      for (int i = tid; i < 2 * TR; i += NT) {
+        const T* b = static_cast<const T*>(a.bias[i / TR]);
+        const long f = r0 + i % TR;
+        bias[i] = b && f < a.nr ? (float)b[f] : 0.f;
+      }
+    }
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) {
       stage_unit(0, u);
@@ -623,33 +602,58 @@ template <typename T, int MODE, int BR, int BC, int WC> constexpr int lds_bytes(
   static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
   return bytes;
 }
+// wavefronts per SIMD that the registers have to leave room for
+constexpr int min_waves(int side) { return side == 64 ? 4 : 2; }
 
-template <typename T, int MODE, int BR, int BC, int WR, int WC, int ACT = kAnyActivation> int launch_one(const Args& a, hipStream_t s) {
-  if constexpr (MODE == mz_gff::kGateGrad && ACT == kAnyActivation) {
-    switch (a.activation) {
-      case mz_gff::kSilu: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kSilu>(a, s);
-      case mz_gff::kGelu: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kGelu>(a, s);
-      case mz_gff::kRelu: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kRelu>(a, s);
-      default: return launch_one<T, MODE, BR, BC, WR, WC, mz_gff::kSigmoid>(a, s);
-    }
-  } else {
-  constexpr int TR = MODE <= mz_gff::kGateGrad ? BR / 2 : BR, kLds = lds_bytes<T, MODE, BR, BC, WC>();
-  static bool done[mz::kMaxDevices] = {false};
-  const auto kernel = gff_gemm_kernel<T, MODE, BR, BC, WR, WC, ACT>;
-  if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
-  const long total = ((a.nr + TR - 1) / TR) * ((a.nc + BC - 1) / BC) * (MODE == mz_gff::kWeightGrad ? 2 : 1) * a.splits;
-  if (total > 0x7ffffff0l) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((total + 7) / 8 * 8)), dim3(WR * WC * 64), kLds, s, a);
-  return MZ_OK;
-  }
+template <typename T, int MODE, int S, int WR, int WC, int ACT>
+__global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_gemm_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  gff_gemm<T, MODE, S, S, WR, WC, ACT>(a, blockIdx.x, lds);
+}
+// the two products of a small backward pass side by side: workgroups 0 .. blocks_x - 1 (a multiple of 8) make the input
+// gradient, the others the weights'
+template <typename T, int S, int WR, int WC>
+__global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_both_kernel(Args x, Args w, unsigned blocks_x) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  if (blockIdx.x < blocks_x) gff_gemm<T, mz_gff::kInputGrad, S, S, WR, WC, kAnyActivation>(x, blockIdx.x, lds);
+  else gff_gemm<T, mz_gff::kWeightGrad, S, S, WR, WC, kAnyActivation>(w, blockIdx.x - blocks_x, lds);
 }
 
+// workgroups of a product in S x S tiles: one a tile, a multiple of the 8 XCDs
+template <int MODE, int S> long gemm_blocks(const Args& a) {
+  constexpr int TR = MODE <= mz_gff::kGateGrad ? S / 2 : S;
+  const long total = ((a.nr + TR - 1) / TR) * ((a.nc + S - 1) / S) * (MODE == mz_gff::kWeightGrad ? 2 : 1) * a.splits;
+  return (total + 7) / 8 * 8;
+}
+
+template <typename T, int MODE, int S, int WR, int WC, int ACT> int launch_kernel(const Args& a, hipStream_t s) {
+  constexpr int kLds = lds_bytes<T, MODE, S, S, WC>();
+  static bool done[mz::kMaxDevices] = {false};
+  const auto kernel = gff_gemm_kernel<T, MODE, S, WR, WC, ACT>;
+  if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
+  const long blocks = gemm_blocks<MODE, S>(a);
+  if (blocks > 0x7ffffff0l) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WR * WC * 64), kLds, s, a);
+  return MZ_OK;
+}
+template <typename T, int MODE, int S, int WR, int WC> int launch_one(const Args& a, hipStream_t s) {
+  if constexpr (MODE == mz_gff::kGateGrad) {
+    switch (a.activation) {
+      case mz_gff::kSilu: return launch_kernel<T, MODE, S, WR, WC, mz_gff::kSilu>(a, s);
+      case mz_gff::kGelu: return launch_kernel<T, MODE, S, WR, WC, mz_gff::kGelu>(a, s);
+      case mz_gff::kRelu: return launch_kernel<T, MODE, S, WR, WC, mz_gff::kRelu>(a, s);
+      default: return launch_kernel<T, MODE, S, WR, WC, mz_gff::kSigmoid>(a, s);
+    }
+  } else {
+    return launch_kernel<T, MODE, S, WR, WC, kAnyActivation>(a, s);
+  }
+}
 template <typename T, int MODE> int launch_mode(const Args& a, int tile, hipStream_t s) {
   // float32's matrix instructions are slow enough for the smaller tiles to keep up with (18432 x 256 x 1024: 158 us, 209)
   if constexpr (sizeof(T) == 2)
-    if (tile == 0) return launch_one<T, MODE, 256, 256, 2, 4>(a, s);
-  if (tile <= 1) return launch_one<T, MODE, 128, 128, 2, 2>(a, s);
-  return launch_one<T, MODE, 64, 64, 2, 2>(a, s);
+    if (tile == 0) return launch_one<T, MODE, 256, 2, 4>(a, s);
+  if (tile <= 1) return launch_one<T, MODE, 128, 2, 2>(a, s);
+  return launch_one<T, MODE, 64, 2, 2>(a, s);
 }
 template <typename T> int launch_any(const Args& a, int mode, int tile, hipStream_t s) {
   switch (mode) {
@@ -659,36 +663,44 @@ template <typename T> int launch_any(const Args& a, int mode, int tile, hipStrea
     default: return launch_mode<T, mz_gff::kWeightGrad>(a, tile, s);
   }
 }
+template <typename T, int S> int launch_both_in(const Args& x, const Args& w, hipStream_t s) {
+  constexpr int kLds = lds_bytes<T, mz_gff::kInputGrad, S, S, 2>();
+  static bool done[mz::kMaxDevices] = {false};
+  const auto kernel = gff_both_kernel<T, S, 2, 2>;
+  if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
+  const long bx = gemm_blocks<mz_gff::kInputGrad, S>(x), bw = gemm_blocks<mz_gff::kWeightGrad, S>(w);
+  if (bx + bw > 0x7ffffff0l) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(bx + bw)), dim3(256), kLds, s, x, w, (unsigned)bx);
+  return MZ_OK;
+}
+template <typename T> int launch_both(const Args& x, const Args& w, int tile, hipStream_t s) {
+  return tile == 1 ? launch_both_in<T, 128>(x, w, s) : launch_both_in<T, 64>(x, w, s);
+}
 
-// ---- a few tokens (at most 64): the weights are read once, straight into the matrix instructions' registers; 16
+// ---- a few tokens (at most 16): the weights are read once, straight into the matrix instructions' registers; 16
 // features (their gate and up rows) a workgroup, its four wavefronts split k and add up through LDS.
-template <typename T, int CN> __global__ __launch_bounds__(256) void gff_few_kernel(Args a) {
+template <typename T> __global__ __launch_bounds__(256) void gff_few_kernel(Args a) {
   constexpr int EC = 16 / (int)sizeof(T), KB = 4 * EC;     // k of one round of a wavefront's lanes
-  constexpr int kUnroll = CN == 1 ? 4 : 2;
-  __shared__ f32x4 red[3][2][CN][64];
+  constexpr int kUnroll = 4;
+  __shared__ f32x4 red[3][2][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, l = lane & 15;
   const long f0 = (long)blockIdx.x * 16;
   // rows and tokens past the end read the last one's: their results are not stored
-  const long f_row = f0 + l < a.nr ? f0 + l : a.nr - 1;
+  const long f_row = f0 + l < a.nr ? f0 + l : a.nr - 1, c_row = l < a.nc ? l : a.nc - 1;
   const T* wg = static_cast<const T*>(a.r[0]) + f_row * a.ldr;
   const T* wu = static_cast<const T*>(a.r[1]) + f_row * a.ldr;
-  const T* x[CN];
-#pragma unroll
-  for (int j = 0; j < CN; ++j) x[j] = static_cast<const T*>(a.c[0]) + (j * 16 + l < a.nc ? j * 16 + l : a.nc - 1) * a.ldc;
-  f32x4 acc[2][CN];
-#pragma unroll
-  for (int j = 0; j < CN; ++j) acc[0][j] = acc[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const T* x = static_cast<const T*>(a.c[0]) + c_row * a.ldc;
+  f32x4 acc[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
   const int rounds = (int)((a.nk + KB - 1) / KB);
   for (int q0 = wave * kUnroll; q0 < rounds; q0 += 4 * kUnroll) {
-    Vec16<T> rg[kUnroll], ru[kUnroll], cf[kUnroll][CN];
+    Vec16<T> rg[kUnroll], ru[kUnroll], cf[kUnroll];
     if ((long)(q0 + kUnroll) * KB <= a.nk) {        // all of it inside: loads without conditions, all in flight
 #pragma unroll
       for (int q = 0; q < kUnroll; ++q) {
         const long k = (long)(q0 + q) * KB + g * EC;
         rg[q].load(wg + k);
         ru[q].load(wu + k);
-#pragma unroll
-        for (int j = 0; j < CN; ++j) cf[q][j].load(x[j] + k);
+        cf[q].load(x + k);
       }
     } else {
 #pragma unroll
@@ -696,59 +708,43 @@ template <typename T, int CN> __global__ __launch_bounds__(256) void gff_few_ker
         const long k = (long)(q0 + q) * KB + g * EC;
         rg[q].load_upto(wg + k, a.nk - k);
         ru[q].load_upto(wu + k, a.nk - k);
-#pragma unroll
-        for (int j = 0; j < CN; ++j) cf[q][j].load_upto(x[j] + k, a.nk - k);
+        cf[q].load_upto(x + k, a.nk - k);
       }
     }
 #pragma unroll
-    for (int q = 0; q < kUnroll; ++q)
-#pragma unroll
-      for (int j = 0; j < CN; ++j) {
-        const u32x4 c = __builtin_bit_cast(u32x4, cf[q][j].v);
-        acc[0][j] = mma(__builtin_bit_cast(u32x4, rg[q].v), c, acc[0][j], T{});
-        acc[1][j] = mma(__builtin_bit_cast(u32x4, ru[q].v), c, acc[1][j], T{});
-      }
+    for (int q = 0; q < kUnroll; ++q) {
+      const u32x4 c = __builtin_bit_cast(u32x4, cf[q].v);
+      acc[0] = mma(__builtin_bit_cast(u32x4, rg[q].v), c, acc[0], T{});
+      acc[1] = mma(__builtin_bit_cast(u32x4, ru[q].v), c, acc[1], T{});
+    }
   }
   if (wave > 0) {
-#pragma unroll
-    for (int j = 0; j < CN; ++j) {
-      red[wave - 1][0][j][lane] = acc[0][j];
-      red[wave - 1][1][j][lane] = acc[1][j];
-    }
+    red[wave - 1][0][lane] = acc[0];
+    red[wave - 1][1][lane] = acc[1];
   }
   __syncthreads();
-  if (wave > 0) return;
-  const long f = f0 + g * 4;
-  const int nf = (int)(a.nr - f < 4 ? a.nr - f : 4);
-  float bg[4] = {0.f, 0.f, 0.f, 0.f}, bu[4] = {0.f, 0.f, 0.f, 0.f};
-  if (a.bias[0]) load4(static_cast<const T*>(a.bias[0]) + f, nf, false, bg);
-  if (a.bias[1]) load4(static_cast<const T*>(a.bias[1]) + f, nf, false, bu);
-  const bool vec = nf == 4 && (a.ldo & 3) == 0 && ((size_t)a.out[0] & (4 * sizeof(T) - 1)) == 0;
+  if (wave > 0 || l >= a.nc) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    acc[0] += red[w][0][lane];
+    acc[1] += red[w][1][lane];
+  }
+  const T* bg = static_cast<const T*>(a.bias[0]);
+  const T* bu = static_cast<const T*>(a.bias[1]);
+  T* out = static_cast<T*>(a.out[0]) + l * a.ldo;
   with_activation<kAnyActivation>(a.activation, [&](auto kind) __attribute__((always_inline)) {
-    constexpr int KIND = decltype(kind)::value;
 #pragma unroll
-    for (int j = 0; j < CN; ++j) {
-      f32x4 s0 = acc[0][j], s1 = acc[1][j];
-#pragma unroll
-      for (int w = 0; w < 3; ++w) {
-        s0 += red[w][0][j][lane];
-        s1 += red[w][1][j][lane];
-      }
-      const long c = j * 16 + l;
-      if (c >= a.nc) continue;
-      float o[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = activate<T, KIND>(s0[q] + bg[q]) * (s1[q] + bu[q]);
-      store4(static_cast<T*>(a.out[0]) + c * a.ldo + f, nf, vec, o);
+    for (int q = 0; q < 4; ++q) {
+      const long f = f0 + g * 4 + q;
+      if (f >= a.nr) continue;
+      const float gate = acc[0][q] + (bg ? (float)bg[f] : 0.f), up = acc[1][q] + (bu ? (float)bu[f] : 0.f);
+      out[f] = (T)(activate<T, decltype(kind)::value>(gate) * up);
     }
   });
 }
 
 template <typename T> int launch_few(const Args& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.nr + 15) / 16)), block(256);
-  if (a.nc <= 16) hipLaunchKernelGGL((gff_few_kernel<T, 1>), grid, block, 0, s, a);
-  else if (a.nc <= 32) hipLaunchKernelGGL((gff_few_kernel<T, 2>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((gff_few_kernel<T, 4>), grid, block, 0, s, a);
+  hipLaunchKernelGGL((gff_few_kernel<T>), dim3((unsigned)((a.nr + 15) / 16)), dim3(256), 0, s, a);
   return MZ_OK;
 }
 

@@ -24,66 +24,100 @@ int launch(const Args& a, int dtype, int mode, int tile, hipStream_t s) {
                             : mz_gff::launch_f16(a, mode, tile, s);
 }
 
-// out[p][c][r] = sum over the splits of partial[split][p][c][r]
-template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(const float* __restrict__ partial, int splits, long per_problem,
-                                                   int problems, T* out0, T* out1) {
-  const long n = per_problem * problems;
-  for (long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long)gridDim.x * 1024) {
+int launch_both(const Args& x, const Args& w, int dtype, int tile, hipStream_t s) {
+  return dtype == MZ_F32 ? mz_gff::launch_both_f32(x, w, tile, s)
+         : dtype == MZ_BF16 ? mz_gff::launch_both_bf16(x, w, tile, s)
+                            : mz_gff::launch_both_f16(x, w, tile, s);
+}
+
+// What is left of a backward pass, in one launch: cut sums joined - out[p][c][r] = sum over the splits of
+// partial[split][p][c][r] - and the bias gradients, dbias[side][f] = sum over the token tiles of col[tile][side][f].
+struct Join {
+  const float* partial;
+  long n, per_problem;       // elements of all problems, of one
+  int splits;
+  void* out[2];
+  unsigned blocks;
+};
+struct Finish {
+  Join join[2];
+  const float* col;
+  long tiles, F;
+  void* dbias[2];
+  unsigned bias_blocks;
+};
+
+template <typename T> __device__ __forceinline__ void join_part(const Join& j, unsigned block) {
+  T* out0 = static_cast<T*>(j.out[0]);
+  T* out1 = static_cast<T*>(j.out[1]);
+  for (long i = ((long)block * 256 + threadIdx.x) * 4; i < j.n; i += (long)j.blocks * 1024) {
     float v[4] = {0.f, 0.f, 0.f, 0.f};
-    const int m = (int)(n - i < 4 ? n - i : 4);
-    for (int s = 0; s < splits; ++s) {
-      const float* p = partial + s * n + i;
-      if (m == 4 && (n & 3) == 0) {
-        const float4 t = *reinterpret_cast<const float4*>(p);
+    const int m = (int)(j.n - i < 4 ? j.n - i : 4);
+    if (m == 4 && (j.n & 3) == 0) {
+#pragma unroll 4
+      for (int s = 0; s < j.splits; ++s) {
+        const float4 t = *reinterpret_cast<const float4*>(j.partial + s * j.n + i);
         v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
-      } else {
-        for (int j = 0; j < m; ++j) v[j] += p[j];
       }
+    } else {
+      for (int s = 0; s < j.splits; ++s)
+        for (int q = 0; q < m; ++q) v[q] += j.partial[s * j.n + i + q];
     }
-    for (int j = 0; j < m; ++j) {
-      const long e = i + j;
-      if (e < per_problem) out0[e] = (T)v[j];
-      else out1[e - per_problem] = (T)v[j];
+    for (int q = 0; q < m; ++q) {
+      const long e = i + q;
+      if (e < j.per_problem) out0[e] = (T)v[q];
+      else out1[e - j.per_problem] = (T)v[q];
     }
   }
 }
-template <typename T> void join_t(const Args& a, int problems, hipStream_t s) {
-  const long n = a.nr * a.nc * problems, want = (n + 1023) / 1024, cap = 8L * mz::compute_units();
-  hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(want < cap ? want : cap)), dim3(256), 0, s, a.partial, a.splits,
-                     a.nr * a.nc, problems, static_cast<T*>(a.out[0]), static_cast<T*>(a.out[1]));
-}
-void join(const Args& a, int problems, int dtype, hipStream_t s) {
-  if (dtype == MZ_F32) join_t<float>(a, problems, s);
-  else if (dtype == MZ_BF16) join_t<__bf16>(a, problems, s);
-  else join_t<_Float16>(a, problems, s);
-}
 
-// bias gradients: dbias[side][f] = sum over the token tiles of col_partial[tile][side][f]; 32 features x 32 tile lanes
-template <typename T>
-__global__ __launch_bounds__(1024) void bias_grad_kernel(const float* __restrict__ partial, long tiles, long F, T* dbg, T* dbu) {
-  __shared__ float red[2][32][33];
-  const int col = threadIdx.x & 31, lane = threadIdx.x >> 5;
-  const long f = (long)blockIdx.x * 32 + col;
+template <typename T> __global__ __launch_bounds__(256) void finish_kernel(Finish f) {
+  __shared__ float red[2][32][9];
+  unsigned b = blockIdx.x;
+  if (b < f.join[0].blocks) return join_part<T>(f.join[0], b);
+  b -= f.join[0].blocks;
+  if (b < f.join[1].blocks) return join_part<T>(f.join[1], b);
+  b -= f.join[1].blocks;
+  const int col = threadIdx.x & 7, lane = threadIdx.x >> 3;             // 8 features, 32 tile lanes
+  const long c = (long)b * 8 + col;
   float g = 0.f, u = 0.f;
-  if (f < F)
-    for (long t = lane; t < tiles; t += 32) {
-      g += partial[(t * 2 + 0) * F + f];
-      u += partial[(t * 2 + 1) * F + f];
+  if (c < f.F) {
+    for (long t0 = lane; t0 < f.tiles; t0 += 32 * 4) {                  // eight loads in flight
+      float v[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long t = t0 + 32 * i;
+        v[0][i] = t < f.tiles ? f.col[(t * 2 + 0) * f.F + c] : 0.f;
+        v[1][i] = t < f.tiles ? f.col[(t * 2 + 1) * f.F + c] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        g += v[0][i];
+        u += v[1][i];
+      }
     }
+  }
   red[0][lane][col] = g;
   red[1][lane][col] = u;
   __syncthreads();
-  if (lane >= 2 || f >= F) return;
+  if (lane >= 2 || c >= f.F) return;
   float v = 0.f;
 #pragma unroll
   for (int k = 0; k < 32; ++k) v += red[lane][k][col];
-  T* out = lane == 0 ? dbg : dbu;
-  if (out) out[f] = (T)v;
+  T* out = static_cast<T*>(f.dbias[lane]);
+  if (out) out[c] = (T)v;
 }
-template <typename T> void bias_grad_t(const float* p, long tiles, long F, void* g, void* u, hipStream_t s) {
-  hipLaunchKernelGGL((bias_grad_kernel<T>), dim3((unsigned)((F + 31) / 32)), dim3(1024), 0, s, p, tiles, F,
-                     static_cast<T*>(g), static_cast<T*>(u));
+
+Join make_join(const Args& a, int problems) {
+  const long n = a.nr * a.nc * problems, want = (n + 1023) / 1024, cap = 8L * mz::compute_units();
+  return {a.partial, n, a.nr * a.nc, a.splits, {a.out[0], a.out[1]}, (unsigned)(want < cap ? want : cap)};
+}
+void finish(const Finish& f, int dtype, hipStream_t s) {
+  const dim3 grid(f.join[0].blocks + f.join[1].blocks + f.bias_blocks);
+  if (grid.x == 0) return;
+  if (dtype == MZ_F32) hipLaunchKernelGGL((finish_kernel<float>), grid, dim3(256), 0, s, f);
+  else if (dtype == MZ_BF16) hipLaunchKernelGGL((finish_kernel<__bf16>), grid, dim3(256), 0, s, f);
+  else hipLaunchKernelGGL((finish_kernel<_Float16>), grid, dim3(256), 0, s, f);
 }
 
 int64_t tiles(int64_t nr, int64_t nc, int tr, int bc) { return ((nr + tr - 1) / tr) * ((nc + bc - 1) / bc); }
@@ -102,16 +136,20 @@ struct TileCost {
 constexpr TileCost kCost16[3] = {{1, 1.4f, 1.45f, {7.f, 14.f, 8.f}}, {2, .58f, .5f, {3.5f, 6.f, 4.5f}}, {5, .34f, .23f, {2.2f, 4.5f, 2.5f}}};
 constexpr TileCost kCost32[3] = {{}, {2, 2.1f, 1.95f, {4.f, 8.f, 5.f}}, {5, .72f, .53f, {2.5f, 4.f, 3.f}}};
 
-struct Split { int tile, splits, steps; };
+struct Split {
+  int tile, splits, steps;
+  float time;
+  int64_t groups;                                  // workgroups
+};
 constexpr int kMaxSplits = 32;
 
-Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode) {
+Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only = -1) {
   const bool pair = mode <= mz_gff::kGateGrad;
   const int problems = mode == mz_gff::kWeightGrad ? 2 : 1;
   const int cus = 256;                             // of an MI355X: the choice, and with it a sum's order, is the same everywhere
-  Split best = {2, 1, (int)steps};
-  float least = -1.f;
+  Split best = {2, 1, (int)steps, -1.f, 0};
   for (int t = dtype == MZ_F32 ? 1 : 0; t < 3; ++t) {
+    if (only >= 0 && t != only) continue;
     const TileCost& c = (dtype == MZ_F32 ? kCost32 : kCost16)[t];
     const int side = mz_gff::tile_side(t);
     const int64_t whole = tiles(nr, nc, pair ? side / 2 : side, side) * problems;
@@ -125,10 +163,7 @@ Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode) {
       };
       float time = rounds * round(c.at_once) + (rest ? round(rest) : 0.f);
       if (splits > 1) time += 3.f + (float)(nr * nc * problems) * splits * 8.f / 8e6f;
-      if (least < 0.f || time < least) {
-        least = time;
-        best = {t, (int)splits, (int)per};
-      }
+      if (best.time < 0.f || time < best.time) best = {t, (int)splits, (int)per, time, whole * splits};
     }
   }
   return best;
@@ -153,23 +188,40 @@ Shape make_shape(int64_t M, int64_t K, int64_t F, int dtype) {
   const int e = unit_elems(dtype);
   return {M, K, F, round_up(F, e), dtype, K % e != 0};
 }
-constexpr int64_t kFew = 64;   // tokens the streaming kernel takes
+// Tokens the streaming kernel takes: at 16, 2048 x 2048 bf16 7.7 us (64 x 64 tiles 11.8), 1000 x 5000 float32 12.7
+// (23.4), 4096 x 16384 bf16 out of the caches 47 (43); at 32, with two blocks of tokens, 9.8 (12.0), 19.9 (23.6), 59 (43).
+constexpr int64_t kFew = 16;
 
 struct Backward {
   Split dx, dw;
+  bool both;                 // the two products fit on the chip together: one launch, in the same tiles
   int gate_tile;
-  int64_t dgu_bytes, col_bytes, partial_bytes;
+  int64_t dgu_bytes, col_bytes, dx_bytes, dw_bytes;
 };
 Backward plan_backward(const Shape& h) {
   Backward b;
   b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad).tile;
-  b.dx = pick(h.K, h.M, 2 * h.steps(h.nk_F()), h.dtype, mz_gff::kInputGrad);
-  b.dw = pick(h.K, h.F, h.steps(h.nk_M()), h.dtype, mz_gff::kWeightGrad);
+  const int64_t fs = 2 * h.steps(h.nk_F()), ms = h.steps(h.nk_M());
+  b.dx = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad);
+  b.dw = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad);
+  // side by side, where one round of workgroups holds both: the longer of the two, not their sum
+  b.both = false;
+  float least = b.dx.time + b.dw.time;
+  for (int t = 1; t < 3; ++t) {
+    const Split x = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, t), w = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, t);
+    const int64_t room = 256 * (h.dtype == MZ_F32 ? kCost32 : kCost16)[t].at_once;
+    const float longer = x.time > w.time ? x.time : w.time, time = longer + .3f * (x.time + w.time - longer);
+    if (x.groups + w.groups > room || time >= least) continue;
+    b.both = true;
+    least = time;
+    b.dx = x;
+    b.dw = w;
+  }
   b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
   const int side = mz_gff::tile_side(b.gate_tile);
   b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
-  const int64_t px = b.dx.splits > 1 ? b.dx.splits * h.M * h.K * 4 : 0, pw = b.dw.splits > 1 ? b.dw.splits * 2 * h.F * h.K * 4 : 0;
-  b.partial_bytes = round_up(px > pw ? px : pw, 256);
+  b.dx_bytes = b.dx.splits > 1 ? round_up(b.dx.splits * h.M * h.K * 4, 256) : 0;
+  b.dw_bytes = b.dw.splits > 1 ? round_up(b.dw.splits * 2 * h.F * h.K * 4, 256) : 0;
   return b;
 }
 
@@ -195,7 +247,7 @@ int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dty
   if (check_shape("mz_gated_ff_workspace_bytes", M, K, F, dtype, 0)) return -1;
   if (!backward) return 0;
   const Backward b = plan_backward(make_shape(M, K, F, dtype));
-  return 2 * b.dgu_bytes + b.col_bytes + b.partial_bytes;
+  return 2 * b.dgu_bytes + b.col_bytes + b.dx_bytes + b.dw_bytes;
 }
 
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
@@ -244,7 +296,7 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   char* dg = static_cast<char*>(workspace);
   char* du = dg + plan.dgu_bytes;
   float* cols = reinterpret_cast<float*>(du + plan.dgu_bytes);
-  float* partial = reinterpret_cast<float*>(du + plan.dgu_bytes + plan.col_bytes);
+  char* partial = du + plan.dgu_bytes + plan.col_bytes;
   const bool biases = db_gate || db_up;
 
   Args a = {};                                     // dg, du
@@ -261,37 +313,41 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   a.splits = 1;
   a.steps_per_split = (int)sh.steps(a.nk);
   if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
+  Args p = {}, q = {};                             // dx; dw
+  p.r[0] = w_gate; p.r[1] = w_up;
+  p.c[0] = dg; p.c[1] = du;
+  p.ldr = K; p.ldc = sh.Fp;
+  p.nr = K; p.nc = M; p.nk = sh.nk_F(); p.nk_all = F;
+  p.out[0] = p.out[1] = dx; p.ldo = K;
+  p.partial = reinterpret_cast<float*>(partial);
+  p.splits = plan.dx.splits; p.steps_per_split = plan.dx.steps;
+  q.r[0] = q.r[1] = x;
+  q.c[0] = dg; q.c[1] = du;
+  q.ldr = ldx; q.ldc = sh.Fp;
+  q.nr = K; q.nc = F; q.nk = sh.nk_M(); q.nk_all = M;
+  q.out[0] = dw_gate; q.out[1] = dw_up; q.ldo = K;
+  q.partial = reinterpret_cast<float*>(partial + plan.dx_bytes);
+  q.splits = plan.dw.splits; q.steps_per_split = plan.dw.steps;
+  if (plan.both && dx && dw_gate) {
+    if (int rc = launch_both(p, q, dtype, plan.dx.tile, s)) return rc;
+  } else {
+    if (dx)
+      if (int rc = launch(p, dtype, mz_gff::kInputGrad, plan.dx.tile, s)) return rc;
+    if (dw_gate)
+      if (int rc = launch(q, dtype, mz_gff::kWeightGrad, plan.dw.tile, s)) return rc;
+  }
+  Finish f = {};
+  if (dx && p.splits > 1) f.join[0] = make_join(p, 1);
+  if (dw_gate && q.splits > 1) f.join[1] = make_join(q, 2);
   if (biases) {
     const int side = mz_gff::tile_side(plan.gate_tile);
-    const long n = (long)((M + side - 1) / side);
-    if (dtype == MZ_F32) bias_grad_t<float>(cols, n, F, db_gate, db_up, s);
-    else if (dtype == MZ_BF16) bias_grad_t<__bf16>(cols, n, F, db_gate, db_up, s);
-    else bias_grad_t<_Float16>(cols, n, F, db_gate, db_up, s);
+    f.col = cols;
+    f.tiles = (M + side - 1) / side;
+    f.F = F;
+    f.dbias[0] = db_gate; f.dbias[1] = db_up;
+    f.bias_blocks = (unsigned)((F + 7) / 8);
   }
-  if (dx) {
-    Args p = {};
-    p.r[0] = w_gate; p.r[1] = w_up;
-    p.c[0] = dg; p.c[1] = du;
-    p.ldr = K; p.ldc = sh.Fp;
-    p.nr = K; p.nc = M; p.nk = sh.nk_F(); p.nk_all = F;
-    p.out[0] = p.out[1] = dx; p.ldo = K;
-    p.partial = partial;
-    p.splits = plan.dx.splits; p.steps_per_split = plan.dx.steps;
-    if (int rc = launch(p, dtype, mz_gff::kInputGrad, plan.dx.tile, s)) return rc;
-    if (p.splits > 1) join(p, 1, dtype, s);
-  }
-  if (dw_gate) {
-    Args p = {};
-    p.r[0] = p.r[1] = x;
-    p.c[0] = dg; p.c[1] = du;
-    p.ldr = ldx; p.ldc = sh.Fp;
-    p.nr = K; p.nc = F; p.nk = sh.nk_M(); p.nk_all = M;
-    p.out[0] = dw_gate; p.out[1] = dw_up; p.ldo = K;
-    p.partial = partial;
-    p.splits = plan.dw.splits; p.steps_per_split = plan.dw.steps;
-    if (int rc = launch(p, dtype, mz_gff::kWeightGrad, plan.dw.tile, s)) return rc;
-    if (p.splits > 1) join(p, 2, dtype, s);
-  }
+  finish(f, dtype, s);
   return mz::check_launch("mz_gated_ff_bwd");
 }
 
