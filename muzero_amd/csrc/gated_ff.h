@@ -28,11 +28,12 @@ enum Activation { kSilu = 0, kGelu = 1, kRelu = 2, kSigmoid = 3 };
 struct Args {
   // operands: one matrix for gate and one for up where there are two, the same twice where there is one
   const void* r[2];
-  const void* c[2];
+  const void* c[4];          // kInputGrad: dg, du and, with parts, dg_lo, du_lo; kWeightGrad: the same
+  int parts;                 // 1, or 2: dg and du come as two terms, the rounded value and what rounding left
   long ldr, ldc;             // elements between rows of the matrices as they lie in memory
   long nr, nc, nk;           // extents of r (kForward / kGateGrad: features), c and k - the k that the steps take
   long nk_all;               // all k: nk .. nk_all - 1 are added element by element, at most tail_units(mode) 16-byte units of them
-  void* out[2];
+  void* out[4];              // kGateGrad: dg, du and, with parts, dg_lo, du_lo
   long ldo;
   const void* bias[2];
   const void* dh;            // kGateGrad: [nc][nr]
@@ -268,9 +269,18 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
     for (int i = 0; i < kHalf; ++i) opr.off[kHalf + i] = opr.off[i];
   }
   opc.init(tid, a.ldc, a.nc - c0);
-  // steps: kInputGrad runs over the features of dg and then over those of du
+  // steps: kInputGrad runs over the features of dg and then over those of du; where these come in two parts - small
+  // problems, in the smallest tiles - the second parts' steps follow the first's
+  constexpr int kParts = BR == 64 && sizeof(T) == 2 && !kPair ? 2 : 1, kSides = MODE == kInputGrad ? 2 : 1, kSegs = kParts * kSides;
   const long seg_steps = (a.nk + KS - 1) / KS;
-  const long all_steps = MODE == kInputGrad ? 2 * seg_steps : seg_steps;
+  const int segs = kSides * (kParts == 2 ? a.parts : 1);
+  const long all_steps = seg_steps * segs;
+  auto c_matrix = [&](int seg) __attribute__((always_inline)) {
+    const int i = MODE == kInputGrad ? seg : which + 2 * seg;
+    const void* m = i == 0 ? a.c[0] : a.c[1];
+    if constexpr (kParts == 2) m = i < 2 ? m : i == 2 ? a.c[2] : a.c[3];
+    return static_cast<const T*>(m);
+  };
   const long first = (long)split * a.steps_per_split;
   const long last = first + a.steps_per_split < all_steps ? first + a.steps_per_split : all_steps;
 
@@ -282,11 +292,13 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
     int k_left;
   };
   auto source = [&](long s) __attribute__((always_inline)) {
-    const int seg = MODE == kInputGrad && s >= seg_steps ? 1 : 0;
+    int seg = 0;
+#pragma unroll
+    for (int i = 1; i < kSegs; ++i) seg += i < segs && s >= i * seg_steps ? 1 : 0;   // past the end: in the last, behind its k
     const long k0 = (s - seg * seg_steps) * KS, left = a.nk - k0;
-    const T* cm = static_cast<const T*>(a.c[MODE == kWeightGrad ? which : seg]);
-    const T* rm0 = static_cast<const T*>(a.r[seg]);
-    const T* rm1 = static_cast<const T*>(a.r[kPair ? 1 : seg]);
+    const T* cm = c_matrix(seg);
+    const T* rm0 = static_cast<const T*>(MODE == kInputGrad && (seg & 1) ? a.r[1] : a.r[0]);
+    const T* rm1 = kPair ? static_cast<const T*>(a.r[1]) : rm0;
     const long ro = kPair ? r0 * a.ldr + k0 : k0 * a.ldr + r0, co = kCAcross ? k0 * a.ldc + c0 : c0 * a.ldc + k0;
     Source src;
     src.r[0] = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(rm0) + ro, 0, 0x7fffffff, 0x00020000);
@@ -393,35 +405,35 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
   __syncthreads();               // the epilogue uses the buffers
   __builtin_amdgcn_sched_barrier(0);                                  // and none of its registers before
 
-  // ---- the k left out of the steps: staged as rows of one unit (kInputGrad: two of dg's and two of du's), one more half
-  // step
+  // ---- the k left out of the steps: staged as rows of one unit (kInputGrad: two) for each of dg, du and their second
+  // parts, one or two more half steps
   if (a.nk_all > a.nk && split == a.splits - 1) {
     using TailR = Operand<T, false, BR, NT>;
     using TailC = Operand<T, false, BC, NT>;
+    constexpr int kTail = tail_units(MODE);
     for (int row = tid; row < BR + BC; row += NT) {
       const bool is_r = row < BR;
       const int q = is_r ? row : row - BR;
       char* base = lds + (is_r ? 0 : BR * 128) + q * 128;
 #pragma unroll
-      for (int unit = 0; unit < 4; ++unit) {
-        constexpr int kTail = tail_units(MODE);
-        const int seg = MODE == kInputGrad ? unit / kTail : 0;
+      for (int unit = 0; unit < (kSegs * kTail > 4 ? 8 : 4); ++unit) {
+        const int seg = unit / kTail;
         const long k = a.nk + unit % kTail * OpR::EC;
         Vec16<T> e;
 #pragma unroll
         for (int t = 0; t < OpR::EC; ++t) e.v[t] = (T)0.f;
-        if (MODE == kInputGrad || unit < kTail) {
+        if (seg < kSegs && (seg < kSides || a.parts == 2)) {
           const T* p;
           long along;              // elements between k's
           bool exists;
           if (is_r) {
             const int r = kPair ? q % TR : q;
             exists = r0 + r < a.nr;
-            p = static_cast<const T*>(a.r[kPair ? q / TR : seg]) + (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
+            p = static_cast<const T*>((kPair ? q / TR : MODE == kInputGrad ? seg & 1 : 0) ? a.r[1] : a.r[0]) + (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
             along = kRAcross ? a.ldr : 1;
           } else {
             exists = c0 + q < a.nc;
-            p = static_cast<const T*>(a.c[MODE == kWeightGrad ? which : seg]) + (kCAcross ? k * a.ldc + c0 + q : (c0 + q) * a.ldc + k);
+            p = c_matrix(seg) + (kCAcross ? k * a.ldc + c0 + q : (c0 + q) * a.ldc + k);
             along = kCAcross ? a.ldc : 1;
           }
 #pragma unroll
@@ -433,12 +445,15 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < CN; ++j) cf[0][j] = TailC::fragment(lds + BR * 128, wc * CN + j, 0, lane);
+    for (int sub = 0; sub < (kSegs * kTail > 4 ? 2 : 1); ++sub) {
 #pragma unroll
-    for (int i = 0; i < RM; ++i) {
-      rf[i] = TailR::fragment(lds, r_block(i), 0, lane);
+      for (int j = 0; j < CN; ++j) cf[0][j] = TailC::fragment(lds + BR * 128, wc * CN + j, sub, lane);
 #pragma unroll
-      for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
+      for (int i = 0; i < RM; ++i) {
+        rf[i] = TailR::fragment(lds, r_block(i), sub, lane);
+#pragma unroll
+        for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
+      }
     }
     __syncthreads();
   }
@@ -460,7 +475,8 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
         }
     }
     const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
-    float* colsum = reinterpret_cast<float*>(lds + 3 * kRegion);      // kGateGrad: [WC][2][TR]
+    constexpr bool kLow = MODE == kGateGrad && BR == 64 && sizeof(T) == 2;      // second parts are written for small problems
+    float* colsum = reinterpret_cast<float*>(lds + (kLow ? 5 : 3) * kRegion);   // kGateGrad: [WC][2][TR]
     const int my_row = (wc * 16 + lc) * kPitch;                       // of a pass's region
     const long limit = (MODE == kGateGrad ? a.nr_pad : a.nr) - r0;    // columns of the outputs from r0 on
     with_activation<ACT>(a.activation, [&](auto kind) __attribute__((always_inline)) {
@@ -498,7 +514,7 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
           const int fr = (wr * (RM / 2) + i) * 16 + lr;               // feature within the tile
           const f32x4 g = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + fr);
           const f32x4 u = acc[i + RM / 2][j] + *reinterpret_cast<const f32x4*>(bias + TR + fr);
-          vec4<T> o0, o1;
+          vec4<T> o0, o1, l0, l1;
           if constexpr (MODE == kForward) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) o0[q] = (T)(activate<T, KIND>(g[q]) * u[q]);
@@ -515,8 +531,18 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
               su[i][q] += du;
               o0[q] = (T)dg;
               o1[q] = (T)du;
+              if constexpr (kLow) {
+                l0[q] = (T)(dg - (float)o0[q]);
+                l1[q] = (T)(du - (float)o1[q]);
+              }
             }
             *reinterpret_cast<vec4<T>*>(region + kRegion + my_row + fr * (int)sizeof(T)) = o1;
+            if constexpr (kLow) {
+              if (a.parts == 2) {
+                *reinterpret_cast<vec4<T>*>(region + 2 * kRegion + my_row + fr * (int)sizeof(T)) = l0;
+                *reinterpret_cast<vec4<T>*>(region + 3 * kRegion + my_row + fr * (int)sizeof(T)) = l1;
+              }
+            }
           }
           *reinterpret_cast<vec4<T>*>(region + my_row + fr * (int)sizeof(T)) = o0;
         }
@@ -527,7 +553,8 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
           const long c = c0 + pass_row(q, j), left = limit - f;
           if (q >= PR || c >= a.nc || left <= 0) continue;
 #pragma unroll
-          for (int w = 0; w < (MODE == kGateGrad ? 2 : 1); ++w) {
+          for (int w = 0; w < (kLow ? 4 : MODE == kGateGrad ? 2 : 1); ++w) {
+            if (w >= 2 && a.parts != 2) break;
             Vec16<T> o;
             o.load(reinterpret_cast<const T*>(region + w * kRegion + q * kPitch + f * (int)sizeof(T)));
             o.store_upto(static_cast<T*>(a.out[w]) + c * a.ldo + r0 + f, left);
@@ -585,7 +612,7 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
         }
       }
     };
-    if (a.splits == 1) finish(static_cast<T*>(a.out[which]), a.ldo);
+    if (a.splits == 1) finish(static_cast<T*>(which ? a.out[1] : a.out[0]), a.ldo);
     else finish(a.partial + ((long)split * problems + which) * a.nc * a.nr, a.nr);
   }
 }
@@ -595,7 +622,7 @@ template <typename T, int MODE, int BR, int BC, int WC> constexpr int lds_bytes(
   constexpr bool kPair = MODE <= mz_gff::kGateGrad;
   constexpr int TR = kPair ? BR / 2 : BR, PR = WC * 16, buffers = 2 * (BR + BC) * 128;
   constexpr int regions = MODE == mz_gff::kForward    ? 2 * PR * (TR * (int)sizeof(T) + 16)
-                          : MODE == mz_gff::kGateGrad ? 3 * PR * (TR * (int)sizeof(T) + 16) + WC * 2 * TR * 4
+                          : MODE == mz_gff::kGateGrad ? (BR == 64 ? 5 : 3) * PR * (TR * (int)sizeof(T) + 16) + WC * 2 * TR * 4
                                                       : 2 * PR * (BR * 4 + 16);
   static_assert(!kPair || regions <= buffers, "the biases lie behind the buffers");
   constexpr int bytes = (regions > buffers ? regions : buffers) + (kPair ? 2 * TR * 4 : 0);

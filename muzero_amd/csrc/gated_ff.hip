@@ -6,7 +6,8 @@
 // happen in its registers and only h is written.  Nothing else is kept for the backward pass: it computes g and u again
 // (4 M K F operations against 8 M F bytes written and read back in 16 bits - and without rounding g and u), writes
 // dg and du in the operands' type - they are matrix operands next, and their rounding adds one half step to a sum's
-// terms - and runs the two products that need them.  Sums over few tiles are split along k into float32 partial
+// terms, which averages out over a sum as long as they are many - and runs the two products that need them.  Where there
+// are few (16-bit types, M F <= 8192) what the rounding left goes along as a second operand of the same products.  Sums over few tiles are split along k into float32 partial
 // results that a second launch adds up in a fixed order: no atomics, the same bits on every run.
 #include "gated_ff.h"
 
@@ -194,20 +195,23 @@ constexpr int64_t kFew = 16;
 
 struct Backward {
   Split dx, dw;
+  int parts;                 // of dg and du (Args::parts)
   bool both;                 // the two products fit on the chip together: one launch, in the same tiles
   int gate_tile;
   int64_t dgu_bytes, col_bytes, dx_bytes, dw_bytes;
 };
 Backward plan_backward(const Shape& h) {
   Backward b;
-  b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad).tile;
-  const int64_t fs = 2 * h.steps(h.nk_F()), ms = h.steps(h.nk_M());
-  b.dx = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad);
-  b.dw = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad);
+  b.parts = h.dtype != MZ_F32 && h.M * h.F <= 8192 ? 2 : 1;
+  const int only = b.parts == 2 ? 2 : -1;          // in the smallest tiles
+  b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad, only).tile;
+  const int64_t fs = 2 * b.parts * h.steps(h.nk_F()), ms = b.parts * h.steps(h.nk_M());
+  b.dx = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, only);
+  b.dw = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, only);
   // side by side, where one round of workgroups holds both: the longer of the two, not their sum
   b.both = false;
   float least = b.dx.time + b.dw.time;
-  for (int t = 1; t < 3; ++t) {
+  for (int t = b.parts; t < 3; ++t) {
     const Split x = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, t), w = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, t);
     const int64_t room = 256 * (h.dtype == MZ_F32 ? kCost32 : kCost16)[t].at_once;
     const float longer = x.time > w.time ? x.time : w.time, time = longer + .3f * (x.time + w.time - longer);
@@ -247,7 +251,7 @@ int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dty
   if (check_shape("mz_gated_ff_workspace_bytes", M, K, F, dtype, 0)) return -1;
   if (!backward) return 0;
   const Backward b = plan_backward(make_shape(M, K, F, dtype));
-  return 2 * b.dgu_bytes + b.col_bytes + b.dx_bytes + b.dw_bytes;
+  return 2 * b.parts * b.dgu_bytes + b.col_bytes + b.dx_bytes + b.dw_bytes;
 }
 
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
@@ -295,8 +299,9 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   hipStream_t s = mz::as_stream(stream);
   char* dg = static_cast<char*>(workspace);
   char* du = dg + plan.dgu_bytes;
-  float* cols = reinterpret_cast<float*>(du + plan.dgu_bytes);
-  char* partial = du + plan.dgu_bytes + plan.col_bytes;
+  char* behind = dg + 2 * plan.parts * plan.dgu_bytes;   // dg, du [, dg_lo, du_lo]
+  float* cols = reinterpret_cast<float*>(behind);
+  char* partial = behind + plan.col_bytes;
   const bool biases = db_gate || db_up;
 
   Args a = {};                                     // dg, du
@@ -305,6 +310,8 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   a.ldr = K; a.ldc = ldx;
   a.nr = F; a.nc = M; a.nk = sh.nk_K(); a.nk_all = K;
   a.out[0] = dg; a.out[1] = du; a.ldo = sh.Fp;
+  a.parts = plan.parts;
+  if (plan.parts == 2) { a.out[2] = du + plan.dgu_bytes; a.out[3] = du + 2 * plan.dgu_bytes; }
   a.bias[0] = b_gate; a.bias[1] = b_up;
   a.dh = dh; a.lddh = F;
   a.col_partial = biases ? cols : nullptr;
@@ -315,14 +322,16 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
   Args p = {}, q = {};                             // dx; dw
   p.r[0] = w_gate; p.r[1] = w_up;
-  p.c[0] = dg; p.c[1] = du;
+  p.c[0] = dg; p.c[1] = du; p.c[2] = a.out[2]; p.c[3] = a.out[3];
+  p.parts = plan.parts;
   p.ldr = K; p.ldc = sh.Fp;
   p.nr = K; p.nc = M; p.nk = sh.nk_F(); p.nk_all = F;
   p.out[0] = p.out[1] = dx; p.ldo = K;
   p.partial = reinterpret_cast<float*>(partial);
   p.splits = plan.dx.splits; p.steps_per_split = plan.dx.steps;
   q.r[0] = q.r[1] = x;
-  q.c[0] = dg; q.c[1] = du;
+  q.c[0] = dg; q.c[1] = du; q.c[2] = a.out[2]; q.c[3] = a.out[3];
+  q.parts = plan.parts;
   q.ldr = ldx; q.ldc = sh.Fp;
   q.nr = K; q.nc = F; q.nk = sh.nk_M(); q.nk_all = M;
   q.out[0] = dw_gate; q.out[1] = dw_up; q.ldo = K;

@@ -197,8 +197,9 @@ def check_gated_ff(x, wg, wu, bg, bu, dh, activation, got):
     e_du = dhd.abs() * e_a + 2 * U * du.abs()
     r_dg, r_du = e_dg, e_du                      # rounded to the operands' type for the products, not for the biases
     if t != torch.float32:
-        r_dg = e_dg + half(t) * (dg.abs() + e_dg) + tiny(t)
-        r_du = e_du + half(t) * (du.abs() + e_du) + tiny(t)
+        step = half(t) if m * f > 8192 else half(t) ** 2         # few: in two parts, the second rounded
+        r_dg = e_dg + step * (dg.abs() + e_dg) + tiny(t)
+        r_du = e_du + step * (du.abs() + e_du) + tiny(t)
     if dx is not None:
         size = dg.abs() @ gd.abs() + du.abs() @ ud.abs()
         within(dx, dg @ gd + du @ ud, r_dg @ gd.abs() + r_du @ ud.abs() + (2 * f + 40) * U * size * 1.01, "dx")
@@ -230,7 +231,8 @@ def ff_run(x, wg, wu, bg, bu, dh, activation):
 # whole unit, whole steps and not; F likewise
 FF_SHAPES = [(1, 1, 1), (1, 256, 1024), (2, 7, 5), (16, 64, 33), (17, 96, 40), (33, 130, 48), (64, 257, 65), (65, 64, 64),
              (66, 33, 20), (128, 256, 128), (129, 264, 130), (300, 72, 1000), (1000, 257, 1001), (513, 520, 264), (4100, 64, 24),
-             (777, 8, 8), (2500, 512, 136), (300, 1, 200), (300, 2, 101), (200, 3, 70), (129, 5, 9), (70, 6, 16), (66, 4, 7)]
+             (777, 8, 8), (2500, 512, 136), (300, 1, 200), (300, 2, 101), (200, 3, 70), (129, 5, 9), (70, 6, 16), (66, 4, 7),
+             (1, 4096, 300), (3, 300, 2500), (40, 1001, 200), (8, 136, 1024)]
 
 
 @pytest.mark.parametrize("t", TYPES)
