@@ -226,7 +226,7 @@ __device__ __forceinline__ void half_step_order() {
 }
 
 template <typename T, int MODE, int BR, int BC, int WR, int WC, int ACT>
-__device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
+__device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks, char* lds) {
   using namespace mz_gff;
   constexpr int NT = WR * WC * 64;
   constexpr bool kPair = MODE == kForward || MODE == kGateGrad;       // a tile's R rows: half gate, half up features
@@ -241,21 +241,30 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wave / WC, wc = wave % WC;
 
-  // ---- this workgroup's tile.  Workgroups go to the 8 XCDs in turn: XCD x takes the x-th run of consecutive tiles, and
-  // consecutive tiles walk 8 tiles of c under each tile of r, so that an L2 holds what its workgroups share.
+  // ---- this workgroup's tiles.  Workgroups go to the 8 XCDs in turn: XCD x takes the x-th run of consecutive tiles, and
+  // consecutive tiles walk 8 tiles of c under each tile of r, so that an L2 holds what its workgroups share.  A pair
+  // product's workgroups stay for several tiles - the next one's first units are on their way while a tile's epilogue runs -
+  // the plain products' take one each.
   const unsigned tiles_r = (unsigned)((a.nr + TR - 1) / TR), tiles_c = (unsigned)((a.nc + BC - 1) / BC);
   const unsigned problems = MODE == kWeightGrad ? 2 : 1;
   const unsigned per_problem = tiles_r * tiles_c, total = per_problem * problems * (unsigned)a.splits;
   const unsigned per_xcd = (total + 7) / 8;
-  const unsigned id = (block & 7) * per_xcd + (block >> 3);
-  if (id >= total) return;
-  const unsigned job = id / per_problem, t = id - job * per_problem;
-  const int which = MODE == kWeightGrad ? (int)(job % 2) : 0;
-  const int split = (int)(MODE == kWeightGrad ? job / 2 : job);
+  const unsigned xcd0 = (block & 7) * per_xcd;                        // the XCD's first tile
+  unsigned local = block >> 3;                                        // of its run
+  if (local >= per_xcd || xcd0 + local >= total) return;
+  long r0 = 0, c0 = 0;
+  int which = 0, split = 0;
   constexpr unsigned kGroup = 8;
-  const unsigned band = t / (kGroup * tiles_r), in_band = t - band * (kGroup * tiles_r);
-  const unsigned band_c = tiles_c - band * kGroup < kGroup ? tiles_c - band * kGroup : kGroup;
-  const long r0 = (long)(in_band / band_c) * TR, c0 = (long)(band * kGroup + in_band % band_c) * BC;
+  auto locate = [&]() __attribute__((always_inline)) {
+    const unsigned id = xcd0 + local, job = id / per_problem, t = id - job * per_problem;
+    which = MODE == kWeightGrad ? (int)(job % 2) : 0;
+    split = (int)(MODE == kWeightGrad ? job / 2 : job);
+    const unsigned band = t / (kGroup * tiles_r), in_band = t - band * (kGroup * tiles_r);
+    const unsigned band_c = tiles_c - band * kGroup < kGroup ? tiles_c - band * kGroup : kGroup;
+    r0 = (long)(in_band / band_c) * TR;
+    c0 = (long)(band * kGroup + in_band % band_c) * BC;
+  };
+  locate();
 
   // ---- operands
   OpR opr;
@@ -263,12 +272,15 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
   // a pair tile's two halves are two matrices: the rounds of threads split evenly between them
   constexpr int kHalf = kPair ? OpR::UNITS / 2 : OpR::UNITS;
   static_assert(!kPair || (OpR::UNITS % 2 == 0 && kHalf * OpR::RPR == BR / 2), "rounds cover a half");
-  opr.init(tid, a.ldr, a.nr - r0);
-  if constexpr (kPair) {          // rows of the second half are rows 0 .. BR/2 of the other matrix
+  auto aim = [&]() __attribute__((always_inline)) {
+    opr.init(tid, a.ldr, a.nr - r0);
+    if constexpr (kPair) {        // rows of the second half are rows 0 .. BR/2 of the other matrix
 #pragma unroll
-    for (int i = 0; i < kHalf; ++i) opr.off[kHalf + i] = opr.off[i];
-  }
-  opc.init(tid, a.ldc, a.nc - c0);
+      for (int i = 0; i < kHalf; ++i) opr.off[kHalf + i] = opr.off[i];
+    }
+    opc.init(tid, a.ldc, a.nc - c0);
+  };
+  aim();
   // steps: kInputGrad runs over the features of dg and then over those of du; where these come in two parts - small
   // problems, in the smallest tiles - the second parts' steps follow the first's
   constexpr int kParts = BR == 64 && sizeof(T) == 2 && !kPair ? 2 : 1, kSides = MODE == kInputGrad ? 2 : 1, kSegs = kParts * kSides;
@@ -318,10 +330,6 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
   };
 
   f32x4 acc[RM][CN];
-#pragma unroll
-  for (int i = 0; i < RM; ++i)
-#pragma unroll
-    for (int j = 0; j < CN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   // the tile's 16-row block that this wavefront's block i is (pair tiles: the same features of both halves)
   auto r_block = [&](int i) {
     if constexpr (kPair) return (i / (RM / 2)) * (BR / 32) + wr * (RM / 2) + i % (RM / 2);
@@ -335,29 +343,22 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
   // outside) and stage zeros.
   constexpr int kMmas = sizeof(T) == 4 ? 4 : 1;
   u32x4 rf[RM], cf[2][CN];
-  {
-    const Source src = source(first), after = source(first + 1);
+  // the next tile's first units are loaded before this one's epilogue where the registers have room for them
+  constexpr bool kAhead = kPair && BR != 256;
+  auto start_tile = [&]() __attribute__((always_inline)) {
+    const Source src = source(first);
 #pragma unroll
     for (int u = 0; u < kUnits; ++u) load_unit(src, u);
-    if constexpr (kPair) {        // meanwhile the tile's biases, as float32 behind the two buffers: [gate, up][TR]
-      float* bias = reinterpret_cast<float*>(lds + 2 * (BR + BC) * 128);
-      for (int i = tid; i < 2 * TR; i += NT) {
-        const T* b = static_cast<const T*>(a.bias[i / TR]);
-        const long f = r0 + i % TR;
-        bias[i] = b && f < a.nr ? (float)b[f] : 0.f;
-      }
+  };
+  // the tile's biases, as float32 behind the two buffers: [gate, up][TR]
+  auto load_bias = [&]() __attribute__((always_inline)) {
+    float* bias = reinterpret_cast<float*>(lds + 2 * (BR + BC) * 128);
+    for (int i = tid; i < 2 * TR; i += NT) {
+      const T* b = static_cast<const T*>(a.bias[i / TR]);
+      const long f = r0 + i % TR;
+      bias[i] = b && f < a.nr ? (float)b[f] : 0.f;
     }
-#pragma unroll
-    for (int u = 0; u < kUnits; ++u) {
-      stage_unit(0, u);
-      load_unit(after, u);
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < CN; ++j) cf[0][j] = OpC::fragment(lds + BR * 128, wc * CN + j, 0, lane);
-#pragma unroll
-  for (int i = 0; i < RM; ++i) rf[i] = OpR::fragment(lds, r_block(i), 0, lane);
+  };
   // The epilogue goes over the tile in CN passes, each one 16-token block of every wavefront: values pass through LDS so
   // that memory is read and written in whole 16-byte units of consecutive features, whatever the rows' alignment.
   constexpr int PR = WC * 16;                                          // tokens of a pass
@@ -398,222 +399,267 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, char* lds) {
     }
     if constexpr (!LAST) half_step_order<0, RM, CN * kMmas, OpR::READS, CN, OpC::READS, 0>();
   };
-  int buf = 0;
-  for (long s = first; s + 1 < last; ++s, buf ^= 1)
-    step(lds + buf * ((BR + BC) * 128), lds + (buf ^ 1) * ((BR + BC) * 128), buf ^ 1, s, std::false_type{});
-  if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
-  __syncthreads();               // the epilogue uses the buffers
-  __builtin_amdgcn_sched_barrier(0);                                  // and none of its registers before
-
-  // ---- the k left out of the steps: staged as rows of one unit (kInputGrad: two) for each of dg, du and their second
-  // parts, one or two more half steps
-  if (a.nk_all > a.nk && split == a.splits - 1) {
-    using TailR = Operand<T, false, BR, NT>;
-    using TailC = Operand<T, false, BC, NT>;
-    constexpr int kTail = tail_units(MODE);
-    for (int row = tid; row < BR + BC; row += NT) {
-      const bool is_r = row < BR;
-      const int q = is_r ? row : row - BR;
-      char* base = lds + (is_r ? 0 : BR * 128) + q * 128;
+  start_tile();
+  for (;;) {
+    if constexpr (kPair) load_bias();
+    const Source second = source(first + 1);
 #pragma unroll
-      for (int unit = 0; unit < (kSegs * kTail > 4 ? 8 : 4); ++unit) {
-        const int seg = unit / kTail;
-        const long k = a.nk + unit % kTail * OpR::EC;
-        Vec16<T> e;
-#pragma unroll
-        for (int t = 0; t < OpR::EC; ++t) e.v[t] = (T)0.f;
-        if (seg < kSegs && (seg < kSides || a.parts == 2)) {
-          const T* p;
-          long along;              // elements between k's
-          bool exists;
-          if (is_r) {
-            const int r = kPair ? q % TR : q;
-            exists = r0 + r < a.nr;
-            p = static_cast<const T*>((kPair ? q / TR : MODE == kInputGrad ? seg & 1 : 0) ? a.r[1] : a.r[0]) + (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
-            along = kRAcross ? a.ldr : 1;
-          } else {
-            exists = c0 + q < a.nc;
-            p = c_matrix(seg) + (kCAcross ? k * a.ldc + c0 + q : (c0 + q) * a.ldc + k);
-            along = kCAcross ? a.ldc : 1;
-          }
-#pragma unroll
-          for (int t = 0; t < OpR::EC; ++t)
-            if (exists && k + t < a.nk_all) e.v[t] = p[t * along];
-        }
-        e.store(reinterpret_cast<T*>(base + TailR::place(q, unit) * 16));
-      }
+    for (int u = 0; u < kUnits; ++u) {
+      stage_unit(0, u);
+      load_unit(second, u);
     }
+#pragma unroll
+    for (int i = 0; i < RM; ++i)
+#pragma unroll
+      for (int j = 0; j < CN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
 #pragma unroll
-    for (int sub = 0; sub < (kSegs * kTail > 4 ? 2 : 1); ++sub) {
+    for (int j = 0; j < CN; ++j) cf[0][j] = OpC::fragment(lds + BR * 128, wc * CN + j, 0, lane);
 #pragma unroll
-      for (int j = 0; j < CN; ++j) cf[0][j] = TailC::fragment(lds + BR * 128, wc * CN + j, sub, lane);
-#pragma unroll
-      for (int i = 0; i < RM; ++i) {
-        rf[i] = TailR::fragment(lds, r_block(i), sub, lane);
-#pragma unroll
-        for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
-      }
-    }
-    __syncthreads();
-  }
+    for (int i = 0; i < RM; ++i) rf[i] = OpR::fragment(lds, r_block(i), 0, lane);
+    int buf = 0;
+    for (long s = first; s + 1 < last; ++s, buf ^= 1)
+      step(lds + buf * ((BR + BC) * 128), lds + (buf ^ 1) * ((BR + BC) * 128), buf ^ 1, s, std::false_type{});
+    if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
+    __syncthreads();               // the epilogue uses the buffers
+    __builtin_amdgcn_sched_barrier(0);                                  // and none of its registers before
 
-  // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
-  if constexpr (kPair) {
-    constexpr int kPitch = TR * (int)sizeof(T) + 16, kRegion = PR * kPitch;
-    // kGateGrad: the tile of dh, sent for as a whole where it has no ragged edge (16-bit types: 32 registers)
-    constexpr bool kDhAhead = MODE == kGateGrad && sizeof(T) == 2;
-    const bool full = r0 + TR <= a.nr && c0 + BC <= a.nc;
-    Vec16<T> dh_unit[kDhAhead ? CN : 1][PU];
-    if (kDhAhead && full) {
+    // ---- the k left out of the steps: staged as rows of one unit (kInputGrad: two) for each of dg, du and their second
+    // parts, one or two more half steps
+    if (a.nk_all > a.nk && split == a.splits - 1) {
+      using TailR = Operand<T, false, BR, NT>;
+      using TailC = Operand<T, false, BC, NT>;
+      constexpr int kTail = tail_units(MODE);
+      for (int row = tid; row < BR + BC; row += NT) {
+        const bool is_r = row < BR;
+        const int q = is_r ? row : row - BR;
+        char* base = lds + (is_r ? 0 : BR * 128) + q * 128;
 #pragma unroll
-      for (int j = 0; j < CN; ++j)
+        for (int unit = 0; unit < (kSegs * kTail > 4 ? 8 : 4); ++unit) {
+          const int seg = unit / kTail;
+          const long k = a.nk + unit % kTail * OpR::EC;
+          Vec16<T> e;
 #pragma unroll
-        for (int n = 0; n < PU; ++n) {
-          const int e = tid + n * NT < PR * EU ? tid + n * NT : 0;
-          dh_unit[kDhAhead ? j : 0][n].load(static_cast<const T*>(a.dh) + (c0 + pass_row(e / EU, j)) * a.lddh + r0 + e % EU * OpR::EC);
-        }
-    }
-    const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
-    constexpr bool kLow = MODE == kGateGrad && BR == 64 && sizeof(T) == 2;      // second parts are written for small problems
-    float* colsum = reinterpret_cast<float*>(lds + (kLow ? 5 : 3) * kRegion);   // kGateGrad: [WC][2][TR]
-    const int my_row = (wc * 16 + lc) * kPitch;                       // of a pass's region
-    const long limit = (MODE == kGateGrad ? a.nr_pad : a.nr) - r0;    // columns of the outputs from r0 on
-    with_activation<ACT>(a.activation, [&](auto kind) __attribute__((always_inline)) {
-      constexpr int KIND = decltype(kind)::value;
-      float sg[RM / 2][4], su[RM / 2][4];
-#pragma unroll
-      for (int i = 0; i < RM / 2; ++i)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) sg[i][q] = su[i][q] = 0.f;
-#pragma unroll
-      for (int j = 0; j < CN; ++j) {
-        char* region = lds + (MODE == kForward ? j & 1 : 1) * kRegion;  // kGateGrad: dh, dg, du
-        if constexpr (MODE == kGateGrad) {
-          if (kDhAhead && full) {
-#pragma unroll
-            for (int n = 0; n < PU; ++n) {
-              const int e = tid + n * NT;
-              if (e < PR * EU) dh_unit[kDhAhead ? j : 0][n].store(reinterpret_cast<T*>(lds + e / EU * kPitch + e % EU * 16));
+          for (int t = 0; t < OpR::EC; ++t) e.v[t] = (T)0.f;
+          if (seg < kSegs && (seg < kSides || a.parts == 2)) {
+            const T* p;
+            long along;              // elements between k's
+            bool exists;
+            if (is_r) {
+              const int r = kPair ? q % TR : q;
+              exists = r0 + r < a.nr;
+              p = static_cast<const T*>((kPair ? q / TR : MODE == kInputGrad ? seg & 1 : 0) ? a.r[1] : a.r[0]) + (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
+              along = kRAcross ? a.ldr : 1;
+            } else {
+              exists = c0 + q < a.nc;
+              p = c_matrix(seg) + (kCAcross ? k * a.ldc + c0 + q : (c0 + q) * a.ldc + k);
+              along = kCAcross ? a.ldc : 1;
             }
-          } else {
-#pragma unroll 1
-            for (int e = tid; e < PR * EU; e += NT) {
-              const int q = e / EU, f = e % EU * OpR::EC;
-              const long c = c0 + pass_row(q, j);
-              Vec16<T> d;
-              d.load_upto(static_cast<const T*>(a.dh) + c * a.lddh + r0 + f, c < a.nc ? a.nr - r0 - f : 0);
-              d.store(reinterpret_cast<T*>(lds + q * kPitch + f * (int)sizeof(T)));
-            }
+#pragma unroll
+            for (int t = 0; t < OpR::EC; ++t)
+              if (exists && k + t < a.nk_all) e.v[t] = p[t * along];
           }
-          __syncthreads();
-        }
-        const bool token = c0 + pass_row(wc * 16 + lc, j) < a.nc;
-#pragma unroll
-        for (int i = 0; i < RM / 2; ++i) {
-          const int fr = (wr * (RM / 2) + i) * 16 + lr;               // feature within the tile
-          const f32x4 g = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + fr);
-          const f32x4 u = acc[i + RM / 2][j] + *reinterpret_cast<const f32x4*>(bias + TR + fr);
-          vec4<T> o0, o1, l0, l1;
-          if constexpr (MODE == kForward) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) o0[q] = (T)(activate<T, KIND>(g[q]) * u[q]);
-          } else {
-            const vec4<T> d = *reinterpret_cast<const vec4<T>*>(lds + my_row + fr * (int)sizeof(T));
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float act, slope;
-              activate_grad<T, KIND>(g[q], act, slope);
-              // what lies past the last token or feature counts as zero, also as k of the input gradient (nr .. nr_pad)
-              const bool exists = token && r0 + fr + q < a.nr;
-              const float dg = exists ? (float)d[q] * u[q] * slope : 0.f, du = exists ? (float)d[q] * act : 0.f;
-              sg[i][q] += dg;
-              su[i][q] += du;
-              o0[q] = (T)dg;
-              o1[q] = (T)du;
-              if constexpr (kLow) {
-                l0[q] = (T)(dg - (float)o0[q]);
-                l1[q] = (T)(du - (float)o1[q]);
-              }
-            }
-            *reinterpret_cast<vec4<T>*>(region + kRegion + my_row + fr * (int)sizeof(T)) = o1;
-            if constexpr (kLow) {
-              if (a.parts == 2) {
-                *reinterpret_cast<vec4<T>*>(region + 2 * kRegion + my_row + fr * (int)sizeof(T)) = l0;
-                *reinterpret_cast<vec4<T>*>(region + 3 * kRegion + my_row + fr * (int)sizeof(T)) = l1;
-              }
-            }
-          }
-          *reinterpret_cast<vec4<T>*>(region + my_row + fr * (int)sizeof(T)) = o0;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < PU; ++n) {
-          const int e = tid + n * NT, q = e / EU, f = e % EU * OpR::EC;
-          const long c = c0 + pass_row(q, j), left = limit - f;
-          if (q >= PR || c >= a.nc || left <= 0) continue;
-#pragma unroll
-          for (int w = 0; w < (kLow ? 4 : MODE == kGateGrad ? 2 : 1); ++w) {
-            if (w >= 2 && a.parts != 2) break;
-            Vec16<T> o;
-            o.load(reinterpret_cast<const T*>(region + w * kRegion + q * kPitch + f * (int)sizeof(T)));
-            o.store_upto(static_cast<T*>(a.out[w]) + c * a.ldo + r0 + f, left);
-          }
+          e.store(reinterpret_cast<T*>(base + TailR::place(q, unit) * 16));
         }
       }
-      if constexpr (MODE == kGateGrad) {
-        if (a.col_partial) {       // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
+      __syncthreads();
 #pragma unroll
-          for (int i = 0; i < RM / 2; ++i)
+      for (int sub = 0; sub < (kSegs * kTail > 4 ? 2 : 1); ++sub) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int fr = (wr * (RM / 2) + i) * 16 + lr + q;
-              const float g = lanes_sum<16>(sg[i][q]), u = lanes_sum<16>(su[i][q]);
-              if (lc == 0) {
-                colsum[(wc * 2 + 0) * TR + fr] = g;
-                colsum[(wc * 2 + 1) * TR + fr] = u;
-              }
-            }
-          __syncthreads();
-          for (int i = tid; i < 2 * TR; i += NT) {
-            const int side = i / TR, f = i % TR;
-            if (r0 + f >= a.nr) continue;
-            float v = 0.f;
-#pragma unroll
-            for (int w = 0; w < WC; ++w) v += colsum[(w * 2 + side) * TR + f];
-            a.col_partial[((c0 / BC) * 2 + side) * a.nr + r0 + f] = v;
-          }
-        }
-      }
-    });
-  } else {
-    // out in elements of O: the result itself, or float32 partial results of a cut sum
-    auto finish = [&](auto* out, long ldo) __attribute__((always_inline)) {
-      using O = std::remove_pointer_t<decltype(out)>;
-      constexpr int EO = Vec16<O>::N, UO = BR / EO, kPitch = BR * (int)sizeof(O) + 16, kRegion = PR * kPitch;
-#pragma unroll
-      for (int j = 0; j < CN; ++j) {
-        char* region = lds + (j & 1) * kRegion;
+        for (int j = 0; j < CN; ++j) cf[0][j] = TailC::fragment(lds + BR * 128, wc * CN + j, sub, lane);
 #pragma unroll
         for (int i = 0; i < RM; ++i) {
-          vec4<O> o;
+          rf[i] = TailR::fragment(lds, r_block(i), sub, lane);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) o[q] = (O)acc[i][j][q];
-          *reinterpret_cast<vec4<O>*>(region + (wc * 16 + lc) * kPitch + ((wr * RM + i) * 16 + lr) * (int)sizeof(O)) = o;
-        }
-        __syncthreads();
-        for (int e = tid; e < PR * UO; e += NT) {
-          const int q = e / UO, r = e % UO * EO;
-          const long c = c0 + pass_row(q, j), left = a.nr - r0 - r;
-          if (c >= a.nc || left <= 0) continue;
-          Vec16<O> o;
-          o.load(reinterpret_cast<const O*>(region + q * kPitch + r * (int)sizeof(O)));
-          o.store_upto(out + c * ldo + r0 + r, left);
+          for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
         }
       }
-    };
-    if (a.splits == 1) finish(static_cast<T*>(which ? a.out[1] : a.out[0]), a.ldo);
-    else finish(a.partial + ((long)split * problems + which) * a.nc * a.nr, a.nr);
+      __syncthreads();
+    }
+
+    const long er = r0, ec = c0;     // the tile whose epilogue follows
+    bool more = false;
+    if constexpr (kAhead) {
+      local += blocks >> 3;
+      more = local < per_xcd && xcd0 + local < total;
+      if (more) {
+        locate();
+        aim();
+        if constexpr (kAhead) start_tile();
+      }
+    }
+
+    // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
+    if constexpr (kPair) {
+      constexpr int kPitch = TR * (int)sizeof(T) + 16, kRegion = PR * kPitch;
+      // kGateGrad: the tile of dh, sent for as a whole where it has no ragged edge (16-bit types: 32 registers)
+      constexpr bool kDhAhead = MODE == kGateGrad && sizeof(T) == 2;
+      const bool full = er + TR <= a.nr && ec + BC <= a.nc;
+      Vec16<T> dh_unit[kDhAhead ? CN : 1][PU];
+      if (kDhAhead && full) {
+#pragma unroll
+        for (int j = 0; j < CN; ++j)
+#pragma unroll
+          for (int n = 0; n < PU; ++n) {
+            const int e = tid + n * NT < PR * EU ? tid + n * NT : 0;
+            dh_unit[kDhAhead ? j : 0][n].load(static_cast<const T*>(a.dh) + (ec + pass_row(e / EU, j)) * a.lddh + er + e % EU * OpR::EC);
+          }
+      }
+      const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
+      constexpr bool kLow = MODE == kGateGrad && BR == 64 && sizeof(T) == 2;      // second parts are written for small problems
+      float* colsum = reinterpret_cast<float*>(lds + (kLow ? 5 : 3) * kRegion);   // kGateGrad: [WC][2][TR]
+      const int my_row = (wc * 16 + lc) * kPitch;                       // of a pass's region
+      const long limit = (MODE == kGateGrad ? a.nr_pad : a.nr) - er;    // columns of the outputs from er on
+      with_activation<ACT>(a.activation, [&](auto kind) __attribute__((always_inline)) {
+        constexpr int KIND = decltype(kind)::value;
+        float sg[RM / 2][4], su[RM / 2][4];
+#pragma unroll
+        for (int i = 0; i < RM / 2; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) sg[i][q] = su[i][q] = 0.f;
+#pragma unroll
+        for (int j = 0; j < CN; ++j) {
+          char* region = lds + (MODE == kForward ? j & 1 : 1) * kRegion;  // kGateGrad: dh, dg, du
+          if constexpr (MODE == kGateGrad) {
+            if (kDhAhead && full) {
+#pragma unroll
+              for (int n = 0; n < PU; ++n) {
+                const int e = tid + n * NT;
+                if (e < PR * EU) dh_unit[kDhAhead ? j : 0][n].store(reinterpret_cast<T*>(lds + e / EU * kPitch + e % EU * 16));
+              }
+            } else {
+#pragma unroll 1
+              for (int e = tid; e < PR * EU; e += NT) {
+                const int q = e / EU, f = e % EU * OpR::EC;
+                const long c = ec + pass_row(q, j);
+                Vec16<T> d;
+                d.load_upto(static_cast<const T*>(a.dh) + c * a.lddh + er + f, c < a.nc ? a.nr - er - f : 0);
+                d.store(reinterpret_cast<T*>(lds + q * kPitch + f * (int)sizeof(T)));
+              }
+            }
+            __syncthreads();
+          }
+          const bool token = ec + pass_row(wc * 16 + lc, j) < a.nc;
+#pragma unroll
+          for (int i = 0; i < RM / 2; ++i) {
+            const int fr = (wr * (RM / 2) + i) * 16 + lr;               // feature within the tile
+            const f32x4 g = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + fr);
+            const f32x4 u = acc[i + RM / 2][j] + *reinterpret_cast<const f32x4*>(bias + TR + fr);
+            vec4<T> o0, o1, l0, l1;
+            if constexpr (MODE == kForward) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) o0[q] = (T)(activate<T, KIND>(g[q]) * u[q]);
+            } else {
+              const vec4<T> d = *reinterpret_cast<const vec4<T>*>(lds + my_row + fr * (int)sizeof(T));
+              float dg[4], du[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float act, slope;
+                activate_grad<T, KIND>(g[q], act, slope);
+                dg[q] = (float)d[q] * u[q] * slope;
+                du[q] = (float)d[q] * act;
+              }
+              if (!full) {           // what lies past the last token or feature counts as zero
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  const bool exists = token && er + fr + q < a.nr;
+                  dg[q] = exists ? dg[q] : 0.f;
+                  du[q] = exists ? du[q] : 0.f;
+                }
+              }
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                sg[i][q] += dg[q];
+                su[i][q] += du[q];
+                o0[q] = (T)dg[q];
+                o1[q] = (T)du[q];
+                if constexpr (kLow) {
+                  l0[q] = (T)(dg[q] - (float)o0[q]);
+                  l1[q] = (T)(du[q] - (float)o1[q]);
+                }
+              }
+              *reinterpret_cast<vec4<T>*>(region + kRegion + my_row + fr * (int)sizeof(T)) = o1;
+              if constexpr (kLow) {
+                if (a.parts == 2) {
+                  *reinterpret_cast<vec4<T>*>(region + 2 * kRegion + my_row + fr * (int)sizeof(T)) = l0;
+                  *reinterpret_cast<vec4<T>*>(region + 3 * kRegion + my_row + fr * (int)sizeof(T)) = l1;
+                }
+              }
+            }
+            *reinterpret_cast<vec4<T>*>(region + my_row + fr * (int)sizeof(T)) = o0;
+          }
+          __syncthreads();
+#pragma unroll
+          for (int n = 0; n < PU; ++n) {
+            const int e = tid + n * NT, q = e / EU, f = e % EU * OpR::EC;
+            const long c = ec + pass_row(q, j), left = limit - f;
+            if (q >= PR || c >= a.nc || left <= 0) continue;
+#pragma unroll
+            for (int w = 0; w < (kLow ? 4 : MODE == kGateGrad ? 2 : 1); ++w) {
+              if (w >= 2 && a.parts != 2) break;
+              Vec16<T> o;
+              o.load(reinterpret_cast<const T*>(region + w * kRegion + q * kPitch + f * (int)sizeof(T)));
+              o.store_upto(static_cast<T*>(a.out[w]) + c * a.ldo + er + f, left);
+            }
+          }
+        }
+        if constexpr (MODE == kGateGrad) {
+          if (a.col_partial) {       // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
+#pragma unroll
+            for (int i = 0; i < RM / 2; ++i)
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int fr = (wr * (RM / 2) + i) * 16 + lr + q;
+                const float g = lanes_sum<16>(sg[i][q]), u = lanes_sum<16>(su[i][q]);
+                if (lc == 0) {
+                  colsum[(wc * 2 + 0) * TR + fr] = g;
+                  colsum[(wc * 2 + 1) * TR + fr] = u;
+                }
+              }
+            __syncthreads();
+            for (int i = tid; i < 2 * TR; i += NT) {
+              const int side = i / TR, f = i % TR;
+              if (er + f >= a.nr) continue;
+              float v = 0.f;
+#pragma unroll
+              for (int w = 0; w < WC; ++w) v += colsum[(w * 2 + side) * TR + f];
+              a.col_partial[((ec / BC) * 2 + side) * a.nr + er + f] = v;
+            }
+          }
+        }
+      });
+    } else {
+      // out in elements of O: the result itself, or float32 partial results of a cut sum
+      auto finish = [&](auto* out, long ldo) __attribute__((always_inline)) {
+        using O = std::remove_pointer_t<decltype(out)>;
+        constexpr int EO = Vec16<O>::N, UO = BR / EO, kPitch = BR * (int)sizeof(O) + 16, kRegion = PR * kPitch;
+#pragma unroll
+        for (int j = 0; j < CN; ++j) {
+          char* region = lds + (j & 1) * kRegion;
+#pragma unroll
+          for (int i = 0; i < RM; ++i) {
+            vec4<O> o;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) o[q] = (O)acc[i][j][q];
+            *reinterpret_cast<vec4<O>*>(region + (wc * 16 + lc) * kPitch + ((wr * RM + i) * 16 + lr) * (int)sizeof(O)) = o;
+          }
+          __syncthreads();
+          for (int e = tid; e < PR * UO; e += NT) {
+            const int q = e / UO, r = e % UO * EO;
+            const long c = ec + pass_row(q, j), left = a.nr - er - r;
+            if (c >= a.nc || left <= 0) continue;
+            Vec16<O> o;
+            o.load(reinterpret_cast<const O*>(region + q * kPitch + r * (int)sizeof(O)));
+            o.store_upto(out + c * ldo + er + r, left);
+          }
+        }
+      };
+      if (a.splits == 1) finish(static_cast<T*>(which ? a.out[1] : a.out[0]), a.ldo);
+      else finish(a.partial + ((long)split * problems + which) * a.nc * a.nr, a.nr);
+    }
+    if constexpr (!kAhead) return;
+    if (!more) return;
+    __syncthreads();               // the epilogue's reads of LDS are done
   }
 }
 
@@ -635,22 +681,24 @@ constexpr int min_waves(int side) { return side == 64 ? 4 : 2; }
 template <typename T, int MODE, int S, int WR, int WC, int ACT>
 __global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_gemm_kernel(Args a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  gff_gemm<T, MODE, S, S, WR, WC, ACT>(a, blockIdx.x, lds);
+  gff_gemm<T, MODE, S, S, WR, WC, ACT>(a, blockIdx.x, gridDim.x, lds);
 }
 // the two products of a small backward pass side by side: workgroups 0 .. blocks_x - 1 (a multiple of 8) make the input
 // gradient, the others the weights'
 template <typename T, int S, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_both_kernel(Args x, Args w, unsigned blocks_x) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  if (blockIdx.x < blocks_x) gff_gemm<T, mz_gff::kInputGrad, S, S, WR, WC, kAnyActivation>(x, blockIdx.x, lds);
-  else gff_gemm<T, mz_gff::kWeightGrad, S, S, WR, WC, kAnyActivation>(w, blockIdx.x - blocks_x, lds);
+  if (blockIdx.x < blocks_x) gff_gemm<T, mz_gff::kInputGrad, S, S, WR, WC, kAnyActivation>(x, blockIdx.x, blocks_x, lds);
+  else gff_gemm<T, mz_gff::kWeightGrad, S, S, WR, WC, kAnyActivation>(w, blockIdx.x - blocks_x, gridDim.x - blocks_x, lds);
 }
 
-// workgroups of a product in S x S tiles: one a tile, a multiple of the 8 XCDs
+// workgroups of a product in S x S tiles, a multiple of the 8 XCDs: one a tile, or for pair products what the chip holds
 template <int MODE, int S> long gemm_blocks(const Args& a) {
-  constexpr int TR = MODE <= mz_gff::kGateGrad ? S / 2 : S;
+  constexpr bool kPair = MODE <= mz_gff::kGateGrad;
+  constexpr int TR = kPair ? S / 2 : S;
   const long total = ((a.nr + TR - 1) / TR) * ((a.nc + S - 1) / S) * (MODE == mz_gff::kWeightGrad ? 2 : 1) * a.splits;
-  return (total + 7) / 8 * 8;
+  const long held = (long)mz::compute_units() / 8 * 8 * (S == 256 ? 1 : S == 128 ? 2 : 4), blocks = (total + 7) / 8 * 8;
+  return kPair && S != 256 && blocks > held ? held : blocks;
 }
 
 template <typename T, int MODE, int S, int WR, int WC, int ACT> int launch_kernel(const Args& a, hipStream_t s) {
