@@ -69,18 +69,21 @@ Tensor like(const Tensor& x) { return at::empty_like(x, x.options(), at::MemoryF
 Tensor bytes(int64_t n, const Tensor& x) { return n > 0 ? at::empty({n}, x.options().dtype(at::kByte)) : Tensor(); }
 mz_stream_t stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.get_device()).stream(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// values as they lie in memory (the imaginary part of a conjugate is a float tensor whose sign is to be read the other way)
+Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
 // the gradient of an output in the output's type, which is the input's
-Tensor grad_as(const Tensor& g, at::ScalarType t) { return g.scalar_type() == t ? g : g.to(t); }
+Tensor grad_as(const Tensor& g, at::ScalarType t) { return g.scalar_type() == t ? plain(g) : g.to(t); }
 
 // ---- arguments
-Tensor optional_tensor(py::handle h, const char* name) {
-  if (h.is_none()) return Tensor();
-  if (!THPVariable_Check(h.ptr())) refuse(name, ": tensor required");
-  return THPVariable_Unpack(h.ptr());
-}
 Tensor tensor(py::handle h, const char* name) {
   if (!THPVariable_Check(h.ptr())) refuse(name, ": tensor required");
-  return THPVariable_Unpack(h.ptr());
+  const Tensor t = THPVariable_Unpack(h.ptr());
+  if (t._fw_grad(0).defined()) refuse(name, ": forward-mode derivatives are not offered");
+  return plain(t);
+}
+Tensor optional_tensor(py::handle h, const char* name) {
+  if (h.is_none()) return Tensor();
+  return tensor(h, name);
 }
 void check_activation(const Tensor& x, const char* name) {
   if (!x.is_cuda()) refuse(name, ": must live on the GPU");
@@ -204,6 +207,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(py::handle hx, py::handle hw, py::handle hb, double eps) {
   const Tensor x = tensor(hx, "layer_norm: x"), w = optional_tensor(hw, "layer_norm: weight"),
                b = optional_tensor(hb, "layer_norm: bias");
+  const py::gil_scoped_release others_run;
   check_activation(x, "layer_norm: x");
   const int64_t c = x.size(-1);
   if (c > kMaxCols) refuse("layer_norm: x: at most ", kMaxCols, " columns");
@@ -288,10 +292,11 @@ Tensor gated_ff(py::handle hx, py::handle hwg, py::handle hwu, py::handle hbg, p
   if (act == 4) refuse("gated_ff: activation '", activation, "', expected one of silu, gelu, relu, sigmoid");
   Tensor x = tensor(hx, "gated_ff: x"), wg = tensor(hwg, "gated_ff: w_gate"), wu = tensor(hwu, "gated_ff: w_up"),
          bg = optional_tensor(hbg, "gated_ff: b_gate"), bu = optional_tensor(hbu, "gated_ff: b_up");
+  const py::gil_scoped_release others_run;
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const auto t = at::autocast::get_autocast_dtype(at::kCUDA);
     for (Tensor* v : {&x, &wg, &wu, &bg, &bu})
-      if (v->defined() && v->is_cuda() && v->is_floating_point()) *v = v->to(t);
+      if (v->defined()) *v = at::autocast::cached_cast(t, *v, at::kCUDA);
   }
   check_activation(x, "gated_ff: x");
   if (wg.dim() != 2 || wg.size(0) == 0) refuse("gated_ff: w_gate: [F, K] tensor with F of at least 1 expected");
@@ -344,12 +349,13 @@ struct Dropout : torch::autograd::Function<Dropout> {
 };
 
 Tensor dropout(py::handle hx, double p, py::handle hrng, int64_t call, py::handle hresidual) {
-  const Tensor x = tensor(hx, "dropout: x"), residual = optional_tensor(hresidual, "dropout: residual");
+  const Tensor x = tensor(hx, "dropout: x"), residual = optional_tensor(hresidual, "dropout: residual"),
+               rng = tensor(hrng, "dropout: rng");
+  const py::gil_scoped_release others_run;
   check_activation(x, "dropout: x");
   if (x.numel() > (int64_t)1 << 35) refuse("dropout: x: at most 2^35 elements");
   if (!(p >= 0.0 && p <= 1.0)) refuse("dropout: p ", p, ", expected 0 to 1");
   if (call < 0 || call >= (int64_t)1 << 32) refuse("dropout: call ", call, ", expected 0 to 2^32 - 1");
-  const Tensor rng = tensor(hrng, "dropout: rng");
   check_param(rng, "dropout: rng", {2}, x, at::kLong, at::kLong);
   if (!rng.is_contiguous()) refuse("dropout: rng: must be contiguous");
   if (residual.defined()) check_param(residual, "dropout: residual", x.sizes(), x, x.scalar_type(), x.scalar_type());

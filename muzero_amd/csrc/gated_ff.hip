@@ -231,8 +231,8 @@ Backward plan_backward(const Shape& h) {
 
 int check_shape(const char* who, int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation) {
   MZ_REQUIRE(dtype == MZ_F32 || dtype == MZ_BF16 || dtype == MZ_F16, "%s: unknown element type %d", who, dtype);
-  MZ_REQUIRE(M > 0 && K > 0 && F > 0 && K <= (1 << 20) && F <= (1 << 20) && M <= (1ll << 40),
-             "%s: sizes out of range (M = %lld, K = %lld, F = %lld; K and F up to 2^20)", who, (long long)M, (long long)K,
+  MZ_REQUIRE(M > 0 && K > 0 && F > 0 && K <= (1 << 20) && F <= (1 << 20) && M <= (1ll << 36),
+             "%s: sizes out of range (M = %lld, K = %lld, F = %lld; M up to 2^36, K and F up to 2^20)", who, (long long)M, (long long)K,
              (long long)F);
   MZ_REQUIRE(activation >= 0 && activation <= mz_gff::kSigmoid, "%s: unknown activation %d", who, activation);
   return MZ_OK;

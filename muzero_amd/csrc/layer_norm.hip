@@ -459,8 +459,8 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
   if (int rc = check("mz_layer_norm_bwd", rows, C, ldx, dtype, affine_dtype)) return rc;
   MZ_REQUIRE(lddy >= C || rows == 1, "mz_layer_norm_bwd: rows of dy overlap (stride %lld < C = %d)", (long long)lddy, C);
   const bool params = dweight || dbias;
-  MZ_REQUIRE(!params || (workspace && workspace_bytes >= mz_layer_norm_workspace_bytes(rows, C)),
-             "mz_layer_norm_bwd: workspace too small");
+  MZ_REQUIRE(!params || (workspace && workspace_bytes >= mz_layer_norm_workspace_bytes(rows, C) && (size_t)workspace % 4 == 0),
+             "mz_layer_norm_bwd: workspace too small or not aligned to float");
   const LnArgs a = {x, dy, weight, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd),
                     params ? static_cast<float*>(workspace) : nullptr, ldx, lddy, rows, C, affine_dtype == MZ_F32, 0.f};
   hipStream_t s = mz::as_stream(stream);

@@ -88,3 +88,12 @@ def test_dropout_entry_point_refuses():
     _fails("mz_dropout", *call(p=1.5), match=r"p in")
     _fails("mz_dropout", *call(p=float("nan")), match=r"p in")
     _fails("mz_dropout", *call(dt=3), match="element type")
+
+
+def test_sizes_that_cannot_be_numbered_and_float_alignment():
+    lib = _lib.lib()
+    assert lib.mz_gated_ff_workspace_bytes(1 << 37, 1, 1, 1, 1) == -1
+    assert lib.mz_gated_ff_workspace_bytes(1 << 36, 1 << 20, 1 << 20, 0, 1) > 0        # no overflow on the way
+    _fails("mz_gated_ff_fwd", ONE, 64, ONE, ONE, None, None, 1 << 37, 64, 32, 1, 0, ONE, None, 0, None, match="out of range")
+    _fails("mz_layer_norm_bwd", ONE, 8, ONE, 8, None, 0, ONE, ONE, 4, 8, 0, ONE, ONE, None, C.c_void_p(18), 1 << 20, None,
+           match="aligned")

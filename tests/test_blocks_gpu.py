@@ -705,3 +705,112 @@ def test_captured_training_steps(rows):
             masks.add(float(outs[0].double().sum()))
         torch.cuda.synchronize()
     assert len(masks) == 8
+
+
+# ------------------------------------------------------------------------------------------- calls that programs also make
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,k,f", [(4483, 37, 509), (14100, 72, 257), (33000, 20, 130)])
+def test_gated_ff_more_tiles_than_workgroups(rows, k, f, t):
+    """Pair products of more tiles than the chip holds workgroups (they stay for several), ragged in all three."""
+    x, wg, wu, bg, bu, dh = ff_inputs(rows, rows, k, f, TYPES[t])
+    check_gated_ff(x, wg, wu, bg, bu, dh, "gelu", ff_run(x, wg, wu, bg, bu, dh, "gelu"))
+
+
+def test_operands_that_lie_negated_in_memory():
+    """The imaginary part of a conjugate is a view whose elements count with the other sign."""
+    from muzero_amd import blocks
+    z = torch.complex(normal(gen(1), 40, 1), normal(gen(2), 40, 1)).conj()
+    x = z.imag
+    assert x.is_neg()
+    wg, wu = normal(gen(3), 24, 1), normal(gen(4), 24, 1)
+    assert torch.equal(blocks.gated_ff(x, wg, wu), blocks.gated_ff(x.clone().resolve_neg(), wg, wu))
+    rng = torch.zeros(2, dtype=torch.int64, device="cuda")
+    assert torch.equal(blocks.dropout(x, 0.0, rng), x.clone().resolve_neg())
+    leaf = normal(gen(5), 40, 1).requires_grad_()
+    got, = torch.autograd.grad(blocks.dropout(leaf, 0.0, rng), leaf, x)
+    assert torch.equal(got, x.clone().resolve_neg())
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+
+    from muzero_amd import blocks
+    x, w = torch.ones(20, 8, device="cuda"), torch.ones(6, 8, device="cuda")
+    rng = torch.zeros(2, dtype=torch.int64, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: blocks.layer_norm(dual), lambda: blocks.gated_ff(dual, w, w),
+                     lambda: blocks.gated_ff(x, w, forward_ad.make_dual(w, w)), lambda: blocks.dropout(dual, 0.5, rng)):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+
+
+def test_autocast_leaves_float64_alone():
+    from muzero_amd import blocks
+    x, w = torch.ones(20, 8, device="cuda"), torch.ones(6, 8, device="cuda", dtype=torch.float64)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with pytest.raises(ValueError, match="dtype"):
+            blocks.gated_ff(x, w, w)
+
+
+def test_recomputed_activations_draw_the_same_mask():
+    """Under torch.utils.checkpoint the forward pass runs again during the backward pass: the same gradients."""
+    from torch.utils.checkpoint import checkpoint
+    block = Block(13, 64, 96, torch.float32)
+    x = normal(gen(14), 200, 64).requires_grad_()
+    dy = normal(gen(15), 200, 64)
+    rng = torch.tensor([3, 1], dtype=torch.int64, device="cuda")
+    want = torch.autograd.grad(block(x, rng, 0.5), [x] + block.params, dy)
+    got = torch.autograd.grad(checkpoint(block, x, rng, 0.5, use_reentrant=False), [x] + block.params, dy)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_two_threads_at_once():
+    """Two threads, each with its own stream and operands, train and infer at the same time: each gets its own results."""
+    import threading
+    work = []
+    for i, rows in enumerate((300, 1100)):
+        block = Block(60 + i, 96, 200, torch.bfloat16)
+        x = normal(gen(70 + i), rows, 96, t=torch.bfloat16).requires_grad_()
+        work.append((block, x, normal(gen(80 + i), rows, 96, t=torch.bfloat16), torch.tensor([i, 9], dtype=torch.int64, device="cuda")))
+
+    def step(block, x, dy, rng):
+        y = block(x, rng)
+        return [y.detach()] + list(torch.autograd.grad(y, [x] + block.params, dy))
+
+    want = [step(*w) for w in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got[i].append(step(*work[i]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for i in range(2):
+        assert len(got[i]) == 10
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(want[i], outs))
+
+
+def test_gate_and_up_may_be_one_matrix_and_outputs_may_be_summed_twice():
+    """The same tensor in two places: gradients add up; a graph kept for a second backward pass gives the same again."""
+    from muzero_amd import blocks
+    x, w, _, b, _, dh = ff_inputs(90, 70, 40, 48, torch.float32)
+    leaf, wl, bl = (v.detach().requires_grad_() for v in (x, w, b))
+    h = blocks.gated_ff(leaf, wl, wl, bl, bl)
+    first = torch.autograd.grad(h, (leaf, wl, bl), dh, retain_graph=True)
+    again = torch.autograd.grad(h, (leaf, wl, bl), dh)
+    parts = ff_run(x, w, w, b, b, dh, "silu")
+    assert torch.equal(first[1], parts[2] + parts[3]) and torch.equal(first[2], parts[4] + parts[5])
+    assert all(torch.equal(a, c) for a, c in zip(first, again))
+    leaf = x.detach().requires_grad_()
+    rng = torch.zeros(2, dtype=torch.int64, device="cuda")
+    both = torch.autograd.grad(blocks.dropout(leaf, 0.25, rng, residual=leaf), leaf, x)[0]
+    assert torch.equal(both, x + blocks.dropout(x, 0.25, rng))
