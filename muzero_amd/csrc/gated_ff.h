@@ -420,6 +420,20 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
     int buf = 0;
     for (long s = first; s + 1 < last; ++s, buf ^= 1)
       step(lds + buf * ((BR + BC) * 128), lds + (buf ^ 1) * ((BR + BC) * 128), buf ^ 1, s, std::false_type{});
+    // kGateGrad: the tile of dh, sent for as a whole where it has no ragged edge (16-bit types: 32 registers), before the
+    // last step, which loads nothing else
+    constexpr bool kDhAhead = MODE == kGateGrad && sizeof(T) == 2;
+    const bool full = r0 + TR <= a.nr && c0 + BC <= a.nc;
+    Vec16<T> dh_unit[kDhAhead ? CN : 1][PU];
+    if (kDhAhead && full) {
+#pragma unroll
+      for (int j = 0; j < CN; ++j)
+#pragma unroll
+        for (int n = 0; n < PU; ++n) {
+          const int e = tid + n * NT < PR * EU ? tid + n * NT : 0;
+          dh_unit[kDhAhead ? j : 0][n].load(static_cast<const T*>(a.dh) + (c0 + pass_row(e / EU, j)) * a.lddh + r0 + e % EU * OpR::EC);
+        }
+    }
     if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
     __syncthreads();               // the epilogue uses the buffers
     __builtin_amdgcn_sched_barrier(0);                                  // and none of its registers before
@@ -492,19 +506,6 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
     // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
     if constexpr (kPair) {
       constexpr int kPitch = TR * (int)sizeof(T) + 16, kRegion = PR * kPitch;
-      // kGateGrad: the tile of dh, sent for as a whole where it has no ragged edge (16-bit types: 32 registers)
-      constexpr bool kDhAhead = MODE == kGateGrad && sizeof(T) == 2;
-      const bool full = er + TR <= a.nr && ec + BC <= a.nc;
-      Vec16<T> dh_unit[kDhAhead ? CN : 1][PU];
-      if (kDhAhead && full) {
-#pragma unroll
-        for (int j = 0; j < CN; ++j)
-#pragma unroll
-          for (int n = 0; n < PU; ++n) {
-            const int e = tid + n * NT < PR * EU ? tid + n * NT : 0;
-            dh_unit[kDhAhead ? j : 0][n].load(static_cast<const T*>(a.dh) + (ec + pass_row(e / EU, j)) * a.lddh + er + e % EU * OpR::EC);
-          }
-      }
       const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
       constexpr bool kLow = MODE == kGateGrad && BR == 64 && sizeof(T) == 2;      // second parts are written for small problems
       float* colsum = reinterpret_cast<float*>(lds + (kLow ? 5 : 3) * kRegion);   // kGateGrad: [WC][2][TR]
