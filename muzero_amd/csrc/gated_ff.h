@@ -359,12 +359,20 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
       bias[i] = b && f < a.nr ? (float)b[f] : 0.f;
     }
   };
-  // The epilogue goes over the tile in CN passes, each one 16-token block of every wavefront: values pass through LDS so
-  // that memory is read and written in whole 16-byte units of consecutive features, whatever the rows' alignment.
-  constexpr int PR = WC * 16;                                          // tokens of a pass
-  auto pass_row = [&](int q, int j) { return ((q >> 4) * CN + j) * 16 + (q & 15); };   // of the tile, for row q of pass j
+  // The epilogue is each wavefront's own: it goes over its part of the tile - WF features (columns) of CN 16-token blocks - in
+  // passes of PR tokens that go through a region of LDS no other wavefront touches, so that memory is read and written in whole
+  // 16-byte units of consecutive features, whatever the rows' alignment, and no wavefront waits for another.
+  constexpr int WF = TR / WR, EU = WF / OpR::EC;                       // features; 16-byte units of them
+  constexpr int PR = 16 * EU < 64 ? 64 / EU : 16, PU = PR * EU / 64;   // tokens of a pass; units a lane moves in one
+  constexpr int PASSES = CN * 16 / PR;
+  static_assert(CN * 16 % PR == 0 && PR * EU % 64 == 0, "whole passes");
   const int lr = (lane >> 4) * 4, lc = lane & 15;
-  constexpr int EU = TR / OpR::EC, PU = (PR * EU + NT - 1) / NT;       // units of a pass's row; units a thread moves
+  // what the wavefront has written to LDS before, it may read in other lanes after
+  auto wave_sync = [&]() __attribute__((always_inline)) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
   // the last step has nothing to stage or to read ahead
   auto step = [&](const char* here, const char* next, int next_buf, long s, auto is_last) __attribute__((always_inline)) {
     constexpr bool LAST = decltype(is_last)::value;
@@ -420,18 +428,19 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
     int buf = 0;
     for (long s = first; s + 1 < last; ++s, buf ^= 1)
       step(lds + buf * ((BR + BC) * 128), lds + (buf ^ 1) * ((BR + BC) * 128), buf ^ 1, s, std::false_type{});
-    // kGateGrad: the tile of dh, sent for as a whole where it has no ragged edge (16-bit types: 32 registers), before the
-    // last step, which loads nothing else
-    constexpr bool kDhAhead = MODE == kGateGrad && sizeof(T) == 2;
+    // kGateGrad: the wavefront's part of dh, sent for as a whole where the tile has no ragged edge (up to 32 registers, which
+    // float32's larger tile does not have), before the last step, which loads nothing else
+    constexpr bool kDhAhead = MODE == kGateGrad && (sizeof(T) == 2 || BR == 64);
     const bool full = r0 + TR <= a.nr && c0 + BC <= a.nc;
-    Vec16<T> dh_unit[kDhAhead ? CN : 1][PU];
+    Vec16<T> dh_unit[kDhAhead ? PASSES : 1][PU];
     if (kDhAhead && full) {
+      const T* dh = static_cast<const T*>(a.dh) + (c0 + wc * CN * 16) * a.lddh + r0 + wr * WF;
 #pragma unroll
-      for (int j = 0; j < CN; ++j)
+      for (int p = 0; p < PASSES; ++p)
 #pragma unroll
         for (int n = 0; n < PU; ++n) {
-          const int e = tid + n * NT < PR * EU ? tid + n * NT : 0;
-          dh_unit[kDhAhead ? j : 0][n].load(static_cast<const T*>(a.dh) + (c0 + pass_row(e / EU, j)) * a.lddh + r0 + e % EU * OpR::EC);
+          const int e = lane + n * 64;
+          dh_unit[kDhAhead ? p : 0][n].load(dh + (p * PR + e / EU) * a.lddh + e % EU * OpR::EC);
         }
     }
     if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
@@ -505,12 +514,14 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
 
     // ---- epilogue: lane holds r = 16 block + 4 (lane / 16) + 0..3 of c = 16 block + lane % 16
     if constexpr (kPair) {
-      constexpr int kPitch = TR * (int)sizeof(T) + 16, kRegion = PR * kPitch;
-      const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
       constexpr bool kLow = MODE == kGateGrad && BR == 64 && sizeof(T) == 2;      // second parts are written for small problems
-      float* colsum = reinterpret_cast<float*>(lds + (kLow ? 5 : 3) * kRegion);   // kGateGrad: [WC][2][TR]
-      const int my_row = (wc * 16 + lc) * kPitch;                       // of a pass's region
-      const long limit = (MODE == kGateGrad ? a.nr_pad : a.nr) - er;    // columns of the outputs from er on
+      // regions of a wavefront: h; or dh and then dg in its place, du and their second parts
+      constexpr int kPitch = WF * (int)sizeof(T) + 16, kRegion = PR * kPitch, kRegions = kLow ? 4 : MODE == kGateGrad ? 2 : 1;
+      const float* bias = reinterpret_cast<const float*>(lds + 2 * (BR + BC) * 128);
+      char* region = lds + wave * (kRegions * kRegion);
+      float* colsum = reinterpret_cast<float*>(lds + WR * WC * (kRegions * kRegion));    // kGateGrad: [WC][2][TR]
+      const long wf = er + wr * WF, wt = ec + wc * CN * 16;            // the wavefront's first feature, token
+      const long limit = (MODE == kGateGrad ? a.nr_pad : a.nr) - wf;   // columns of the outputs from wf on
       with_activation<ACT>(a.activation, [&](auto kind) __attribute__((always_inline)) {
         constexpr int KIND = decltype(kind)::value;
         float sg[RM / 2][4], su[RM / 2][4];
@@ -519,90 +530,94 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
 #pragma unroll
           for (int q = 0; q < 4; ++q) sg[i][q] = su[i][q] = 0.f;
 #pragma unroll
-        for (int j = 0; j < CN; ++j) {
-          char* region = lds + (MODE == kForward ? j & 1 : 1) * kRegion;  // kGateGrad: dh, dg, du
+        for (int p = 0; p < PASSES; ++p) {
           if constexpr (MODE == kGateGrad) {
             if (kDhAhead && full) {
 #pragma unroll
               for (int n = 0; n < PU; ++n) {
-                const int e = tid + n * NT;
-                if (e < PR * EU) dh_unit[kDhAhead ? j : 0][n].store(reinterpret_cast<T*>(lds + e / EU * kPitch + e % EU * 16));
+                const int e = lane + n * 64;
+                dh_unit[kDhAhead ? p : 0][n].store(reinterpret_cast<T*>(region + e / EU * kPitch + e % EU * 16));
               }
             } else {
 #pragma unroll 1
-              for (int e = tid; e < PR * EU; e += NT) {
-                const int q = e / EU, f = e % EU * OpR::EC;
-                const long c = ec + pass_row(q, j);
+              for (int e = lane; e < PR * EU; e += 64) {
+                const long c = wt + p * PR + e / EU, f = wf + e % EU * OpR::EC;
                 Vec16<T> d;
-                d.load_upto(static_cast<const T*>(a.dh) + c * a.lddh + er + f, c < a.nc ? a.nr - er - f : 0);
-                d.store(reinterpret_cast<T*>(lds + q * kPitch + f * (int)sizeof(T)));
+                d.load_upto(static_cast<const T*>(a.dh) + c * a.lddh + f, c < a.nc ? a.nr - f : 0);
+                d.store(reinterpret_cast<T*>(region + e / EU * kPitch + e % EU * 16));
               }
             }
-            __syncthreads();
+            wave_sync();
           }
-          const bool token = ec + pass_row(wc * 16 + lc, j) < a.nc;
 #pragma unroll
-          for (int i = 0; i < RM / 2; ++i) {
-            const int fr = (wr * (RM / 2) + i) * 16 + lr;               // feature within the tile
-            const f32x4 g = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + fr);
-            const f32x4 u = acc[i + RM / 2][j] + *reinterpret_cast<const f32x4*>(bias + TR + fr);
-            vec4<T> o0, o1, l0, l1;
-            if constexpr (MODE == kForward) {
+          for (int b = 0; b < PR / 16; ++b) {
+            const int j = p * (PR / 16) + b;
+            const bool token = wt + j * 16 + lc < a.nc;
 #pragma unroll
-              for (int q = 0; q < 4; ++q) o0[q] = (T)(activate<T, KIND>(g[q]) * u[q]);
-            } else {
-              const vec4<T> d = *reinterpret_cast<const vec4<T>*>(lds + my_row + fr * (int)sizeof(T));
-              float dg[4], du[4];
+            for (int i = 0; i < RM / 2; ++i) {
+              const int fw = i * 16 + lr, fr = wr * WF + fw;           // feature within the wavefront's, the tile's
+              char* at = region + (b * 16 + lc) * kPitch + fw * (int)sizeof(T);
+              const f32x4 g = acc[i][j] + *reinterpret_cast<const f32x4*>(bias + fr);
+              const f32x4 u = acc[i + RM / 2][j] + *reinterpret_cast<const f32x4*>(bias + TR + fr);
+              vec4<T> o0, o1, l0, l1;
+              if constexpr (MODE == kForward) {
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                float act, slope;
-                activate_grad<T, KIND>(g[q], act, slope);
-                dg[q] = (float)d[q] * u[q] * slope;
-                du[q] = (float)d[q] * act;
-              }
-              if (!full) {           // what lies past the last token or feature counts as zero
+                for (int q = 0; q < 4; ++q) o0[q] = (T)(activate<T, KIND>(g[q]) * u[q]);
+              } else {
+                const vec4<T> d = *reinterpret_cast<const vec4<T>*>(at);
+                float dg[4], du[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                  const bool exists = token && er + fr + q < a.nr;
-                  dg[q] = exists ? dg[q] : 0.f;
-                  du[q] = exists ? du[q] : 0.f;
+                  float act, slope;
+                  activate_grad<T, KIND>(g[q], act, slope);
+                  dg[q] = (float)d[q] * u[q] * slope;
+                  du[q] = (float)d[q] * act;
                 }
-              }
+                if (!full) {         // what lies past the last token or feature counts as zero
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                sg[i][q] += dg[q];
-                su[i][q] += du[q];
-                o0[q] = (T)dg[q];
-                o1[q] = (T)du[q];
+                  for (int q = 0; q < 4; ++q) {
+                    const bool exists = token && wf + fw + q < a.nr;
+                    dg[q] = exists ? dg[q] : 0.f;
+                    du[q] = exists ? du[q] : 0.f;
+                  }
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  sg[i][q] += dg[q];
+                  su[i][q] += du[q];
+                  o0[q] = (T)dg[q];
+                  o1[q] = (T)du[q];
+                  if constexpr (kLow) {
+                    l0[q] = (T)(dg[q] - (float)o0[q]);
+                    l1[q] = (T)(du[q] - (float)o1[q]);
+                  }
+                }
+                *reinterpret_cast<vec4<T>*>(at + kRegion) = o1;
                 if constexpr (kLow) {
-                  l0[q] = (T)(dg[q] - (float)o0[q]);
-                  l1[q] = (T)(du[q] - (float)o1[q]);
+                  if (a.parts == 2) {
+                    *reinterpret_cast<vec4<T>*>(at + 2 * kRegion) = l0;
+                    *reinterpret_cast<vec4<T>*>(at + 3 * kRegion) = l1;
+                  }
                 }
               }
-              *reinterpret_cast<vec4<T>*>(region + kRegion + my_row + fr * (int)sizeof(T)) = o1;
-              if constexpr (kLow) {
-                if (a.parts == 2) {
-                  *reinterpret_cast<vec4<T>*>(region + 2 * kRegion + my_row + fr * (int)sizeof(T)) = l0;
-                  *reinterpret_cast<vec4<T>*>(region + 3 * kRegion + my_row + fr * (int)sizeof(T)) = l1;
-                }
-              }
+              *reinterpret_cast<vec4<T>*>(at) = o0;
             }
-            *reinterpret_cast<vec4<T>*>(region + my_row + fr * (int)sizeof(T)) = o0;
           }
-          __syncthreads();
+          wave_sync();
 #pragma unroll
           for (int n = 0; n < PU; ++n) {
-            const int e = tid + n * NT, q = e / EU, f = e % EU * OpR::EC;
-            const long c = ec + pass_row(q, j), left = limit - f;
-            if (q >= PR || c >= a.nc || left <= 0) continue;
+            const int e = lane + n * 64, f = e % EU * OpR::EC;
+            const long c = wt + p * PR + e / EU, left = limit - f;
+            if (c >= a.nc || left <= 0) continue;
 #pragma unroll
-            for (int w = 0; w < (kLow ? 4 : MODE == kGateGrad ? 2 : 1); ++w) {
+            for (int w = 0; w < kRegions; ++w) {
               if (w >= 2 && a.parts != 2) break;
               Vec16<T> o;
-              o.load(reinterpret_cast<const T*>(region + w * kRegion + q * kPitch + f * (int)sizeof(T)));
-              o.store_upto(static_cast<T*>(a.out[w]) + c * a.ldo + er + f, left);
+              o.load(reinterpret_cast<const T*>(region + w * kRegion + e / EU * kPitch + e % EU * 16));
+              o.store_upto(static_cast<T*>(a.out[w]) + c * a.ldo + wf + f, left);
             }
           }
+          wave_sync();
         }
         if constexpr (MODE == kGateGrad) {
           if (a.col_partial) {       // over the 16 tokens of the lanes, then (below) over the wavefronts side by side
@@ -633,26 +648,30 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
       // out in elements of O: the result itself, or float32 partial results of a cut sum
       auto finish = [&](auto* out, long ldo) __attribute__((always_inline)) {
         using O = std::remove_pointer_t<decltype(out)>;
-        constexpr int EO = Vec16<O>::N, UO = BR / EO, kPitch = BR * (int)sizeof(O) + 16, kRegion = PR * kPitch;
+        constexpr int EO = Vec16<O>::N, UO = WF / EO, kPitch = WF * (int)sizeof(O) + 16, kRegion = 16 * kPitch;
+        static_assert(16 * UO % 64 == 0, "whole units a lane");
+        char* region = lds + wave * kRegion;
+        const long wr0 = er + wr * WF, wc0 = ec + wc * CN * 16;
 #pragma unroll
         for (int j = 0; j < CN; ++j) {
-          char* region = lds + (j & 1) * kRegion;
 #pragma unroll
           for (int i = 0; i < RM; ++i) {
             vec4<O> o;
 #pragma unroll
             for (int q = 0; q < 4; ++q) o[q] = (O)acc[i][j][q];
-            *reinterpret_cast<vec4<O>*>(region + (wc * 16 + lc) * kPitch + ((wr * RM + i) * 16 + lr) * (int)sizeof(O)) = o;
+            *reinterpret_cast<vec4<O>*>(region + lc * kPitch + (i * 16 + lr) * (int)sizeof(O)) = o;
           }
-          __syncthreads();
-          for (int e = tid; e < PR * UO; e += NT) {
-            const int q = e / UO, r = e % UO * EO;
-            const long c = ec + pass_row(q, j), left = a.nr - er - r;
+          wave_sync();
+#pragma unroll 2
+          for (int n = 0; n < 16 * UO / 64; ++n) {
+            const int e = lane + n * 64, r = e % UO * EO;
+            const long c = wc0 + j * 16 + e / UO, left = a.nr - wr0 - r;
             if (c >= a.nc || left <= 0) continue;
             Vec16<O> o;
-            o.load(reinterpret_cast<const O*>(region + q * kPitch + r * (int)sizeof(O)));
-            o.store_upto(out + c * ldo + er + r, left);
+            o.load(reinterpret_cast<const O*>(region + e / UO * kPitch + e % UO * 16));
+            o.store_upto(out + c * ldo + wr0 + r, left);
           }
+          wave_sync();
         }
       };
       if (a.splits == 1) finish(static_cast<T*>(which ? a.out[1] : a.out[0]), a.ldo);
@@ -665,12 +684,13 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
 }
 
 // LDS of a kernel: the two buffers and the biases, or what the epilogue's regions take
-template <typename T, int MODE, int BR, int BC, int WC> constexpr int lds_bytes() {
+template <typename T, int MODE, int BR, int BC, int WR, int WC> constexpr int lds_bytes() {
   constexpr bool kPair = MODE <= mz_gff::kGateGrad;
-  constexpr int TR = kPair ? BR / 2 : BR, PR = WC * 16, buffers = 2 * (BR + BC) * 128;
-  constexpr int regions = MODE == mz_gff::kForward    ? 2 * PR * (TR * (int)sizeof(T) + 16)
-                          : MODE == mz_gff::kGateGrad ? (BR == 64 ? 5 : 3) * PR * (TR * (int)sizeof(T) + 16) + WC * 2 * TR * 4
-                                                      : 2 * PR * (BR * 4 + 16);
+  constexpr int TR = kPair ? BR / 2 : BR, WF = TR / WR, units = WF * (int)sizeof(T) / 16, PR = 16 * units < 64 ? 64 / units : 16;
+  constexpr int buffers = 2 * (BR + BC) * 128, region = PR * (WF * (int)sizeof(T) + 16);
+  constexpr int regions = MODE == mz_gff::kForward    ? WR * WC * region
+                          : MODE == mz_gff::kGateGrad ? WR * WC * (BR == 64 ? 4 : 2) * region + WC * 2 * TR * 4
+                                                      : WR * WC * 16 * (WF * 4 + 16);
   static_assert(!kPair || regions <= buffers, "the biases lie behind the buffers");
   constexpr int bytes = (regions > buffers ? regions : buffers) + (kPair ? 2 * TR * 4 : 0);
   static_assert(bytes <= 160 * 1024, "LDS of a compute unit");
@@ -705,7 +725,7 @@ template <int MODE, int S> long gemm_blocks(const Args& a) {
 }
 
 template <typename T, int MODE, int S, int WR, int WC, int ACT> int launch_kernel(const Args& a, hipStream_t s) {
-  constexpr int kLds = lds_bytes<T, MODE, S, S, WC>();
+  constexpr int kLds = lds_bytes<T, MODE, S, S, WR, WC>();
   static bool done[mz::kMaxDevices] = {false};
   const auto kernel = gff_gemm_kernel<T, MODE, S, WR, WC, ACT>;
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
@@ -742,7 +762,7 @@ template <typename T> int launch_any(const Args& a, int mode, int tile, hipStrea
   }
 }
 template <typename T, int S> int launch_both_in(const Args& x, const Args& w, hipStream_t s) {
-  constexpr int kLds = lds_bytes<T, mz_gff::kInputGrad, S, S, 2>();
+  constexpr int kLds = lds_bytes<T, mz_gff::kInputGrad, S, S, 2, 2>();
   static bool done[mz::kMaxDevices] = {false};
   const auto kernel = gff_both_kernel<T, S, 2, 2>;
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
