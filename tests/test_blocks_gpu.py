@@ -814,3 +814,24 @@ def test_gate_and_up_may_be_one_matrix_and_outputs_may_be_summed_twice():
     rng = torch.zeros(2, dtype=torch.int64, device="cuda")
     both = torch.autograd.grad(blocks.dropout(leaf, 0.25, rng, residual=leaf), leaf, x)[0]
     assert torch.equal(both, x + blocks.dropout(x, 0.25, rng))
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [9, 150, 2300])
+def test_gated_ff_large_biases(rows, t):
+    """Biases far above the products: the definition's, in float32 to its last digits (the bias is added to the finished
+    sum, whose own error it does not enter)."""
+    t = TYPES[t]
+    x, wg, wu, bg, bu, dh = ff_inputs(95, rows, 520, 72, t)
+    bg, bu = (bg.float() * 400).to(t), (bu.float() * 400).to(t)
+    if t == torch.float32:
+        check_gated_ff(x, wg, wu, bg, bu, dh, "relu", ff_run(x, wg, wu, bg, bu, dh, "relu"))
+    else:
+        h = ff_run(x, wg, wu, bg, bu, dh, "relu")[0]
+        gate, up = x.double() @ wg.double().t() + bg.double(), x.double() @ wu.double().t() + bu.double()
+        # a sum that starts at the bias passes through at most K additions: K u (sum|terms| + |bias|) each
+        e_g, e_u = (521 * U * (x.double().abs() @ w.double().abs().t() + b.double().abs()) for w, b in ((wg, bg), (wu, bu)))
+        ref = gate.clamp(min=0) * up
+        fits = ref.abs() < 0.99 * torch.finfo(t).max
+        assert fits.float().mean() > 0.9
+        within(h[fits], ref[fits], (e_g * up.abs() + gate.abs() * e_u + e_g * e_u + 3 * U * ref.abs())[fits], "h")
