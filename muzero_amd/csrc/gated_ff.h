@@ -439,20 +439,22 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
     int buf = 0;
     for (long s = first; s + 1 < last; ++s, buf ^= 1)
       step(lds + buf * ((BR + BC) * 128), lds + (buf ^ 1) * ((BR + BC) * 128), buf ^ 1, s, std::false_type{});
-    // kGateGrad: the wavefront's part of dh, sent for as a whole where the tile has no ragged edge (up to 32 registers, which
-    // float32's larger tile does not have), before the last step, which loads nothing else
-    constexpr bool kDhAhead = MODE == kGateGrad && (sizeof(T) == 2 || BR == 64);
+    // kGateGrad: the wavefront's part of dh, sent for as a whole (up to 32 registers) before the last step, which loads nothing
+    // else, or, in float32's larger tile, two passes ahead; a tile with a ragged edge reads its dh pass by pass
+    constexpr int kDhPasses = sizeof(T) == 2 || BR == 64 ? PASSES : 2;
     const bool full = r0 + TR <= a.nr && c0 + BC <= a.nc;
-    Vec16<T> dh_unit[kDhAhead ? PASSES : 1][PU];
-    if (kDhAhead && full) {
-      const T* dh = static_cast<const T*>(a.dh) + (c0 + wc * CN * 16) * a.lddh + r0 + wr * WF;
+    Vec16<T> dh_unit[MODE == kGateGrad ? kDhPasses : 1][PU];
+    const T* const dh = MODE == kGateGrad ? static_cast<const T*>(a.dh) + (c0 + wc * CN * 16) * a.lddh + r0 + wr * WF : nullptr;
+    auto load_dh = [&](int p) __attribute__((always_inline)) {
 #pragma unroll
-      for (int p = 0; p < PASSES; ++p)
+      for (int n = 0; n < PU; ++n) {
+        const int e = lane + n * 64;
+        dh_unit[p % kDhPasses][n].load(dh + (p * PR + e / EU) * a.lddh + e % EU * OpR::EC);
+      }
+    };
+    if (MODE == kGateGrad && full) {
 #pragma unroll
-        for (int n = 0; n < PU; ++n) {
-          const int e = lane + n * 64;
-          dh_unit[kDhAhead ? p : 0][n].load(dh + (p * PR + e / EU) * a.lddh + e % EU * OpR::EC);
-        }
+      for (int p = 0; p < kDhPasses; ++p) load_dh(MODE == kGateGrad ? p : 0);
     }
     if (first < last) step(lds + buf * ((BR + BC) * 128), nullptr, 0, last - 1, std::true_type{});
     __syncthreads();               // the epilogue uses the buffers
@@ -542,12 +544,13 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
           if constexpr (MODE == kGateGrad) {
-            if (kDhAhead && full) {
+            if (full) {
 #pragma unroll
               for (int n = 0; n < PU; ++n) {
                 const int e = lane + n * 64;
-                dh_unit[kDhAhead ? p : 0][n].store(reinterpret_cast<T*>(region + e / EU * kPitch + e % EU * 16));
+                dh_unit[p % kDhPasses][n].store(reinterpret_cast<T*>(region + e / EU * kPitch + e % EU * 16));
               }
+              if (p + kDhPasses < PASSES) load_dh(p + kDhPasses);
             } else {
 #pragma unroll 1
               for (int e = lane; e < PR * EU; e += 64) {
