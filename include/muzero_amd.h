@@ -584,7 +584,8 @@ int mz_bn_relu_train_bwd_acc(const void* x, const void* dy, const void* y, const
  * contiguous.  weight, bias (either may be NULL: 1 and 0): [C] of affine_dtype, which is MZ_F32 or dtype.  mean, rstd:
  * float [rows] for the backward pass, or both NULL.  No alignment beyond the elements' is needed.
  * Backward: from dy (rows lddy apart) dx (contiguous), dweight and dbias ([C] of affine_dtype); any of the three may
- * be NULL.  workspace (for dweight / dbias): mz_layer_norm_workspace_bytes(rows, C) bytes.  No atomics. */
+ * be NULL.  workspace (for dweight / dbias): mz_layer_norm_workspace_bytes(rows, C) bytes, aligned to float.  No
+ * atomics. */
 int mz_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, int32_t affine_dtype, double eps,
                       int64_t rows, int32_t C, int32_t dtype, void* y, float* mean, float* rstd, mz_stream_t stream);
 int64_t mz_layer_norm_workspace_bytes(int64_t rows, int32_t C);
@@ -594,11 +595,12 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
 
 /* Gated feed-forward projection in one kernel: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up).  x: [M] rows of K
  * elements, ldx apart; w_gate, w_up: [F][K]; b_gate, b_up: [F] or NULL; h: [M][F]; all of `dtype`, float32
- * accumulation.  activation: 0 SiLU, 1 GELU (erf), 2 ReLU, 3 sigmoid.  K, F up to 2^20; rows of x up to 4 MiB apart.  No
- * alignment beyond the elements' is needed.  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which may
+ * accumulation.  activation: 0 SiLU, 1 GELU (erf), 2 ReLU, 3 sigmoid.  M up to 2^36, K and F up to 2^20; rows of x up to
+ * 4 MiB apart.  No alignment beyond the elements' is needed.  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which may
  * be 0 (then NULL will do).
  * Backward: recomputes both products; dh [M][F] -> dx [M][K], dw_gate / dw_up [F][K] (both or neither), db_gate / db_up
- * [F]; NULL for what is not wanted.  The gradients of the two products are rounded to `dtype` between the launches.
+ * [F]; NULL for what is not wanted.  The gradients of the two products are rounded to `dtype` between the launches
+ * (16-bit types with M F <= 8192 carry what that rounding left in a second term).
  * workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 1) bytes, 16-byte aligned.  No atomics. */
 int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward);
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,

@@ -10,8 +10,9 @@ unequal length.  The reference has no counterpart.
 
 All take CUDA tensors of any leading shape (the last dimension is the operator's), in bfloat16, float16 or float32,
 accumulate in float32, run on the tensors' device and that device's current stream, allocate their outputs and scratch
-with torch's allocator per call (so they can be recorded into HIP graphs) and are differentiable once.  Wrong types,
-shapes or devices raise ValueError; there is no CPU path.
+with torch's allocator per call (so they can be recorded into HIP graphs) and are differentiable once, in reverse mode.
+Wrong types, shapes or devices raise ValueError; there is no CPU path.  While a backward pass is being recorded into a HIP
+graph, no eager autograd graph of the same parameters may be alive (as for any torch operator).
 """
 import ctypes as C
 from typing import Optional
@@ -54,8 +55,8 @@ def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optio
     ``torch.autocast`` they are cast to its dtype first, as torch's linear does).  activation: "silu", "gelu" (erf),
     "relu" or "sigmoid".  Returns [..., F].  The backward pass computes the two products again from x: nothing of the
     hidden width is kept but the result.  In bfloat16 and float16 it rounds the products' gradients to that type
-    (they are matrix operands next); float16 gradients below 6e-5 lose digits as any float16 value does - scale the
-    loss."""
+    (they are matrix operands next; where there are at most 8192 of each, what the rounding left is carried along);
+    float16 gradients below 6e-5 lose digits and those above 65504 overflow as any float16 value does - scale the loss."""
     return (_ext or _load()).gated_ff(x, w_gate, w_up, b_gate, b_up, activation)
 
 

@@ -6,7 +6,9 @@
 // 32 x 32 -> 64 bit products, which the vector units do at a quarter of their rate, so 32 bits an element would make
 // the kernel bound by them instead of by memory; 16 round p to a multiple of 2^-16, and the scale is that p's own.
 // The backward pass is the same kernel on the gradient.  A dropped element is zero whatever it held (NaN, infinity).
-// HBM-bound: reads x (+ residual), writes y.
+// HBM-bound: reads x (+ residual), writes y.  Measured on an MI355X: 16385 x 8191 bf16 with a residual, forward and
+// backward 259 us (1.34 GB: 5.2 TB/s, a copy of 2 GiB runs at 5.0); 18432 x 256 bf16 6.4 us, 128 x 256 float32 2.8 us (a
+// launch).
 #include "block_common.h"
 
 namespace {

@@ -14,6 +14,14 @@
 // float32) of both operands go to one of two LDS buffers; the next step's travel in registers meanwhile, loaded through
 // a buffer descriptor that returns zeros for what lies outside the matrix (ragged edges cost a compare, no branch).
 // One barrier a step.
+//
+// What bounds it (MI355X): a step of the 256 x 256 tile keeps the matrix cores and LDS busy for 2048 cycles each (64
+// matrix instructions of 16 cycles a wavefront, two wavefronts a SIMD; 192 KB read and 64 KB staged at 128 bytes a cycle)
+// and takes 1.4 us, 3000 cycles or so at the clock the chip holds there; the smaller tiles read twice the bytes an
+// operation and lean on LDS.  8192 x 2048 x 8192 bf16: forward 426 us, input gradient 422, weight gradient 429 (1.28 to
+// 1.30 PFLOP/s), gate gradient 488 (1.13); the library's plain product of that size 452 (1.22).  18432 x 256 x 1024 bf16, where a tile has four steps: forward
+// 31 us, gate gradient 44 (113 MB of dh, dg and du), input gradient 28 - 288 tiles on 256 compute units - and weight
+// gradient 27.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the 151 TFLOP/s of a large product.
 #pragma once
 #include "block_common.h"
 
@@ -389,7 +397,8 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
 #pragma unroll
       for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[0][j], acc[i][j], T{});
 #pragma unroll
-      for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[1][j] = OpC::fragment(here + BR * 128, wc * CN + j, 1, lane);
+      for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j)
+        cf[1][j] = OpC::fragment(here + BR * 128, wc * CN + j, 1, lane);
       rf[i] = OpR::fragment(here, r_block(i), 1, lane);
       if constexpr (!LAST) {
 #pragma unroll
@@ -407,7 +416,8 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
       for (int j = 0; j < CN; ++j) acc[i][j] = mma(rf[i], cf[1][j], acc[i][j], T{});
       if constexpr (!LAST) {
 #pragma unroll
-        for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j) cf[0][j] = OpC::fragment(next + BR * 128, wc * CN + j, 0, lane);
+        for (int j = turn_begin(i, CN, RM); j < turn_begin(i + 1, CN, RM); ++j)
+          cf[0][j] = OpC::fragment(next + BR * 128, wc * CN + j, 0, lane);
         rf[i] = OpR::fragment(next, r_block(i), 0, lane);
       }
     }
@@ -484,7 +494,8 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
             if (is_r) {
               const int r = kPair ? q % TR : q;
               exists = r0 + r < a.nr;
-              p = static_cast<const T*>((kPair ? q / TR : MODE == kInputGrad ? seg & 1 : 0) ? a.r[1] : a.r[0]) + (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
+              p = static_cast<const T*>((kPair ? q / TR : MODE == kInputGrad ? seg & 1 : 0) ? a.r[1] : a.r[0]) +
+                  (kRAcross ? k * a.ldr + r0 + r : (r0 + r) * a.ldr + k);
               along = kRAcross ? a.ldr : 1;
             } else {
               exists = c0 + q < a.nc;
@@ -763,7 +774,8 @@ template <typename T, int MODE, int S, int WR, int WC> int launch_one(const Args
   }
 }
 template <typename T, int MODE> int launch_mode(const Args& a, int tile, hipStream_t s) {
-  // float32's matrix instructions are slow enough for the smaller tiles to keep up with (18432 x 256 x 1024: 158 us, 209)
+  // float32's matrix instructions are slow enough for the smaller tiles to keep up with (18432 x 256 x 1024 forward: 128 x
+  // 128 tiles 160 us, 64 x 64 172)
   if constexpr (sizeof(T) == 2)
     if (tile == 0) return launch_one<T, MODE, 256, 2, 4>(a, s);
   if (tile <= 1) return launch_one<T, MODE, 128, 2, 2>(a, s);

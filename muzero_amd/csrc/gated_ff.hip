@@ -7,8 +7,9 @@
 // (4 M K F operations against 8 M F bytes written and read back in 16 bits - and without rounding g and u), writes
 // dg and du in the operands' type - they are matrix operands next, and their rounding adds one half step to a sum's
 // terms, which averages out over a sum as long as they are many - and runs the two products that need them.  Where there
-// are few (16-bit types, M F <= 8192) what the rounding left goes along as a second operand of the same products.  Sums over few tiles are split along k into float32 partial
-// results that a second launch adds up in a fixed order: no atomics, the same bits on every run.
+// are few (16-bit types, M F <= 8192) what the rounding left goes along as a second operand of the same products.  Sums
+// over few tiles are split along k into float32 partial results that a second launch adds up in a fixed order: no atomics,
+// the same bits on every run.
 #include "gated_ff.h"
 
 namespace {
@@ -128,8 +129,8 @@ int64_t tiles(int64_t nr, int64_t nc, int tr, int bc) { return ((nr + tr - 1) / 
 // costs besides its steps (first loads, epilogue), by mode.  A sum cut into parts costs another launch and its partial
 // results' way through memory.  Measured per step (64 16-bit or 32 float32 values of k), one workgroup alone / the
 // compute unit full, on products of one to 4096 tiles; the estimate is within a fifth of what it was fitted to, and
-// choosing by it within a tenth of the best of all choices (18432 x 256 x 1024, dx: 128 x 128 tiles 33 us, 64 x 64 40,
-// 256 x 256 48; 1000 x 256 x 1000 float32, dx: 64 x 64 in 4 parts 18 us, 128 x 128 in 16 21, whole 137).
+// choosing by it within a tenth of the best of all choices (18432 x 256 x 1024, dx: 128 x 128 tiles 29 us, 64 x 64 39,
+// 256 x 256 40; 1000 x 256 x 1000 float32, dx: 64 x 64 in 8 parts 17 us, whole 46, 128 x 128 in 16 parts 19, whole 138).
 struct TileCost {
   int at_once;
   float alone, shared, ends[3];                    // ends: kForward, kGateGrad, the plain products
@@ -189,8 +190,8 @@ Shape make_shape(int64_t M, int64_t K, int64_t F, int dtype) {
   const int e = unit_elems(dtype);
   return {M, K, F, round_up(F, e), dtype, K % e != 0};
 }
-// Tokens the streaming kernel takes: at 16, 2048 x 2048 bf16 7.7 us (64 x 64 tiles 11.8), 1000 x 5000 float32 12.7
-// (23.4), 4096 x 16384 bf16 out of the caches 47 (43); at 32, with two blocks of tokens, 9.8 (12.0), 19.9 (23.6), 59 (43).
+// Tokens the streaming kernel takes: at 16, 2048 x 2048 bf16 8.3 us (64 x 64 tiles 12.3), 1000 x 5000 float32 13.6
+// (23.2), 4096 x 16384 bf16 out of the caches 47 (42); at 32, with two blocks of tokens, 9.8 (12.0), 19.9 (23.6), 59 (43).
 constexpr int64_t kFew = 16;
 
 struct Backward {

@@ -10,6 +10,11 @@
 // down the rows with the parameters of their columns - and, backward, the columns' running dw and db - in registers.
 // Every workgroup leaves its dw and db in a float32 partial row and a second launch adds those up: no atomics, the
 // same bits on every run.
+//
+// Measured on an MI355X, forward / backward with both launches: 65536 x 4096 bf16 196 / 331 us (5.5 and 4.9 TB/s; a copy
+// of 2 GiB runs at 5.0), 18432 x 256 bf16 5.6 / 11.7 us, 4097 x 1001 float32 8.7 / 19.2 us, 1000 x 256 bf16 2.4 / 5.2 us:
+// the smaller ones live in the Infinity Cache and are bound by the launches' own time - a third of the backward's is the
+// second launch, a few workgroups that add up what up to 768 have left.
 #include "block_common.h"
 
 namespace {
