@@ -15,6 +15,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <sstream>
@@ -71,14 +72,19 @@ mz_stream_t stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 // values as they lie in memory (the imaginary part of a conjugate is a float tensor whose sign is to be read the other way)
 Tensor plain(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
-// the gradient of an output in the output's type, which is the input's
-Tensor grad_as(const Tensor& g, at::ScalarType t) { return g.scalar_type() == t ? plain(g) : g.to(t); }
+// the gradient of an output in the output's type, which is the input's, in memory
+Tensor grad_as(const Tensor& g, at::ScalarType t) {
+  if (g._is_zerotensor()) return at::zeros(g.sizes(), g.options().dtype(t));
+  return g.scalar_type() == t ? plain(g) : g.to(t);
+}
 
 // ---- arguments
 Tensor tensor(py::handle h, const char* name) {
   if (!THPVariable_Check(h.ptr())) refuse(name, ": tensor required");
   const Tensor t = THPVariable_Unpack(h.ptr());
   if (t._fw_grad(0).defined()) refuse(name, ": forward-mode derivatives are not offered");
+  if (t._is_zerotensor()) refuse(name, ": a tensor without memory");
+  if (torch::jit::tracer::isTracing()) refuse(name, ": cannot be traced (the trace would hold no trace of the kernels)");
   return plain(t);
 }
 Tensor optional_tensor(py::handle h, const char* name) {

@@ -835,3 +835,44 @@ def test_gated_ff_large_biases(rows, t):
         fits = ref.abs() < 0.99 * torch.finfo(t).max
         assert fits.float().mean() > 0.9
         within(h[fits], ref[fits], (e_g * up.abs() + gate.abs() * e_u + e_g * e_u + 3 * U * ref.abs())[fits], "h")
+
+
+def test_transforms_that_see_only_torch_operations_are_refused():
+    """A trace, a batched or a functional transform would not record the kernels: an error, never a wrong result."""
+    from muzero_amd import blocks
+    x, w = torch.ones(20, 8, device="cuda"), torch.ones(6, 8, device="cuda")
+    rng = torch.zeros(2, dtype=torch.int64, device="cuda")
+    calls = (lambda v: blocks.layer_norm(v), lambda v: blocks.gated_ff(v, w, w), lambda v: blocks.dropout(v, 0.5, rng))
+    for call in calls:
+        with pytest.raises(ValueError, match="traced"):
+            torch.jit.trace(call, (x,), check_trace=False)
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x.expand(3, 20, 8))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda v: call(v).sum())(x)
+        with pytest.raises(ValueError, match="without memory"):
+            call(torch._efficientzerotensor((20, 8), device="cuda"))
+
+
+def test_graphed_callables():
+    """torch.cuda.make_graphed_callables: forward and backward as two graphs, several steps with other inputs."""
+    from muzero_amd import blocks
+
+    class Module(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            g = gen(21)
+            self.w, self.b = torch.nn.Parameter(normal(g, 64, mean=1.0)), torch.nn.Parameter(normal(g, 64))
+            self.gate, self.up = torch.nn.Parameter(normal(g, 96, 64)), torch.nn.Parameter(normal(g, 96, 64))
+
+        def forward(self, x):
+            return blocks.gated_ff(blocks.layer_norm(x, self.w, self.b), self.gate, self.up, activation="gelu")
+
+    eager, module = Module(), Module()
+    graphed = torch.cuda.make_graphed_callables(module, (normal(gen(22), 150, 64).requires_grad_(),))
+    for i in range(3):
+        x, dy = normal(gen(30 + i), 150, 64).requires_grad_(), normal(gen(40 + i), 150, 96)
+        want = torch.autograd.grad(eager(x), [x] + list(eager.parameters()), dy)
+        got = torch.autograd.grad(graphed(x), [x] + list(module.parameters()), dy)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
