@@ -54,7 +54,8 @@ def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optio
     x: [..., K]; w_gate, w_up: [F, K]; b_gate, b_up: [F] or None; K and F up to 2^20, all of one dtype (under
     ``torch.autocast`` they are cast to its dtype first, as torch's linear does).  activation: "silu", "gelu" (erf),
     "relu" or "sigmoid".  Returns [..., F].  The backward pass computes the two products again from x: nothing of the
-    hidden width is kept but the result.  In bfloat16 and float16 it rounds the products' gradients to that type
+    hidden width is kept but the result; while it runs it takes scratch of twice the result's size and for the partial
+    results of sums that are cut over workgroups.  In bfloat16 and float16 it rounds the products' gradients to that type
     (they are matrix operands next; where there are at most 8192 of each, what the rounding left is carried along);
     float16 gradients below 6e-5 lose digits and those above 65504 overflow as any float16 value does - scale the loss."""
     return (_ext or _load()).gated_ff(x, w_gate, w_up, b_gate, b_up, activation)
