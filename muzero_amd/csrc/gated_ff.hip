@@ -53,17 +53,14 @@ template <typename T> __device__ __forceinline__ void join_part(const Join& j, u
   T* out0 = static_cast<T*>(j.out[0]);
   T* out1 = static_cast<T*>(j.out[1]);
   for (long i = ((long)block * 256 + threadIdx.x) * 4; i < j.n; i += (long)j.blocks * 1024) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
     const int m = (int)(j.n - i < 4 ? j.n - i : 4);
-    if (m == 4 && (j.n & 3) == 0) {
-#pragma unroll 4
-      for (int s = 0; s < j.splits; ++s) {
-        const float4 t = *reinterpret_cast<const float4*>(j.partial + s * j.n + i);
-        v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
-      }
-    } else {
-      for (int s = 0; s < j.splits; ++s)
-        for (int q = 0; q < m; ++q) v[q] += j.partial[s * j.n + i + q];
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int s = 0; s < j.splits; ++s) {           // rows of odd lengths start anywhere: a vector of float's alignment
+      Vec16<float> t;
+      t.load_upto(j.partial + s * j.n + i, m);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] += t.v[q];
     }
     for (int q = 0; q < m; ++q) {
       const long e = i + q;
