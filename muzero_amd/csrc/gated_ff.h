@@ -731,7 +731,7 @@ __global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_gemm_kernel(Ar
   extern __shared__ __attribute__((aligned(16))) char lds[];
   gff_gemm<T, MODE, S, S, WR, WC, ACT>(a, blockIdx.x, gridDim.x, lds);
 }
-// the two products of a small backward pass side by side: workgroups 0 .. blocks_x - 1 (a multiple of 8) make the input
+// the two products of a backward pass in one launch: workgroups 0 .. blocks_x - 1 (a multiple of 8) make the input
 // gradient, the others the weights'
 template <typename T, int S, int WR, int WC>
 __global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_both_kernel(Args x, Args w, unsigned blocks_x) {

@@ -121,7 +121,7 @@ void finish(const Finish& f, int dtype, hipStream_t s) {
 
 int64_t tiles(int64_t nr, int64_t nc, int tr, int bc) { return ((nr + tr - 1) / tr) * ((nc + bc - 1) / bc); }
 
-// Tile and split of a product, by its estimated time (microseconds).  A tile's workgroups share a compute unit `at_once`
+// Tile and split of a product launched by itself, by its estimated time (microseconds).  A tile's workgroups share a compute unit `at_once`
 // at a time; a step of one takes `alone`, and no less than `shared` times the workgroups there; `ends` is what a round
 // costs besides its steps (first loads, epilogue), by mode.  A sum cut into parts costs another launch and its partial
 // results' way through memory.  Measured per step (64 16-bit or 32 float32 values of k), one workgroup alone / the
@@ -140,32 +140,64 @@ struct Split {
   float time;
   int64_t groups;                                  // workgroups
 };
-constexpr int kMaxSplits = 32;
+constexpr int kMaxSplits = 32, kCus = 256;         // of an MI355X: the choice, and with it a sum's order, is the same everywhere
+
+const TileCost& cost_of(int dtype, int tile) { return (dtype == MZ_F32 ? kCost32 : kCost16)[tile]; }
+float join_time(int64_t elements, int splits) { return splits > 1 ? (float)elements * splits * 8.f / 8e6f : 0.f; }
+
+// f(the product of nr x nc results, `problems` of them, in `tile` with its sum cut into 1, 2, 3 .. parts)
+template <typename Fn> void for_cuts(int64_t nr, int64_t nc, int64_t steps, int tile, int problems, bool pair, Fn&& f) {
+  const int side = mz_gff::tile_side(tile);
+  const int64_t whole = tiles(nr, nc, pair ? side / 2 : side, side) * problems;
+  for (int want = 1; want <= (pair ? 1 : kMaxSplits); want += want < 4 ? 1 : want < 8 ? 2 : want < 16 ? 4 : 8) {
+    if (want > 1 && want > steps / 2) break;
+    const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+    f(Split{tile, (int)splits, (int)per, 0.f, whole * splits});
+  }
+}
 
 Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only = -1) {
   const bool pair = mode <= mz_gff::kGateGrad;
   const int problems = mode == mz_gff::kWeightGrad ? 2 : 1;
-  const int cus = 256;                             // of an MI355X: the choice, and with it a sum's order, is the same everywhere
   Split best = {2, 1, (int)steps, -1.f, 0};
   for (int t = dtype == MZ_F32 ? 1 : 0; t < 3; ++t) {
     if (only >= 0 && t != only) continue;
-    const TileCost& c = (dtype == MZ_F32 ? kCost32 : kCost16)[t];
-    const int side = mz_gff::tile_side(t);
-    const int64_t whole = tiles(nr, nc, pair ? side / 2 : side, side) * problems;
-    for (int want = 1; want <= (pair ? 1 : kMaxSplits); want += want < 4 ? 1 : want < 8 ? 2 : want < 16 ? 4 : 8) {
-      if (want > 1 && want > steps / 2) break;
-      const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
-      const int64_t share = (whole * splits + cus - 1) / cus, rounds = share / c.at_once, rest = share % c.at_once;
+    const TileCost& c = cost_of(dtype, t);
+    for_cuts(nr, nc, steps, t, problems, pair, [&](Split s) {
+      const int64_t share = (s.groups + kCus - 1) / kCus, rounds = share / c.at_once, rest = share % c.at_once;
       auto round = [&](int64_t n) {
-        const float s = c.shared * n > c.alone ? c.shared * n : c.alone;
-        return per * s + c.ends[mode < 2 ? mode : 2];
+        const float step = c.shared * n > c.alone ? c.shared * n : c.alone;
+        return s.steps * step + c.ends[mode < 2 ? mode : 2];
       };
-      float time = rounds * round(c.at_once) + (rest ? round(rest) : 0.f);
-      if (splits > 1) time += 3.f + (float)(nr * nc * problems) * splits * 8.f / 8e6f;
-      if (best.time < 0.f || time < best.time) best = {t, (int)splits, (int)per, time, whole * splits};
-    }
+      s.time = rounds * round(c.at_once) + (rest ? round(rest) : 0.f);
+      if (s.splits > 1) s.time += 3.f + join_time(nr * nc * problems, s.splits);
+      if (best.time < 0.f || s.time < best.time) best = s;
+    });
   }
   return best;
+}
+
+// Two products in one launch, where the second's workgroups fill what the first's leave free: the larger of two estimates.
+// One is all steps at the compute units' full rate - less of it while fewer than `at_once` share one - with part of the ends
+// and of the last workgroups; the other the compute unit with most steps, if all workgroups are there at once.  Fitted to 60
+// backward passes of all sizes with 40 to 126 pairs of cuts each: what this and pick() choose - separate launches, which
+// alone have the largest tiles, where that is estimated faster - is within 2.4 % of the best on average, one launch only where a
+// single round holds both within 6 % (18432 x 256 x 1024 bf16: 71 us then, 53 now; 3000 x 3000 x 100: 32, 21).
+float time_together(const TileCost& c, const Split& x, const Split& w) {
+  const int64_t n = x.groups + w.groups, most = (n + kCus - 1) / kCus, x_most = (x.groups + kCus - 1) / kCus;
+  const float at_once = (float)c.at_once, held = n <= kCus ? 1.f : n >= kCus * c.at_once ? at_once : (float)n / kCus;
+  auto rate = [&](float h) { return c.shared * (1.f + .4f * (1.f - h / at_once)); };     // a step's time, of h together
+  const float last = w.steps * (c.shared * held > c.alone ? c.shared * held : c.alone) + c.ends[2];
+  const float all = ((x.groups * x.steps + w.groups * w.steps) * rate(held) + n * c.ends[2] * .35f) / kCus + .25f * last;
+  const int longer = x.steps > w.steps ? x.steps : w.steps;
+  float one = longer * rate(at_once) * at_once;
+  if (most <= c.at_once) {
+    const int64_t l0 = x_most * x.steps + (most - x_most) * w.steps, l1 = l0 - x.steps + w.steps;
+    one = (l0 > l1 ? l0 : l1) * rate((float)most);
+  }
+  if (one < longer * c.alone) one = longer * c.alone;
+  one += c.ends[2];
+  return all > one ? all : one;
 }
 
 struct Shape {
@@ -194,11 +226,12 @@ constexpr int64_t kFew = 16;
 struct Backward {
   Split dx, dw;
   int parts;                 // of dg and du (Args::parts)
-  bool both;                 // the two products fit on the chip together: one launch, in the same tiles
+  bool both;                 // the two products in one launch, in the same tiles
   int gate_tile;
   int64_t dgu_bytes, col_bytes, dx_bytes, dw_bytes;
+  int64_t bytes() const { return 2 * parts * dgu_bytes + col_bytes + dx_bytes + dw_bytes; }
 };
-Backward plan_backward(const Shape& h) {
+Backward make_plan(const Shape& h) {
   Backward b;
   b.parts = h.dtype != MZ_F32 && h.M * h.F <= 8192 ? 2 : 1;
   const int only = b.parts == 2 ? 2 : -1;          // in the smallest tiles
@@ -206,25 +239,42 @@ Backward plan_backward(const Shape& h) {
   const int64_t fs = 2 * b.parts * h.steps(h.nk_F()), ms = b.parts * h.steps(h.nk_M());
   b.dx = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, only);
   b.dw = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, only);
-  // side by side, where one round of workgroups holds both: the longer of the two, not their sum
   b.both = false;
-  float least = b.dx.time + b.dw.time;
-  for (int t = b.parts; t < 3; ++t) {
-    const Split x = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, t), w = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, t);
-    const int64_t room = 256 * (h.dtype == MZ_F32 ? kCost32 : kCost16)[t].at_once;
-    const float longer = x.time > w.time ? x.time : w.time, time = longer + .3f * (x.time + w.time - longer);
-    if (x.groups + w.groups > room || time >= least) continue;
-    b.both = true;
-    least = time;
-    b.dx = x;
-    b.dw = w;
-  }
+  float least = b.dx.time + b.dw.time + 9.f;       // and a launch more
+  for (int t = b.parts; t < 3; ++t)                // parts: the smallest tiles only; the largest has no kernel of both
+    for_cuts(h.K, h.M, fs, t, 1, false, [&](const Split& x) {
+      for_cuts(h.K, h.F, ms, t, 2, false, [&](const Split& w) {
+        const float time = time_together(cost_of(h.dtype, t), x, w) + join_time(h.M * h.K, x.splits) + join_time(2 * h.F * h.K, w.splits);
+        if (time >= least) return;
+        b.both = true;
+        least = time;
+        b.dx = x;
+        b.dw = w;
+      });
+    });
   b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
   const int side = mz_gff::tile_side(b.gate_tile);
   b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
   b.dx_bytes = b.dx.splits > 1 ? round_up(b.dx.splits * h.M * h.K * 4, 256) : 0;
   b.dw_bytes = b.dw.splits > 1 ? round_up(b.dw.splits * 2 * h.F * h.K * 4, 256) : 0;
   return b;
+}
+
+// Weighing all pairs of cuts takes 4 us of the host, several times a training step of the same few sizes: each thread keeps
+// the plans of sizes it has met.
+Backward plan_backward(const Shape& h) {
+  struct Kept {
+    int64_t M = 0, K = 0, F = 0;                   // no plan has M = 0
+    int dtype = 0;
+    Backward plan;
+  };
+  thread_local Kept kept[16];
+  Kept& k = kept[(uint64_t)(h.M * 31 + h.K * 17 + h.F * 7 + h.dtype) % 16];
+  if (k.M != h.M || k.K != h.K || k.F != h.F || k.dtype != h.dtype) {
+    k.plan = make_plan(h);
+    k.M = h.M; k.K = h.K; k.F = h.F; k.dtype = h.dtype;
+  }
+  return k.plan;
 }
 
 int check_shape(const char* who, int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation) {
@@ -248,8 +298,7 @@ extern "C" {
 int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward) {
   if (check_shape("mz_gated_ff_workspace_bytes", M, K, F, dtype, 0)) return -1;
   if (!backward) return 0;
-  const Backward b = plan_backward(make_shape(M, K, F, dtype));
-  return 2 * b.parts * b.dgu_bytes + b.col_bytes + b.dx_bytes + b.dw_bytes;
+  return plan_backward(make_shape(M, K, F, dtype)).bytes();
 }
 
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
@@ -290,7 +339,7 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   const Shape sh = make_shape(M, K, F, dtype);
   if (int rc = check_stride("mz_gated_ff_bwd", sh, ldx)) return rc;
   const Backward plan = plan_backward(sh);
-  const int64_t need = mz_gated_ff_workspace_bytes(M, K, F, dtype, 1);
+  const int64_t need = plan.bytes();
   MZ_REQUIRE(workspace && workspace_bytes >= need && (size_t)workspace % 16 == 0,
              "mz_gated_ff_bwd: workspace too small (%lld of %lld bytes) or not 16-byte aligned", (long long)workspace_bytes,
              (long long)need);
