@@ -17,11 +17,12 @@
 //
 // What bounds it (MI355X): a step of the 256 x 256 tile keeps the matrix cores and LDS busy for 2048 cycles each (64
 // matrix instructions of 16 cycles a wavefront, two wavefronts a SIMD; 192 KB read and 64 KB staged at 128 bytes a cycle)
-// and takes 1.4 us, 3000 cycles or so at the clock the chip holds there; the smaller tiles read twice the bytes an
-// operation and lean on LDS.  8192 x 2048 x 8192 bf16: forward 426 us, input gradient 422, weight gradient 429 (1.28 to
-// 1.30 PFLOP/s), gate gradient 488 (1.13); the library's plain product of that size 452 (1.22).  18432 x 256 x 1024 bf16, where a tile has four steps: forward
-// 31 us, gate gradient 44 (113 MB of dh, dg and du), input gradient 28 - 288 tiles on 256 compute units - and weight
-// gradient 27.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the 151 TFLOP/s of a large product.
+// and takes 1.4 us, 3000 cycles or so at the clock the chip holds there; the 128 x 128 tile moves half as much again
+// through LDS an operation.  8192 x 2048 x 8192 bf16: forward 426 us, input gradient 422, weight gradient 429 (1.28 to 1.30
+// PFLOP/s), gate gradient 488 (1.13); the library's plain product of that size 452 (1.22).  18432 x 256 x 1024 bf16, where
+// a tile has four steps: forward 31 us, gate gradient 43 (113 MB of dh, dg and du), input gradient 28 - 288 tiles on 256
+// compute units - and weight gradient 27, the two in one launch 51.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the
+// 151 TFLOP/s of a large product.
 #pragma once
 #include "block_common.h"
 

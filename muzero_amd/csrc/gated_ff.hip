@@ -384,6 +384,7 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   q.out[0] = dw_gate; q.out[1] = dw_up; q.ldo = K;
   q.partial = reinterpret_cast<float*>(partial + plan.dx_bytes);
   q.splits = plan.dw.splits; q.steps_per_split = plan.dw.steps;
+  // a gradient asked for alone has the cut it has with the others: the same bits
   if (plan.both && dx && dw_gate) {
     if (int rc = launch_both(p, q, dtype, plan.dx.tile, s)) return rc;
   } else {
