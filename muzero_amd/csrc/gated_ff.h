@@ -732,13 +732,15 @@ __global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_gemm_kernel(Ar
   extern __shared__ __attribute__((aligned(16))) char lds[];
   gff_gemm<T, MODE, S, S, WR, WC, ACT>(a, blockIdx.x, gridDim.x, lds);
 }
-// the two products of a backward pass in one launch: workgroups 0 .. blocks_x - 1 (a multiple of 8) make the input
-// gradient, the others the weights'
+// the two products of a backward pass in one launch: the input gradient's workgroups (a multiple of 8 of each) come first,
+// or the weights' where those are the longer ones (3000 x 3000 x 100 bf16 backward: 43.1 us, 45.4 with the shorter first;
+// 52331 x 487 x 66: 78, 87)
 template <typename T, int S, int WR, int WC>
-__global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_both_kernel(Args x, Args w, unsigned blocks_x) {
+__global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_both_kernel(Args x, Args w, unsigned blocks_x, unsigned blocks_w, int w_first) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  if (blockIdx.x < blocks_x) gff_gemm<T, mz_gff::kInputGrad, S, S, WR, WC, kAnyActivation>(x, blockIdx.x, blocks_x, lds);
-  else gff_gemm<T, mz_gff::kWeightGrad, S, S, WR, WC, kAnyActivation>(w, blockIdx.x - blocks_x, gridDim.x - blocks_x, lds);
+  const bool is_x = w_first ? blockIdx.x >= blocks_w : blockIdx.x < blocks_x;
+  if (is_x) gff_gemm<T, mz_gff::kInputGrad, S, S, WR, WC, kAnyActivation>(x, w_first ? blockIdx.x - blocks_w : blockIdx.x, blocks_x, lds);
+  else gff_gemm<T, mz_gff::kWeightGrad, S, S, WR, WC, kAnyActivation>(w, w_first ? blockIdx.x : blockIdx.x - blocks_x, blocks_w, lds);
 }
 
 // workgroups of a product in S x S tiles, a multiple of the 8 XCDs: one a tile, or for pair products what the chip holds;
@@ -797,7 +799,8 @@ template <typename T, int S> int launch_both_in(const Args& x, const Args& w, hi
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
   const long bx = gemm_blocks<mz_gff::kInputGrad, S>(x), bw = gemm_blocks<mz_gff::kWeightGrad, S>(w);
   if (bx < 0 || bw < 0) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(bx + bw)), dim3(256), kLds, s, x, w, (unsigned)bx);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(bx + bw)), dim3(256), kLds, s, x, w, (unsigned)bx, (unsigned)bw,
+                     w.steps_per_split > x.steps_per_split ? 1 : 0);
   return MZ_OK;
 }
 template <typename T> int launch_both(const Args& x, const Args& w, int tile, hipStream_t s) {
