@@ -21,7 +21,7 @@
 // through LDS an operation.  8192 x 2048 x 8192 bf16: forward 426 us, input gradient 422, weight gradient 429 (1.28 to 1.30
 // PFLOP/s), gate gradient 488 (1.13); the library's plain product of that size 452 (1.22).  18432 x 256 x 1024 bf16, where
 // a tile has four steps: forward 31 us, gate gradient 43 (113 MB of dh, dg and du), input gradient 28 - 288 tiles on 256
-// compute units - and weight gradient 27, the two in one launch 51.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the
+// compute units - and weight gradient 27, the two in one launch 48.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the
 // 151 TFLOP/s of a large product.
 #pragma once
 #include "block_common.h"

@@ -177,19 +177,20 @@ Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only 
   return best;
 }
 
-// Two products in one launch, where the second's workgroups fill what the first's leave free: the larger of two estimates.
-// One is all steps at the compute units' full rate - less of it while fewer than `at_once` share one - with part of the ends
-// and of the last workgroups; the other the compute unit with most steps, if all workgroups are there at once.  Fitted to 60
-// backward passes of all sizes with 40 to 126 pairs of cuts each: what this and pick() choose - separate launches, which
-// alone have the largest tiles, where that is estimated faster - is within 2.4 % of the best on average, one launch only where a
-// single round holds both within 6 % (18432 x 256 x 1024 bf16: 71 us then, 53 now; 3000 x 3000 x 100: 32, 21).
+// Two products in one launch, the longer workgroups first and the others where those leave room: the larger of two
+// estimates.  One is all steps at the compute units' full rate - less of it while fewer than `at_once` share one - with part of
+// the ends and of the last workgroups; the other the compute unit with most steps, if all workgroups are there at once.
+// Fitted to 62 backward passes of all sizes with 40 to 126 pairs of cuts each: what this and pick() choose - separate
+// launches, which alone have the largest tiles, where that is estimated faster - is within 3 % of the best on average, one
+// launch only where a single round holds both within 6 % (18432 x 256 x 1024 bf16: 71 us then, 48 now; 3000 x 3000 x 100:
+// 32, 19).
 float time_together(const TileCost& c, const Split& x, const Split& w) {
   const int64_t n = x.groups + w.groups, most = (n + kCus - 1) / kCus, x_most = (x.groups + kCus - 1) / kCus;
   const float at_once = (float)c.at_once, held = n <= kCus ? 1.f : n >= kCus * c.at_once ? at_once : (float)n / kCus;
   auto rate = [&](float h) { return c.shared * (1.f + .4f * (1.f - h / at_once)); };     // a step's time, of h together
-  const float last = w.steps * (c.shared * held > c.alone ? c.shared * held : c.alone) + c.ends[2];
+  const int longer = x.steps > w.steps ? x.steps : w.steps, shorter = x.steps + w.steps - longer;
+  const float last = shorter * (c.shared * held > c.alone ? c.shared * held : c.alone) + c.ends[2];
   const float all = ((x.groups * x.steps + w.groups * w.steps) * rate(held) + n * c.ends[2] * .35f) / kCus + .25f * last;
-  const int longer = x.steps > w.steps ? x.steps : w.steps;
   float one = longer * rate(at_once) * at_once;
   if (most <= c.at_once) {
     const int64_t l0 = x_most * x.steps + (most - x_most) * w.steps, l1 = l0 - x.steps + w.steps;
