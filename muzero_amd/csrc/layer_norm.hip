@@ -2,8 +2,13 @@
 // that batch statistics do not suit: single states, unequal games):
 //     y = (x - m) r w + b,   m = mean(x),  r = 1 / sqrt(mean((x - m)^2) + eps)          per row
 //     dx = r (w dy - mean(w dy) - xh mean(w dy xh)),  dw = sum_rows dy xh,  db = sum_rows dy,   xh = (x - m) r
-// All sums in float32; the variance is the mean of squared deviations from the mean already known (a second pass over
-// registers), so a large common offset costs no digits.
+// All sums in float32 (rows too wide for registers: float64).  A float32 mean m0 is off by its own rounding and its sum's, which
+// under a large common offset is no small part of the deviations: a constant row of 12345.6 would come out as 0.3.  So
+// the second pass over the registers sums the deviations d = x - m0 too: t = mean(d) is what m0 is off by (x - m0 is exact
+// where it matters, x and m0 being close), m = m0 + t and var = mean(d^2) - t^2, the error of which is that of d's sums times
+// t^2, far below d's own.  The backward pass gets m rounded to float32 and finds t the same way, from the row it reads
+// anyway, in the same exchange as its other two sums:
+//     mean(w dy xh) = mean(w dy d r) - t r mean(w dy),   xh = (d - t) r
 //
 // HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx, each once.  A row lives in the
 // registers of a group of TPR threads (16, 32 or 64 lanes, or a workgroup), NV 16-byte vectors a thread; groups walk
@@ -11,10 +16,12 @@
 // Every workgroup leaves its dw and db in a float32 partial row and a second launch adds those up: no atomics, the
 // same bits on every run.
 //
-// Measured on an MI355X, forward / backward with both launches: 65536 x 4096 bf16 196 / 331 us (5.5 and 4.9 TB/s; a copy
-// of 2 GiB runs at 5.0), 18432 x 256 bf16 5.6 / 11.7 us, 4097 x 1001 float32 8.7 / 19.2 us, 1000 x 256 bf16 2.4 / 5.2 us:
-// the smaller ones live in the Infinity Cache and are bound by the launches' own time - a third of the backward's is the
-// second launch, a few workgroups that add up what up to 768 have left.
+// Measured on an MI355X, forward / backward with both launches: 65536 x 4096 bf16 204 / 330 us (5.3 and 4.9 TB/s; a copy
+// of 2 GiB runs at 5.0), 4000 x 16384 float32 98 / 167 us, 18432 x 256 bf16 5.7 / 11.7 us, 4097 x 1001 float32 9.4 / 18.3 us,
+// 1000 x 256 bf16 4.1 / 7.1 us: the smaller ones live in the Infinity Cache and are bound by the launches' own time - a third of
+// the backward's is the second launch, a few workgroups that add up what up to 768 have left.  Rows wider than registers: 2000 x
+// 32768 bf16 256 / 324 us.  What t costs: nothing at 65536 x 4096, 0.8 us of 8.6 in the forward pass of 4097 x 1001, and where
+// wide rows' parameters alone want gradients a pass over x (2000 x 32768: 53 us without, 92).
 #include "block_common.h"
 
 namespace {
@@ -31,25 +38,69 @@ struct LnArgs {
   float* mean;
   float* rstd;
   float* partial;          // [blocks][2][C]
+  float* shift;            // wide rows: [rows] t of the backward pass
   long ldx, lddy, rows;
   int C, affine_f32;
   float eps;
 };
 
-// sum of `v` over the TPR threads of a row; `red` holds one float per wavefront of the workgroup.  Rows wider than a
-// wavefront have the workgroup to themselves, and every thread of it gets here.
-template <int TPR> __device__ __forceinline__ float row_sum(float v, float* red) {
-  if constexpr (TPR <= 64) {
-    return lanes_sum<TPR>(v);
-  } else {
-    v = lanes_sum<64>(v);
-    __syncthreads();                        // the previous sum has been read
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = 0.f;
+// sums of v[0], v[1] .. over the TPR threads of a row; `red` holds K floats per wavefront of the workgroup.  Rows wider
+// than a wavefront have the workgroup to themselves, and every thread of it gets here.
+template <int TPR, int K> __device__ __forceinline__ void row_sums(float (&v)[K], float* red) {
 #pragma unroll
-    for (int i = 0; i < TPR / 64; ++i) s += red[i];
-    return s;
+  for (int k = 0; k < K; ++k) v[k] = lanes_sum<TPR <= 64 ? TPR : 64>(v[k]);
+  if constexpr (TPR > 64) {
+    __syncthreads();                        // the previous sums have been read
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[(threadIdx.x >> 6) * K + k] = v[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < TPR / 64; ++i) v[k] += red[i * K + k];
+    }
+  }
+}
+
+// a b, rounded: a mean whose product the compiler fused into some of the differences x - m0 and not into others would be two means
+__device__ __forceinline__ float product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
+// What was computed from `v` before is computed again after, not kept
+template <typename T> __device__ __forceinline__ void forget(Vec16<T>& v) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 t = __builtin_bit_cast(u32x4, v.v);
+  asm volatile("" : "+v"(t));
+  v.v = __builtin_bit_cast(typename Vec16<T>::type, t);
+}
+
+// the variance from the mean square q of the deviations and their mean t
+__device__ __forceinline__ float variance(float q, float t) {
+  return q < __FLT_MAX__ ? q - fminf(t * t, q) : q;            // t^2 <= q but for rounding; an overflowed q stays
+}
+
+// sums over the 1024 threads of a wide row in float64; `red` holds K doubles per wavefront
+template <int K> __device__ __forceinline__ void wide_sums(double (&v)[K], double* red) {
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) v[k] += __shfl_xor(v[k], m);
+  __syncthreads();                          // the previous sums have been read
+  if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) red[(threadIdx.x >> 6) * K + k] = v[k];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    v[k] = 0.;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[k] += red[i * K + k];
   }
 }
 
@@ -59,7 +110,7 @@ template <int TPR> constexpr int block_threads() { return TPR < 256 ? 256 : TPR;
 template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(block_threads<TPR>()) void ln_fwd_kernel(LnArgs a) {
   constexpr int N = Vec16<T>::N, RPB = block_threads<TPR>() / TPR;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  __shared__ float red[TPR > 64 ? TPR / 32 : 1];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const T* x = static_cast<const T*>(a.x);
   T* y = static_cast<T*>(a.out);
@@ -79,24 +130,27 @@ __global__ __launch_bounds__(block_threads<TPR>()) void ln_fwd_kernel(LnArgs a) 
       const int c = (k * TPR + lane) * N;
       v[k].load_upto(x + r * a.ldx + c, live ? a.C - c : 0);
     }
-    float s = 0.f;
+    float s[1] = {0.f};
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += (float)v[k].v[j];
-    const float mean = row_sum<TPR>(s, red) * inv_c;
-    float q = 0.f;
+      for (int j = 0; j < N; ++j) s[0] += (float)v[k].v[j];
+    row_sums<TPR>(s, red);
+    const float m0 = product(s[0], inv_c);
+    float q[2] = {0.f, 0.f};                // sums of d^2 and d
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float d = (float)v[k].v[j] - mean;
-        q += (k * TPR + lane) * N + j < a.C ? d * d : 0.f;
+        const float d = (k * TPR + lane) * N + j < a.C ? (float)v[k].v[j] - m0 : 0.f;
+        q[0] += d * d;
+        q[1] += d;
       }
-    const float rstd = 1.f / sqrtf(row_sum<TPR>(q, red) * inv_c + a.eps);
+    row_sums<TPR>(q, red);
+    const float t = q[1] * inv_c, rstd = 1.f / sqrtf(variance(q[0] * inv_c, t) + a.eps);
     if (!live) continue;
     if (a.mean && lane == 0) {
-      a.mean[r] = mean;
+      a.mean[r] = m0 + t;
       a.rstd[r] = rstd;
     }
 #pragma unroll
@@ -104,41 +158,47 @@ __global__ __launch_bounds__(block_threads<TPR>()) void ln_fwd_kernel(LnArgs a) 
       const int c = (k * TPR + lane) * N;
       Vec16<T> o;
 #pragma unroll
-      for (int j = 0; j < N; ++j) o.v[j] = (T)(((float)v[k].v[j] - mean) * rstd * w[k][j] + b[k][j]);
+      for (int j = 0; j < N; ++j) o.v[j] = (T)(((float)v[k].v[j] - m0 - t) * rstd * w[k][j] + b[k][j]);
       o.store_upto(y + r * (long)a.C + c, a.C - c);
     }
   }
 }
 
-// rows wider than the registers of a workgroup: three passes over the row, the later two out of the caches
+// rows wider than the registers of a workgroup: three passes over the row, the later two out of the caches.  A thread's sum
+// has up to 2^14 terms, which float32 would not hold to the digits that the deviations need: float64, and the mean is used as
+// two floats.
 template <typename T> __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel(LnArgs a) {
   constexpr int N = Vec16<T>::N;
-  __shared__ float red[16];
-  const float inv_c = 1.f / (float)a.C;
+  __shared__ double red[16];
   for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + r * a.ldx;
     T* y = static_cast<T*>(a.out) + r * (long)a.C;
-    float s = 0.f;
+    double s[1] = {0.};
     for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
       Vec16<T> v;
       v.load_upto(x + c, a.C - c);
 #pragma unroll
-      for (int j = 0; j < N; ++j) s += (float)v.v[j];
+      for (int j = 0; j < N; ++j) s[0] += (double)(float)v.v[j];
     }
-    const float mean = row_sum<1024>(s, red) * inv_c;
-    float q = 0.f;
+    wide_sums(s, red);
+    const double mean = s[0] / a.C;
+    const float m0 = (float)mean, t = (float)(mean - (double)m0);
+    double q[1] = {0.};
     for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
       Vec16<T> v;
       v.load_upto(x + c, a.C - c);
+      float part = 0.f;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float d = (float)v.v[j] - mean;
-        q += c + j < a.C ? d * d : 0.f;
+        const float d = (float)v.v[j] - m0 - t;
+        part += c + j < a.C ? d * d : 0.f;
       }
+      q[0] += (double)part;
     }
-    const float rstd = 1.f / sqrtf(row_sum<1024>(q, red) * inv_c + a.eps);
+    wide_sums(q, red);
+    const float rstd = 1.f / sqrtf((float)(q[0] / a.C) + a.eps);
     if (a.mean && threadIdx.x == 0) {
-      a.mean[r] = mean;
+      a.mean[r] = m0;
       a.rstd[r] = rstd;
     }
     for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
@@ -149,7 +209,7 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_fwd_wide_kernel
         if (c + j < a.C) {
           const float w = a.weight ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
           const float b = a.bias ? load_param<T>(a.bias, a.affine_f32, c + j) : 0.f;
-          v.v[j] = (T)(((float)v.v[j] - mean) * rstd * w + b);
+          v.v[j] = (T)(((float)v.v[j] - m0 - t) * rstd * w + b);
         }
       v.store_upto(y + c, a.C - c);
     }
@@ -161,7 +221,12 @@ template <typename T, int TPR, int NV>
 __global__ __launch_bounds__(block_threads<TPR>()) void ln_bwd_kernel(LnArgs a) {
   constexpr int N = Vec16<T>::N, RPB = block_threads<TPR>() / TPR;
   constexpr int kCols = TPR * NV * N;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  // Across a row's sums a thread of many columns keeps x and dy in the elements' type, not their float32 derivatives, and compares
+  // its columns with C anew for every row, not in two scalar registers each: all that kept takes 147 registers instead of 112 at
+  // 4096 columns of 16 bits, and 1024 threads spill (4000 x 16384 float32: 211 us).  With few columns there is room (18432 x 256
+  // bf16: 12.1 us, 12.6 the other way).
+  constexpr bool kTight = NV * N > 8;
+  __shared__ float red[TPR > 64 ? 3 * TPR / 64 : 1];
   __shared__ float cols[RPB > 1 ? RPB * 2 * kCols : 1];
   const int lane = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const T* x = static_cast<const T*>(a.x);
@@ -186,30 +251,37 @@ __global__ __launch_bounds__(block_threads<TPR>()) void ln_bwd_kernel(LnArgs a) 
       gv[k].load_upto(dy + r * a.lddy + c, live ? a.C - c : 0);
     }
     const float mean = live ? a.mean[r] : 0.f, rstd = live ? a.rstd[r] : 0.f;
-    float s1 = 0.f, s2 = 0.f;               // sums of w dy and of w dy xh; columns past the end have dy = 0
+    float s[3] = {0.f, 0.f, 0.f};           // sums of w dy, w dy d r and d; columns past the end have dy = 0
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+    for (int k = 0; k < NV; ++k) {
+      int left = a.C - (k * TPR + lane) * N;
+      if constexpr (kTight) asm volatile("" : "+v"(left));
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float g = (float)gv[k].v[j], xh = ((float)xv[k].v[j] - mean) * rstd;
-        dw[k][j] += g * xh;
-        db[k][j] += g;
-        s1 += g * w[k][j];
-        s2 += g * w[k][j] * xh;
+        const float g = (float)gv[k].v[j] * w[k][j], d = (float)xv[k].v[j] - mean;
+        s[0] += g;
+        s[1] += g * (d * rstd);
+        s[2] += j < left ? d : 0.f;
       }
-    if (!a.out) continue;                   // only the parameters' gradients are wanted
-    const float m1 = row_sum<TPR>(s1, red) * inv_c, m2 = row_sum<TPR>(s2, red) * inv_c;
-    if (!live) continue;
+      if constexpr (kTight) {
+        forget(xv[k]);
+        forget(gv[k]);
+      }
+    }
+    row_sums<TPR>(s, red);
+    const float t = s[2] * inv_c, m1 = s[0] * inv_c, m2 = s[1] * inv_c - t * rstd * m1;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * TPR + lane) * N;
       Vec16<T> o;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const float xh = ((float)xv[k].v[j] - mean) * rstd;
-        o.v[j] = (T)(rstd * ((float)gv[k].v[j] * w[k][j] - m1 - xh * m2));
+        const float g = (float)gv[k].v[j], xh = ((float)xv[k].v[j] - mean - t) * rstd;
+        dw[k][j] += g * xh;
+        db[k][j] += g;
+        o.v[j] = (T)(rstd * (g * w[k][j] - m1 - xh * m2));
       }
-      o.store_upto(dx + r * (long)a.C + c, a.C - c);
+      if (a.out && live) o.store_upto(dx + r * (long)a.C + c, a.C - c);
     }
   }
   if (!a.partial) return;
@@ -246,29 +318,40 @@ __global__ __launch_bounds__(block_threads<TPR>()) void ln_bwd_kernel(LnArgs a) 
   }
 }
 
+// wide rows: dx, and each row's t for the column sums; without dx only the latter
 template <typename T> __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel(LnArgs a) {
   constexpr int N = Vec16<T>::N;
-  __shared__ float red[16];
-  const float inv_c = 1.f / (float)a.C;
+  __shared__ double red[3 * 16];
   for (long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + r * a.ldx;
     const T* dy = static_cast<const T*>(a.dy) + r * a.lddy;
     T* dx = static_cast<T*>(a.out) + r * (long)a.C;
     const float mean = a.mean[r], rstd = a.rstd[r];
-    float s1 = 0.f, s2 = 0.f;
+    double s[3] = {0., 0., 0.};             // sums of w dy, w dy d r and d
     for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
       Vec16<T> xv, gv;
+      float part[3] = {0.f, 0.f, 0.f};
       xv.load_upto(x + c, a.C - c);
-      gv.load_upto(dy + c, a.C - c);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float w = a.weight && c + j < a.C ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
-        const float g = (float)gv.v[j] * w;
-        s1 += g;
-        s2 += g * ((float)xv.v[j] - mean) * rstd;
+      for (int j = 0; j < N; ++j) part[2] += c + j < a.C ? (float)xv.v[j] - mean : 0.f;
+      if (a.out) {
+        gv.load_upto(dy + c, a.C - c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const float w = a.weight && c + j < a.C ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
+          const float g = (float)gv.v[j] * w;
+          part[0] += g;
+          part[1] += g * (((float)xv.v[j] - mean) * rstd);
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 3; ++k) s[k] += (double)part[k];
     }
-    const float m1 = row_sum<1024>(s1, red) * inv_c, m2 = row_sum<1024>(s2, red) * inv_c;
+    wide_sums(s, red);
+    const float t = (float)(s[2] / a.C);
+    if (a.shift && threadIdx.x == 0) a.shift[r] = t;
+    if (!a.out) continue;
+    const float m1 = (float)(s[0] / a.C), m2 = (float)(s[1] / a.C - s[2] / a.C * rstd * (s[0] / a.C));
     for (int c = threadIdx.x * N; c < a.C; c += 1024 * N) {
       Vec16<T> xv, gv;
       xv.load_upto(x + c, a.C - c);
@@ -276,7 +359,7 @@ template <typename T> __global__ __launch_bounds__(1024) void ln_bwd_wide_kernel
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float w = a.weight && c + j < a.C ? load_param<T>(a.weight, a.affine_f32, c + j) : 1.f;
-        const float xh = ((float)xv.v[j] - mean) * rstd;
+        const float xh = ((float)xv.v[j] - mean - t) * rstd;
         gv.v[j] = (T)(rstd * ((float)gv.v[j] * w - m1 - xh * m2));
       }
       gv.store_upto(dx + c, a.C - c);
@@ -296,11 +379,11 @@ template <typename T> __global__ __launch_bounds__(256) void ln_bwd_wide_cols_ke
     Vec16<T> xv, gv;
     xv.load_upto(static_cast<const T*>(a.x) + r * a.ldx + c, a.C - c);
     gv.load_upto(static_cast<const T*>(a.dy) + r * a.lddy + c, a.C - c);
-    const float mean = a.mean[r], rstd = a.rstd[r];
+    const float mean = a.mean[r], t = a.shift[r], rstd = a.rstd[r];
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float g = (float)gv.v[j];
-      dw[j] += g * ((float)xv.v[j] - mean) * rstd;
+      dw[j] += g * (((float)xv.v[j] - mean - t) * rstd);
       db[j] += g;
     }
   }
@@ -400,7 +483,7 @@ template <typename T> int ln_fwd(const LnArgs& a, hipStream_t s) {
 template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hipStream_t s) {
   int blocks = 0;
   if (a.C > kMaxRegisterCols) {
-    if (a.out)
+    if (a.out || a.partial)
       hipLaunchKernelGGL((ln_bwd_wide_kernel<T>), dim3(row_blocks(a.rows, 1, 2 * mz::compute_units())), dim3(1024), 0, s, a);
     if (a.partial) {
       constexpr int kCols = 256 * Vec16<T>::N;
@@ -412,7 +495,9 @@ template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hi
     }
   } else {
     with_shape<T>(a.C, [&](auto tpr, auto nv) {
-      constexpr int TPR = decltype(tpr)::value, NV = decltype(nv)::value, NT = block_threads<TPR>();
+      // the widest float32 rows on half the threads with twice the registers: 1024 threads spill (4000 x 16384: 230 us)
+      constexpr bool kHalve = decltype(tpr)::value == 1024 && sizeof(T) == 4;
+      constexpr int TPR = kHalve ? 512 : decltype(tpr)::value, NV = kHalve ? 8 : decltype(nv)::value, NT = block_threads<TPR>();
       blocks = bwd_blocks(a.rows, NT / TPR, NT);
       hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV>), dim3(blocks), dim3(NT), 0, s, a);
       return MZ_OK;
@@ -423,6 +508,8 @@ template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hi
                        dbias, a.affine_f32);
   return MZ_OK;
 }
+
+int64_t partial_floats(int64_t rows, int32_t C) { return (rows < kMaxPartials ? rows : kMaxPartials) * 2 * (int64_t)C; }
 
 int check(const char* who, int64_t rows, int32_t C, int64_t ld, int32_t dtype, int32_t affine_dtype) {
   MZ_REQUIRE(rows > 0 && C > 0 && C <= (1 << 24), "%s: rows > 0 and 0 < C <= 2^24 expected (rows = %lld, C = %d)", who,
@@ -443,7 +530,7 @@ int mz_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void
   MZ_REQUIRE((mean == nullptr) == (rstd == nullptr), "mz_layer_norm_fwd: mean and rstd go together");
   if (int rc = check("mz_layer_norm_fwd", rows, C, ldx, dtype, affine_dtype)) return rc;
   MZ_REQUIRE(eps >= 0.0, "mz_layer_norm_fwd: eps must not be negative");
-  const LnArgs a = {x, nullptr, weight, bias, y, mean, rstd, nullptr, ldx, 0, rows, C, affine_dtype == MZ_F32, (float)eps};
+  const LnArgs a = {x, nullptr, weight, bias, y, mean, rstd, nullptr, nullptr, ldx, 0, rows, C, affine_dtype == MZ_F32, (float)eps};
   hipStream_t s = mz::as_stream(stream);
   if (dtype == MZ_F32) ln_fwd<float>(a, s);
   else if (dtype == MZ_BF16) ln_fwd<__bf16>(a, s);
@@ -453,7 +540,7 @@ int mz_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void
 
 int64_t mz_layer_norm_workspace_bytes(int64_t rows, int32_t C) {
   if (rows <= 0 || C <= 0) return 0;
-  return (rows < kMaxPartials ? rows : kMaxPartials) * 2 * (int64_t)C * 4;
+  return partial_floats(rows, C) * 4 + (C > kMaxRegisterCols ? rows * 4 : 0);
 }
 
 int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, const void* weight, int32_t affine_dtype,
@@ -466,8 +553,9 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
   const bool params = dweight || dbias;
   MZ_REQUIRE(!params || (workspace && workspace_bytes >= mz_layer_norm_workspace_bytes(rows, C) && (size_t)workspace % 4 == 0),
              "mz_layer_norm_bwd: workspace too small or not aligned to float");
-  const LnArgs a = {x, dy, weight, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd),
-                    params ? static_cast<float*>(workspace) : nullptr, ldx, lddy, rows, C, affine_dtype == MZ_F32, 0.f};
+  float* partial = params ? static_cast<float*>(workspace) : nullptr;
+  float* shift = params && C > kMaxRegisterCols ? partial + partial_floats(rows, C) : nullptr;
+  const LnArgs a = {x, dy, weight, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd), partial, shift, ldx, lddy, rows, C, affine_dtype == MZ_F32, 0.f};
   hipStream_t s = mz::as_stream(stream);
   if (dtype == MZ_F32) ln_bwd<float>(a, dweight, dbias, s);
   else if (dtype == MZ_BF16) ln_bwd<__bf16>(a, dweight, dbias, s);

@@ -1,0 +1,117 @@
+"""What the training-block operators (muzero_amd.blocks) lose to rounding where float32 has few digits to spare, against
+float64.  Bounds are derived, not fitted; u = 2^-24 is float32's half step."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def half(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps / 2
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, t=torch.float32, scale=1.0, mean=0.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale + mean).to(t)
+
+
+def within(got, ref, bound, what):
+    bound = bound + half(got.dtype) * (ref.abs() + bound) + tiny(got.dtype)
+    bad = ~((got.double() - ref).abs() <= bound)
+    assert not bad.any(), (what, int(bad.sum()), got[bad][:3].tolist(), ref[bad][:3].tolist(), bound[bad][:3].tolist())
+
+
+def layer_norm_bounds(x, w, dy, eps):
+    """The definition in float64 and the room that float32 needs when the mean's own rounding does not count.
+
+    With d the additions a term of a row's sum passes through, a float32 mean m0 is off by e = (d + 2) u max|x|.  The
+    deviations x - m0 are off by u of themselves, their mean t by (d + 3) u of their mean size, and so what is left,
+    x - m0 - t, by E = (d + 6) u (|dev| + mean|dev| + e) in all: of e only its product with u stays.  The variance is
+    off by (d + 6) u (var + 2 e^2)."""
+    c = x.shape[1]
+    d = 24 + max(16, c / 1024)
+    xd, dyd, wd = x.double(), dy.double(), w.double()
+    dev = xd - xd.mean(1, keepdim=True)
+    var = (dev ** 2).mean(1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(var + eps)
+    xh = dev * rstd
+    e = (d + 2) * U * xd.abs().amax(1, keepdim=True)
+    e_dev = (d + 6) * U * (dev.abs() + dev.abs().mean(1, keepdim=True) + e)
+    rel = (d + 6) * U * (var + 2 * e ** 2) / (var + eps) + 4 * U
+    e_xh = rstd * e_dev + xh.abs() * rel
+    g = dyd * wd
+    m1, m2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+    size = rstd * (dev.abs() + e)                        # what the sums of dx are made of
+    e_m1 = (d + 2) * U * g.abs().mean(1, keepdim=True)
+    e_m2 = (d + 8) * U * ((g.abs() * size).mean(1, keepdim=True) + rstd * e * m1.abs() + rstd * e * g.abs().mean(1, keepdim=True))
+    e_m2 = e_m2 + (g.abs() * e_xh).mean(1, keepdim=True)
+    inner = g.abs() + m1.abs() + (xh * m2).abs()
+    e_dx = rstd * (e_m1 + xh.abs() * e_m2 + e_xh * (m2.abs() + e_m2) + 6 * U * inner) + rel * rstd * inner
+    dc = x.shape[0] + 70
+    dw, e_dw = (dyd * xh).sum(0), (dc * U * (dyd * xh).abs() + dyd.abs() * e_xh * (1 + dc * U)).sum(0)
+    return xh, e_xh, rstd * (g - m1 - xh * m2), e_dx, dw, e_dw, dyd.sum(0), dc * U * dyd.abs().sum(0)
+
+
+def check_layer_norm(x, w, b, dy, eps=1e-5):
+    from muzero_amd import blocks
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    y = blocks.layer_norm(*leaves, eps=eps)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    xh, e_xh, dxr, e_dx, dwr, e_dw, dbr, e_db = layer_norm_bounds(x, w, dy, eps)
+    wd, bd = w.double(), b.double()
+    within(y.detach(), xh * wd + bd, e_xh * wd.abs() + 3 * U * (xh * wd).abs() + 2 * U * bd.abs(), "y")
+    within(dx, dxr, e_dx, "dx")
+    within(dw, dwr, e_dw, "dweight")
+    within(db, dbr, e_db, "dbias")
+    only = torch.autograd.grad(blocks.layer_norm(x, leaves[1], b, eps=eps), leaves[1], dy)[0]       # without dx: the same bits
+    assert torch.equal(only, dw)
+
+
+@pytest.mark.parametrize("c", [24, 100, 257, 777, 1001, 3000, 8191, 16001, 20001, 40000])
+def test_constant_rows_give_the_bias(c):
+    """Values that are no short binary fractions at widths that are no powers of two: nothing of the mean's rounding may
+    be left in y."""
+    g = gen(c)
+    values = torch.tensor([12345.6, 54321.0, 1000.1, 100.1, -7.3e6, 0.1, -3.3e-5], device="cuda")
+    x = values[:, None].expand(7, c).contiguous()
+    check_layer_norm(x, normal(g, c, mean=1.0), normal(g, c), normal(g, 7, c))
+
+
+@pytest.mark.parametrize("offset", [1e2, 1e4, 1e6])
+@pytest.mark.parametrize("rows,c", [(6, 40), (40, 777), (300, 1001), (5, 9000), (4, 20001)])
+def test_common_offset_costs_no_digits(rows, c, offset):
+    g = gen(rows + c)
+    x = normal(g, rows, c, mean=offset)
+    check_layer_norm(x, normal(g, c, mean=1.0), normal(g, c), normal(g, rows, c))
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("c", [100, 1001, 5000, 20001])
+def test_common_offset_in_16_bits(c, t):
+    g = gen(c + 1)
+    x = torch.cat([normal(g, 20, c, t=TYPES[t], mean=100.0), torch.full((2, c), 1000.1, device="cuda").to(TYPES[t])])
+    check_layer_norm(x, normal(g, c, mean=1.0), normal(g, c), normal(g, 22, c, t=TYPES[t]))
+
+
+def test_rows_whose_squares_overflow_and_bad_rows():
+    """Deviations of 1e30 have no float32 square: y is the bias, as before and as in torch; NaN and infinity stay in their row."""
+    from muzero_amd import blocks
+    g = gen(5)
+    for c in (100, 3000, 20001):
+        x, b = normal(g, 4, c), normal(g, c)
+        good = blocks.layer_norm(x, None, b)
+        x[1] *= 1e30
+        x[2, 5] = float("nan")
+        x[3, c - 1] = float("inf")
+        y = blocks.layer_norm(x, None, b)
+        assert torch.equal(y[0], good[0]) and torch.equal(y[1], b) and torch.isnan(y[2]).all() and torch.isnan(y[3]).all()
