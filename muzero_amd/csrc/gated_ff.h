@@ -370,6 +370,7 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
   };
   // of the lane's four features in the wavefront's block i
   constexpr bool kBiasFirst = kPair && sizeof(T) == 2;
+  constexpr long kBiasFirstK = 1 << 15;
   const int lr = (lane >> 4) * 4, lc = lane & 15;
   auto bias_of = [&](int i) __attribute__((always_inline)) {
     const int f = (i / (RM / 2)) * TR + (wr * (RM / 2) + i % (RM / 2)) * 16 + lr;
@@ -435,11 +436,13 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
     }
     __syncthreads();
     // a pair product's sums start at the biases in the 16-bit types: two additions less for every output of the epilogue
-    // (18432 x 256 x 1024 bf16: 27.8 us, added there 29.7), and what a large bias costs the sum's last float32 digits is far
-    // below the result's rounding; float32 keeps those digits and adds the bias last
+    // (18432 x 256 x 1024 bf16: 27.8 us, added there 29.7).  Each of the sum's additions, one for 32 values of k, then loses up to 2^-24
+    // of the bias: 2^-14 of it at K = 2^15, an eighth of float16's half step, so that longer sums add it last, and so does
+    // float32, which keeps those digits.
+    const bool bias_now = kBiasFirst && a.nk_all <= kBiasFirstK;
 #pragma unroll
     for (int i = 0; i < RM; ++i) {
-      const f32x4 start = kBiasFirst ? bias_of(i) : f32x4{0.f, 0.f, 0.f, 0.f};
+      const f32x4 start = bias_now ? bias_of(i) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < CN; ++j) acc[i][j] = start;
     }
@@ -523,6 +526,13 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
         }
       }
       __syncthreads();
+    }
+
+    if (kBiasFirst && !bias_now) {
+#pragma unroll
+      for (int i = 0; i < RM; ++i)
+#pragma unroll
+        for (int j = 0; j < CN; ++j) acc[i][j] += bias_of(i);
     }
 
     const long er = r0, ec = c0;     // the tile whose epilogue follows

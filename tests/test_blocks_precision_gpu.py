@@ -115,3 +115,32 @@ def test_rows_whose_squares_overflow_and_bad_rows():
         x[3, c - 1] = float("inf")
         y = blocks.layer_norm(x, None, b)
         assert torch.equal(y[0], good[0]) and torch.equal(y[1], b) and torch.isnan(y[2]).all() and torch.isnan(y[3]).all()
+
+
+# ------------------------------------------------------------------------------------------- gated feed-forward
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [9, 64, 300])
+def test_gated_ff_long_sums_beside_large_biases(rows, t):
+    """2^20 terms of 1.9 x 2^-18 beside a bias of 4096: 32 of them are below the last float32 digit of the bias, all of them two
+    steps of a float16 result.  Gradients: dW_up = sum act(g), which takes g's value, and dW_gate = sum dh u."""
+    from muzero_amd import blocks
+    t = TYPES[t]
+    k, f = 1 << 20, 24
+    x = torch.ones(rows, k, dtype=t, device="cuda")
+    wg = torch.full((f, k), 1.9 * 2.0 ** -18, device="cuda").to(t)
+    wu, bg, bu = torch.zeros_like(wg), torch.full((f,), 4096.0, dtype=t, device="cuda"), torch.ones(f, dtype=t, device="cuda")
+    leaves = [v.requires_grad_() for v in (wg, wu)]
+    h = blocks.gated_ff(x, *leaves, bg, bu, activation="relu")
+    gate = 4096.0 + k * wg[0, 0].double().item()
+    # the sum's own error: K / 16 additions at most (float32: K) that each lose u of at most its 8 - 2^20 u 8 = 0.5
+    n = k if t == torch.float32 else k // 16
+    room = torch.full((rows, f), n * U * (gate - 4096.0) + 3 * U * gate, dtype=torch.float64, device="cuda")
+    within(h.detach(), torch.full_like(room, gate), room, "h")
+    dh = torch.full((rows, f), 2.0 ** -10, dtype=t, device="cuda")
+    dwg, dwu = torch.autograd.grad(h, leaves, dh)
+    # every term is the same: one rounding of dg = 2^-10 (exact) and of du = 2^-10 gate, which is held in t, and the sum's
+    step = half(t) if t != torch.float32 else 0.0
+    ref, off = rows * 2.0 ** -10 * gate, rows * 2.0 ** -10 * (room[0, 0].item() + step * gate)
+    bound = torch.full((f, k), off + (rows + 40) * U * ref, dtype=torch.float64, device="cuda")
+    within(dwu, torch.full_like(bound, ref), bound, "dw_up")
+    assert (dwg == rows * 2.0 ** -10).all()
