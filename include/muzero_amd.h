@@ -600,7 +600,7 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
  * be 0 (then NULL will do).
  * Backward: recomputes both products; dh [M][F] -> dx [M][K], dw_gate / dw_up [F][K] (both or neither), db_gate / db_up
  * [F]; NULL for what is not wanted.  The gradients of the two products are rounded to `dtype` between the launches
- * (16-bit types with M F <= 8192 carry what that rounding left in a second term).
+ * (16-bit types with M F <= 8192 and K F <= 2^21 carry what that rounding left in a second term).
  * workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 1) bytes, 16-byte aligned.  No atomics. */
 int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward);
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,

@@ -55,8 +55,10 @@ def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optio
     ``torch.autocast`` they are cast to its dtype first, as torch's linear does).  activation: "silu", "gelu" (erf),
     "relu" or "sigmoid".  Returns [..., F].  The backward pass computes the two products again from x: nothing of the
     hidden width is kept but the result; while it runs it takes scratch of twice the result's size and for the partial
-    results of sums that are cut over workgroups.  In bfloat16 and float16 it rounds the products' gradients to that type
-    (they are matrix operands next; where there are at most 8192 of each, what the rounding left is carried along);
+    results of sums that are cut over workgroups.  In bfloat16 and float16 it rounds the two products' gradients to that
+    type, matrix operands as they are next: gradients of x and the weights are then off by sqrt(2) times what rounding the
+    result alone costs (relative RMS 2.4e-3 in bfloat16, 2.9e-4 in float16), at any size.  Small problems - rows x F up to
+    8192 and K x F up to 2^21 - carry what that rounding left along and are off by the result's rounding alone.
     float16 gradients below 6e-5 lose digits and those above 65504 overflow as any float16 value does - scale the loss."""
     return (_ext or _load()).gated_ff(x, w_gate, w_up, b_gate, b_up, activation)
 

@@ -5,9 +5,12 @@
 // Forward is one kernel: a wavefront owns the gate and the up product of the same features, so activation and product
 // happen in its registers and only h is written.  Nothing else is kept for the backward pass: it computes g and u again
 // (4 M K F operations against 8 M F bytes written and read back in 16 bits - and without rounding g and u), writes
-// dg and du in the operands' type - they are matrix operands next, and their rounding adds one half step to a sum's
-// terms, which averages out over a sum as long as they are many - and runs the two products that need them.  Where there
-// are few (16-bit types, M F <= 8192) what the rounding left goes along as a second operand of the same products.  Sums
+// dg and du in the operands' type - they are matrix operands next - and runs the two products that need them.
+// What rounding dg and du to 16 bits costs: every term of dx and dW is off by its own relative error, independent of the others', so
+// the sums are off by that error relative to their own size however long they are; with the result's rounding, as large, that
+// is sqrt(2) of it (relative RMS 2.35e-3 in bf16 and 2.9e-4 in f16 against 1.66e-3 and 2.1e-4, measured from 32 x 256 x 256
+// to 18432 x 256 x 1024 alike).  A second operand that holds what the rounding left takes that away and doubles the products'
+// steps.  It is carried where a pass is bound by its launches and that is all but free, see make_plan().  Sums
 // over few tiles are split along k into float32 partial results that a second launch adds up in a fixed order: no atomics,
 // the same bits on every run.
 #include "gated_ff.h"
@@ -234,7 +237,11 @@ struct Backward {
 };
 Backward make_plan(const Shape& h) {
   Backward b;
-  b.parts = h.dtype != MZ_F32 && h.M * h.F <= 8192 ? 2 : 1;
+  // Second parts of dg and du in the 16-bit types (above) where they cost 0 to 4 us: kernels of the backward pass without / with them
+  // 32 x 256 x 256 12.3 / 12.0 us, 90 x 64 x 72 10.9 / 11.8, 8000 x 256 x 1 15.2 / 17.5, 4 x 1024 x 2048 19.4 / 23.4.  Past these
+  // limits they cost the products' time again: 128 x 256 x 1024 13.1 / 15.0, 1000 x 250 x 700 22.7 / 30.1, 1024 x 256 x 1024
+  // 22.7 / 34.2, and the weights' second reading 1 x 4096 x 8192 77.8 / 127.4.
+  b.parts = h.dtype != MZ_F32 && h.M * h.F <= 8192 && h.K * h.F <= 1 << 21 ? 2 : 1;
   const int only = b.parts == 2 ? 2 : -1;          // in the smallest tiles
   b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad, only).tile;
   const int64_t fs = 2 * b.parts * h.steps(h.nk_F()), ms = b.parts * h.steps(h.nk_M());

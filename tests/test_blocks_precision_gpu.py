@@ -1,5 +1,7 @@
 """What the training-block operators (muzero_amd.blocks) lose to rounding where float32 has few digits to spare, against
 float64.  Bounds are derived, not fitted; u = 2^-24 is float32's half step."""
+import math
+
 import pytest
 import torch
 
@@ -144,3 +146,30 @@ def test_gated_ff_long_sums_beside_large_biases(rows, t):
     bound = torch.full((f, k), off + (rows + 40) * U * ref, dtype=torch.float64, device="cuda")
     within(dwu, torch.full_like(bound, ref), bound, "dw_up")
     assert (dwg == rows * 2.0 ** -10).all()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,k,f,carried", [(32, 256, 256, True), (90, 130, 72, True), (8, 2048, 1024, True), (1, 1500, 8192, False),
+                                              (2, 4100, 4000, False), (33, 256, 256, False), (130, 200, 1000, False),
+                                              (2500, 512, 700, False)])
+def test_gated_ff_gradients_are_off_by_one_rounding_or_two(rows, k, f, carried, t):
+    """The documented error of 16-bit gradients, on both sides of both limits.  Rounding a number m 2^e, 1 <= m < 2, is off by a
+    uniform error of up to half = 2^(e - p): RMS half / (sqrt(3) m) relative, and with m spread over its logarithm, E 1/m^2 =
+    3 / (8 ln 2), sqrt(3 / (8 ln 2) / 3) half = 0.425 half.  Terms that were rounded before give the sum as much again,
+    independent of the result's: sqrt(2) of it.  A tenth of room: at 10^4 elements and more the RMS itself is sharp to a
+    hundredth, the spread of m is not exactly that."""
+    from muzero_amd import blocks
+    t = TYPES[t]
+    g = gen(rows + f)
+    x, wg, wu = (normal(g, *s, t=t, scale=sc).requires_grad_() for s, sc in (((rows, k), 1.0), ((f, k), k ** -0.5), ((f, k), k ** -0.5)))
+    dh = normal(g, rows, f, t=t)
+    got = torch.autograd.grad(blocks.gated_ff(x, wg, wu), (x, wg, wu), dh)
+    xd, gd, ud = (v.detach().double() for v in (x, wg, wu))
+    gate, up = xd @ gd.t(), xd @ ud.t()
+    sig = torch.sigmoid(gate)
+    dg, du = dh.double() * up * sig * (1 + gate * (1 - sig)), dh.double() * gate * sig
+    one = (3 / (8 * math.log(2)) / 3) ** 0.5 * half(t)
+    for v, ref, name in zip(got, (dg @ gd + du @ ud, dg.t() @ xd, du.t() @ xd), ("x", "w_gate", "w_up")):
+        off = ((v.double() - ref).norm() / ref.norm()).item()
+        if v.numel() >= 10000:
+            assert off <= 1.1 * one * (1 if carried else 2 ** 0.5), (name, off, one)
