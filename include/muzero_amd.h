@@ -603,6 +603,12 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
  * (16-bit types with M F <= 8192 and K F <= 2^21 carry what that rounding left in a second term).
  * workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 1) bytes, 16-byte aligned.  No atomics. */
 int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t backward);
+/* The kernels that calls of these sizes run, for tuning and tests; no GPU is needed.  want_dx, want_dw: whether a backward
+ * pass makes the gradients of x and of the weights.  plan [8]: side of the output tiles of the forward pass (0: the streaming
+ * kernel of up to 16 rows), of the products recomputed in the backward pass, of dx, parts that dx's sums are cut into, side and
+ * parts of the weights' gradients (0 where not wanted), 1 if dx and these share a launch, terms (1 or 2) that the products'
+ * gradients are held in. */
+int mz_gated_ff_plan(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t want_dx, int32_t want_dw, int32_t* plan);
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
                     int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation, void* h, void* workspace,
                     int64_t workspace_bytes, mz_stream_t stream);

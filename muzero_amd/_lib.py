@@ -120,6 +120,7 @@ _SIGNATURES = {
     "mz_layer_norm_bwd": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int32, _P, _P, C.c_int64, C.c_int32, C.c_int32, _P,
                                     _P, _P, _P, C.c_int64, _P]),
     "mz_gated_ff_workspace_bytes": (C.c_int64, [C.c_int64] * 3 + [C.c_int32] * 2),
+    "mz_gated_ff_plan": (C.c_int, [C.c_int64] * 3 + [C.c_int32] * 3 + [C.POINTER(C.c_int32)]),
     "mz_gated_ff_fwd": (C.c_int, [_P, C.c_int64] + [_P] * 4 + [C.c_int64] * 3 + [C.c_int32] * 2 + [_P, _P, C.c_int64, _P]),
     "mz_gated_ff_bwd": (C.c_int, [_P, C.c_int64] + [_P] * 5 + [C.c_int64] * 3 + [C.c_int32] * 2 + [_P] * 6 + [C.c_int64, _P]),
     "mz_dropout": (C.c_int, [_P, _P, _P, C.c_int64, C.c_double, _P, C.c_uint32, C.c_int32, _P]),

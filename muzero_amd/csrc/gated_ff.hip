@@ -309,6 +309,22 @@ int64_t mz_gated_ff_workspace_bytes(int64_t M, int64_t K, int64_t F, int32_t dty
   return plan_backward(make_shape(M, K, F, dtype)).bytes();
 }
 
+int mz_gated_ff_plan(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t want_dx, int32_t want_dw, int32_t* plan) {
+  MZ_REQUIRE(plan, "mz_gated_ff_plan: null plan");
+  if (int rc = check_shape("mz_gated_ff_plan", M, K, F, dtype, 0)) return rc;
+  const Shape sh = make_shape(M, K, F, dtype);
+  const Backward b = plan_backward(sh);
+  plan[0] = M <= kFew ? 0 : mz_gff::tile_side(pick(F, M, sh.steps(sh.nk_K()), dtype, mz_gff::kForward).tile);
+  plan[1] = mz_gff::tile_side(b.gate_tile);
+  plan[2] = want_dx ? mz_gff::tile_side(b.dx.tile) : 0;
+  plan[3] = want_dx ? b.dx.splits : 0;
+  plan[4] = want_dw ? mz_gff::tile_side(b.dw.tile) : 0;
+  plan[5] = want_dw ? b.dw.splits : 0;
+  plan[6] = b.both && want_dx && want_dw;
+  plan[7] = b.parts;
+  return MZ_OK;
+}
+
 int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* w_up, const void* b_gate, const void* b_up,
                     int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t activation, void* h, void* workspace,
                     int64_t workspace_bytes, mz_stream_t stream) {
