@@ -55,7 +55,8 @@ def gated_ff(x, w_gate, w_up, b_gate: Optional[torch.Tensor] = None, b_up: Optio
     ``torch.autocast`` they are cast to its dtype first, as torch's linear does).  activation: "silu", "gelu" (erf),
     "relu" or "sigmoid".  Returns [..., F].  The backward pass computes the two products again from x: nothing of the
     hidden width is kept but the result; while it runs it takes scratch of twice the result's size and for the partial
-    results of sums that are cut over workgroups.  In bfloat16 and float16 it rounds the two products' gradients to that
+    results of sums that are cut over workgroups.  How they are cut goes by the sizes and by whether x and the weights both want
+    gradients: the last bits of one that is asked for alone may differ from those it has beside the other.  In bfloat16 and float16 it rounds the two products' gradients to that
     type, matrix operands as they are next: gradients of x and the weights are then off by sqrt(2) times what rounding the
     result alone costs (relative RMS 2.4e-3 in bfloat16, 2.9e-4 in float16), at any size.  Small problems - rows x F up to
     8192 and K x F up to 2^21 - carry what that rounding left along and are off by the result's rounding alone.

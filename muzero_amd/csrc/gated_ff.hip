@@ -15,6 +15,8 @@
 // the same bits on every run.
 #include "gated_ff.h"
 
+#include <algorithm>
+
 namespace {
 
 using mz_gff::Args;
@@ -159,21 +161,25 @@ template <typename Fn> void for_cuts(int64_t nr, int64_t nc, int64_t steps, int 
   }
 }
 
+// the estimated time of `elements` results in the tiles and the cut of s, in a launch of their own
+float time_alone(const Split& s, int64_t elements, int dtype, int mode) {
+  const TileCost& c = cost_of(dtype, s.tile);
+  const int64_t share = (s.groups + kCus - 1) / kCus, rounds = share / c.at_once, rest = share % c.at_once;
+  auto round = [&](int64_t n) {
+    const float step = c.shared * n > c.alone ? c.shared * n : c.alone;
+    return s.steps * step + c.ends[mode < 2 ? mode : 2];
+  };
+  return rounds * round(c.at_once) + (rest ? round(rest) : 0.f) + (s.splits > 1 ? 3.f + join_time(elements, s.splits) : 0.f);
+}
+
 Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only = -1) {
   const bool pair = mode <= mz_gff::kGateGrad;
   const int problems = mode == mz_gff::kWeightGrad ? 2 : 1;
   Split best = {2, 1, (int)steps, -1.f, 0};
   for (int t = dtype == MZ_F32 ? 1 : 0; t < 3; ++t) {
     if (only >= 0 && t != only) continue;
-    const TileCost& c = cost_of(dtype, t);
     for_cuts(nr, nc, steps, t, problems, pair, [&](Split s) {
-      const int64_t share = (s.groups + kCus - 1) / kCus, rounds = share / c.at_once, rest = share % c.at_once;
-      auto round = [&](int64_t n) {
-        const float step = c.shared * n > c.alone ? c.shared * n : c.alone;
-        return s.steps * step + c.ends[mode < 2 ? mode : 2];
-      };
-      s.time = rounds * round(c.at_once) + (rest ? round(rest) : 0.f);
-      if (s.splits > 1) s.time += 3.f + join_time(nr * nc * problems, s.splits);
+      s.time = time_alone(s, nr * nc * problems, dtype, mode);
       if (best.time < 0.f || s.time < best.time) best = s;
     });
   }
@@ -186,7 +192,8 @@ Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only 
 // Fitted to 62 backward passes of all sizes with 40 to 126 pairs of cuts each: what this and pick() choose - separate
 // launches, which alone have the largest tiles, where that is estimated faster - is within 3 % of the best on average, one
 // launch only where a single round holds both within 6 % (18432 x 256 x 1024 bf16: 71 us then, 48 now; 3000 x 3000 x 100:
-// 32, 19).
+// 32, 19).  The worst that the choice was seen to lose: 4553 x 1505 x 218 float32, backward 193 us, with dw cut in 12 parts and
+// not in 6 179.
 float time_together(const TileCost& c, const Split& x, const Split& w) {
   const int64_t n = x.groups + w.groups, most = (n + kCus - 1) / kCus, x_most = (x.groups + kCus - 1) / kCus;
   const float at_once = (float)c.at_once, held = n <= kCus ? 1.f : n >= kCus * c.at_once ? at_once : (float)n / kCus;
@@ -228,13 +235,16 @@ Shape make_shape(int64_t M, int64_t K, int64_t F, int dtype) {
 constexpr int64_t kFew = 16;
 
 struct Backward {
-  Split dx, dw;
+  Split dx, dw;              // asked for together
+  Split dx_only, dw_only;    // one without the other
   int parts;                 // of dg and du (Args::parts)
   bool both;                 // the two products in one launch, in the same tiles
   int gate_tile;
-  int64_t dgu_bytes, col_bytes, dx_bytes, dw_bytes;
-  int64_t bytes() const { return 2 * parts * dgu_bytes + col_bytes + dx_bytes + dw_bytes; }
+  int64_t dgu_bytes, col_bytes, partial_bytes;     // partial results of cut sums: dx's and then dw's
+  int64_t bytes() const { return 2 * parts * dgu_bytes + col_bytes + partial_bytes; }
 };
+int64_t partial_bytes(const Split& s, int64_t elements) { return s.splits > 1 ? round_up(s.splits * elements * 4, 256) : 0; }
+
 Backward make_plan(const Shape& h) {
   Backward b;
   // Second parts of dg and du in the 16-bit types (above) where they cost 0 to 4 us: kernels of the backward pass without / with them
@@ -245,10 +255,13 @@ Backward make_plan(const Shape& h) {
   const int only = b.parts == 2 ? 2 : -1;          // in the smallest tiles
   b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad, only).tile;
   const int64_t fs = 2 * b.parts * h.steps(h.nk_F()), ms = b.parts * h.steps(h.nk_M());
-  b.dx = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, only);
-  b.dw = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, only);
+  b.dx = b.dx_only = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, only);
+  b.dw = b.dw_only = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, only);
   b.both = false;
   float least = b.dx.time + b.dw.time + 9.f;       // and a launch more
+  // Against launches in the largest tiles, which a shared one does not have, it has to win by more than the estimate is off by
+  // (46984 x 2394 x 166 bf16: estimated 0.96 of the separate launches' time, measured 1.08).
+  if (b.dx.tile == 0 || b.dw.tile == 0) least *= .94f;
   for (int t = b.parts; t < 3; ++t)                // parts: the smallest tiles only; the largest has no kernel of both
     for_cuts(h.K, h.M, fs, t, 1, false, [&](const Split& x) {
       for_cuts(h.K, h.F, ms, t, 2, false, [&](const Split& w) {
@@ -260,11 +273,20 @@ Backward make_plan(const Shape& h) {
         b.dw = w;
       });
     });
+  // A gradient that is asked for without the other (frozen weights, an input without a gradient) has the cut that it has with
+  // it, and so the same bits, unless its own is estimated clearly faster (46984 x 2394 x 166 bf16, dw: 110 us, cut for the shared
+  // launch 180; 7517 x 3248 x 209 float32, dw: 218, 317; 18432 x 256 x 1024 float32, dx: 171, 254).
+  const auto clearly = [&](const Split& own, const Split& joint, int64_t elements, int mode) {
+    const float t = time_alone(joint, elements, h.dtype, mode);
+    return own.time < .9f * t && own.time < t - 4.f;           // by more than a launch
+  };
+  if (!clearly(b.dx_only, b.dx, h.M * h.K, mz_gff::kInputGrad)) b.dx_only = b.dx;
+  if (!clearly(b.dw_only, b.dw, 2 * h.F * h.K, mz_gff::kWeightGrad)) b.dw_only = b.dw;
   b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
   const int side = mz_gff::tile_side(b.gate_tile);
   b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
-  b.dx_bytes = b.dx.splits > 1 ? round_up(b.dx.splits * h.M * h.K * 4, 256) : 0;
-  b.dw_bytes = b.dw.splits > 1 ? round_up(b.dw.splits * 2 * h.F * h.K * 4, 256) : 0;
+  const int64_t only_bytes = std::max(partial_bytes(b.dx_only, h.M * h.K), partial_bytes(b.dw_only, 2 * h.F * h.K));
+  b.partial_bytes = std::max(partial_bytes(b.dx, h.M * h.K) + partial_bytes(b.dw, 2 * h.F * h.K), only_bytes);
   return b;
 }
 
@@ -316,10 +338,11 @@ int mz_gated_ff_plan(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t wan
   const Backward b = plan_backward(sh);
   plan[0] = M <= kFew ? 0 : mz_gff::tile_side(pick(F, M, sh.steps(sh.nk_K()), dtype, mz_gff::kForward).tile);
   plan[1] = mz_gff::tile_side(b.gate_tile);
-  plan[2] = want_dx ? mz_gff::tile_side(b.dx.tile) : 0;
-  plan[3] = want_dx ? b.dx.splits : 0;
-  plan[4] = want_dw ? mz_gff::tile_side(b.dw.tile) : 0;
-  plan[5] = want_dw ? b.dw.splits : 0;
+  const Split &dx = want_dw ? b.dx : b.dx_only, &dw = want_dx ? b.dw : b.dw_only;
+  plan[2] = want_dx ? mz_gff::tile_side(dx.tile) : 0;
+  plan[3] = want_dx ? dx.splits : 0;
+  plan[4] = want_dw ? mz_gff::tile_side(dw.tile) : 0;
+  plan[5] = want_dw ? dw.splits : 0;
   plan[6] = b.both && want_dx && want_dw;
   plan[7] = b.parts;
   return MZ_OK;
@@ -391,6 +414,7 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   a.splits = 1;
   a.steps_per_split = (int)sh.steps(a.nk);
   if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
+  const Split &cut_x = dw_gate ? plan.dx : plan.dx_only, &cut_w = dx ? plan.dw : plan.dw_only;
   Args p = {}, q = {};                             // dx; dw
   p.r[0] = w_gate; p.r[1] = w_up;
   p.c[0] = dg; p.c[1] = du; p.c[2] = a.out[2]; p.c[3] = a.out[3];
@@ -399,23 +423,22 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   p.nr = K; p.nc = M; p.nk = sh.nk_F(); p.nk_all = F;
   p.out[0] = p.out[1] = dx; p.ldo = K;
   p.partial = reinterpret_cast<float*>(partial);
-  p.splits = plan.dx.splits; p.steps_per_split = plan.dx.steps;
+  p.splits = cut_x.splits; p.steps_per_split = cut_x.steps;
   q.r[0] = q.r[1] = x;
   q.c[0] = dg; q.c[1] = du; q.c[2] = a.out[2]; q.c[3] = a.out[3];
   q.parts = plan.parts;
   q.ldr = ldx; q.ldc = sh.Fp;
   q.nr = K; q.nc = F; q.nk = sh.nk_M(); q.nk_all = M;
   q.out[0] = dw_gate; q.out[1] = dw_up; q.ldo = K;
-  q.partial = reinterpret_cast<float*>(partial + plan.dx_bytes);
-  q.splits = plan.dw.splits; q.steps_per_split = plan.dw.steps;
-  // a gradient asked for alone has the cut it has with the others: the same bits
+  q.partial = reinterpret_cast<float*>(partial + (dx ? partial_bytes(cut_x, M * K) : 0));
+  q.splits = cut_w.splits; q.steps_per_split = cut_w.steps;
   if (plan.both && dx && dw_gate) {
     if (int rc = launch_both(p, q, dtype, plan.dx.tile, s)) return rc;
   } else {
     if (dx)
-      if (int rc = launch(p, dtype, mz_gff::kInputGrad, plan.dx.tile, s)) return rc;
+      if (int rc = launch(p, dtype, mz_gff::kInputGrad, cut_x.tile, s)) return rc;
     if (dw_gate)
-      if (int rc = launch(q, dtype, mz_gff::kWeightGrad, plan.dw.tile, s)) return rc;
+      if (int rc = launch(q, dtype, mz_gff::kWeightGrad, cut_w.tile, s)) return rc;
   }
   Finish f = {};
   if (dx && p.splits > 1) f.join[0] = make_join(p, 1);

@@ -67,6 +67,33 @@ def test_the_cases_cover_every_tile():
     assert plan_of(16, 64, 64, "bf16")["forward"] == 0 and plan_of(17, 64, 64, "bf16")["forward"] == 64
 
 
+# gradients that are wanted without the other, at sizes where the cut for a launch of both is a bad one for that
+ALONE = [
+    (46983, 2393, 165, "bf16", "dw", dict(dw=256)), (18431, 255, 1023, "bf16", "dw", dict(dw=128)),
+    (7517, 3247, 209, "f32", "dw", dict(dw=64)), (6179, 3937, 77, "f32", "dw", dict(dw=64)),
+    (18431, 255, 1023, "f32", "dx", dict(dx=64)), (65535, 1023, 31, "f16", "dw", dict(dw=64)),
+    (65535, 1023, 31, "f16", "dx", dict(dx=256)),
+]
+
+
+@pytest.mark.parametrize("rows,k,f,t,which,want", ALONE)
+def test_a_gradient_alone_has_its_own_plan(rows, k, f, t, which, want):
+    joint, alone = plan_of(rows, k, f, t), plan_of(rows, k, f, t, int(which == "dx"), int(which == "dw"))
+    assert alone["together"] == 0 and {n: alone[n] for n in want} == want, alone
+    assert (alone[which], alone[which + "_parts"]) != (joint[which], joint[which + "_parts"]) or joint["together"] == 0
+
+
+def test_a_gradient_alone_has_the_joint_cut_where_little_is_gained():
+    for rows, k, f, t in ((90, 64, 72, "bf16"), (90, 64, 72, "f32"), (300, 300, 300, "bf16"), (128, 256, 1024, "bf16")):
+        joint, dx, dw = plan_of(rows, k, f, t), plan_of(rows, k, f, t, 1, 0), plan_of(rows, k, f, t, 0, 1)
+        assert (dx["dx"], dx["dx_parts"], dw["dw"], dw["dw_parts"]) == (joint["dx"], joint["dx_parts"], joint["dw"], joint["dw_parts"])
+
+
+def test_shared_launches_have_to_win_clearly_against_the_largest_tiles():
+    for rows, k, f, together in ((46984, 2394, 166, 0), (4096, 1024, 4096, 0), (50344, 285, 473, 1), (500, 2000, 8000, 1)):
+        assert plan_of(rows, k, f, "bf16")["together"] == together
+
+
 def test_plan_refuses():
     from muzero_amd import _lib
     p = (C.c_int32 * 8)()
@@ -121,3 +148,25 @@ def test_larger_tiles_strides_and_bad_values(rows, k, f, t):
     got = ff_run(x, wg, wu, bg, bu, dh, "silu")
     for i in (0, 1):
         assert torch.isnan(got[i][-1]).all() and torch.equal(got[i][:-1], good[i][:-1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,f,t,which,want", ALONE)
+def test_a_gradient_alone_against_float64(rows, k, f, t, which, want):
+    """Frozen weights, or an input without a gradient; the workspace between canaries."""
+    from muzero_amd import _lib, blocks
+    x, wg, wu, bg, bu, dh = ff_inputs(rows, rows, k, f, TYPES[t])
+    leaves = [v.detach().requires_grad_(v is x if which == "dx" else v is wg or v is wu) for v in (x, wg, wu, bg, bu)]
+    h = blocks.gated_ff(*leaves)
+    grads = torch.autograd.grad(h, [v for v in leaves if v.requires_grad], dh)
+    parts = [grads[0], None, None] if which == "dx" else [None, grads[0], grads[1]]
+    check_gated_ff(x, wg, wu, bg, bu, dh, "silu", [h.detach()] + parts + [None, None])
+    p, s = (lambda v: v.data_ptr()), _lib.current_stream()
+    need = _lib.lib().mz_gated_ff_workspace_bytes(rows, k, f, MZ[t], 1)
+    ws, out = Canary((need + 3) // 4, torch.float32), [Canary(v.numel(), TYPES[t]) for v in grads]
+    args = (out[0].ptr(), None, None) if which == "dx" else (None, out[0].ptr(), out[1].ptr())
+    _lib.call("mz_gated_ff_bwd", p(x), k, p(wg), p(wu), p(bg), p(bu), p(dh), rows, k, f, MZ[t], 0, *args, None, None, ws.ptr(), need, s)
+    assert (ws.all[:512] == 7.0).all() and (ws.all[-512:] == 7.0).all()
+    for c, v in zip(out, grads):
+        c.check(which)
+        assert torch.equal(c.inner, v.reshape(-1))
