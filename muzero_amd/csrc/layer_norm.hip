@@ -24,10 +24,22 @@
 // wide rows' parameters alone want gradients a pass over x (2000 x 32768: 53 us without, 92).
 #include "block_common.h"
 
+#include <algorithm>
+
 namespace {
 
 constexpr int kMaxRegisterCols = 16384;     // 1024 threads x 16 columns; wider rows take the looping kernels
-constexpr int kMaxPartials = 1024;
+constexpr int kMaxWorkgroupCols = 4096;     // wider rows have 512 threads or more
+// Most workgroups that leave partial sums of C columns, of whichever type: of up to 256 threads, of more (one a compute unit), and
+// down the rows of the column sums of wide rows (256 threads of eight columns, four workgroups a compute unit in all).  An MI355X's
+// compute units, so that a workspace's size is the same everywhere.
+constexpr int kCus = 256;
+constexpr int max_partials(int C) {
+  if (C <= kMaxWorkgroupCols) return 4 * kCus;
+  if (C <= kMaxRegisterCols) return kCus;
+  const int across = (C + 2047) / 2048;
+  return (4 * kCus + across - 1) / across;
+}
 
 struct LnArgs {
   const void* x;
@@ -458,12 +470,12 @@ int row_blocks(long rows, int rows_per_block, int cap) {
 // Workgroups of the backward pass.  Each leaves 8 C bytes of partial sums that are written and read once more, so it
 // should walk at least eight rows (at 2000 x 8192 bf16: 34 us, with four rows 45 us), as long as every compute unit
 // has one (500 x 2048: 10.5 us with one each, 12.4 with one in four).
-int bwd_blocks(long rows, int rows_per_block, int threads) {
+int bwd_blocks(long rows, int rows_per_block, int threads, int C) {
   const int cus = mz::compute_units();
   long cap = threads >= 512 ? cus : 3 * cus;
   const long few = rows / 8 > cus ? rows / 8 : cus;
   if (cap > few) cap = few;
-  if (cap > kMaxPartials) cap = kMaxPartials;
+  if (cap > max_partials(C)) cap = max_partials(C);
   return row_blocks(rows, rows_per_block, (int)cap);
 }
 
@@ -489,7 +501,7 @@ template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hi
       constexpr int kCols = 256 * Vec16<T>::N;
       const int bx = (a.C + kCols - 1) / kCols;
       int by = (4 * mz::compute_units() + bx - 1) / bx;
-      by = row_blocks(a.rows, 1, by < kMaxPartials ? by : kMaxPartials);
+      by = row_blocks(a.rows, 1, by < max_partials(a.C) ? by : max_partials(a.C));
       blocks = by;
       hipLaunchKernelGGL((ln_bwd_wide_cols_kernel<T>), dim3(bx, by), dim3(256), 0, s, a);
     }
@@ -498,7 +510,7 @@ template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hi
       // the widest float32 rows on half the threads with twice the registers: 1024 threads spill (4000 x 16384: 230 us)
       constexpr bool kHalve = decltype(tpr)::value == 1024 && sizeof(T) == 4;
       constexpr int TPR = kHalve ? 512 : decltype(tpr)::value, NV = kHalve ? 8 : decltype(nv)::value, NT = block_threads<TPR>();
-      blocks = bwd_blocks(a.rows, NT / TPR, NT);
+      blocks = bwd_blocks(a.rows, NT / TPR, NT, a.C);
       hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV>), dim3(blocks), dim3(NT), 0, s, a);
       return MZ_OK;
     });
@@ -509,7 +521,7 @@ template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hi
   return MZ_OK;
 }
 
-int64_t partial_floats(int64_t rows, int32_t C) { return (rows < kMaxPartials ? rows : kMaxPartials) * 2 * (int64_t)C; }
+int64_t partial_floats(int64_t rows, int32_t C) { return std::min<int64_t>(rows, max_partials(C)) * 2 * C; }
 
 int check(const char* who, int64_t rows, int32_t C, int64_t ld, int32_t dtype, int32_t affine_dtype) {
   MZ_REQUIRE(rows > 0 && C > 0 && C <= (1 << 24), "%s: rows > 0 and 0 < C <= 2^24 expected (rows = %lld, C = %d)", who,

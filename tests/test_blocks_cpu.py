@@ -97,3 +97,13 @@ def test_sizes_that_cannot_be_numbered_and_float_alignment():
     _fails("mz_gated_ff_fwd", ONE, 64, ONE, ONE, None, None, 1 << 37, 64, 32, 1, 0, ONE, None, 0, None, match="out of range")
     _fails("mz_layer_norm_bwd", ONE, 8, ONE, 8, None, 0, ONE, ONE, 4, 8, 0, ONE, ONE, None, C.c_void_p(18), 1 << 20, None,
            match="aligned")
+
+
+def test_layer_norm_workspace_is_what_the_launch_uses():
+    """Partial rows of the workgroups that there can be, and a float a row where rows are wider than 16384 columns."""
+    need = _lib.lib().mz_layer_norm_workspace_bytes
+    assert need(1 << 20, 4096) == 1024 * 2 * 4096 * 4 and need(1 << 20, 4097) == 256 * 2 * 4097 * 4
+    assert need(1 << 20, 16384) == 256 * 2 * 16384 * 4 and need(100, 16384) == 100 * 2 * 16384 * 4
+    assert need(65536, 65536) == 32 * 2 * 65536 * 4 + 65536 * 4                 # not 537 MB
+    assert need(1024, 1 << 24) == 1 * 2 * (1 << 24) * 4 + 1024 * 4              # not 137 GB
+    assert need(3, 20000) == 3 * 2 * 20000 * 4 + 3 * 4

@@ -119,6 +119,33 @@ def test_rows_whose_squares_overflow_and_bad_rows():
         assert torch.equal(y[0], good[0]) and torch.equal(y[1], b) and torch.isnan(y[2]).all() and torch.isnan(y[3]).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows,c", [(9000, 7), (5000, 300), (3000, 1001), (1500, 4096), (1500, 4097), (700, 9001), (600, 16384),
+                                    (700, 20001), (300, 65537), (3, 70000)])
+def test_layer_norm_stays_inside_its_workspace(rows, c, t):
+    """The workspace asked for between canaries and full of NaN, dx wanted and not: the bits of the Python entry point."""
+    from muzero_amd import _lib, blocks
+    from tests.test_blocks_gpu import Canary
+    g, t = gen(rows + c), TYPES[t]
+    x, dy = normal(g, rows, c, t=t), normal(g, rows, c, t=t)
+    w, b = normal(g, c, mean=1.0).requires_grad_(), normal(g, c).requires_grad_()
+    leaf = x.detach().requires_grad_()
+    dx, dw, db = torch.autograd.grad(blocks.layer_norm(leaf, w, b), (leaf, w, b), dy)
+    p, s = (lambda v: v.data_ptr()), _lib.current_stream()
+    dt = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[t]
+    need = _lib.lib().mz_layer_norm_workspace_bytes(rows, c)
+    for with_dx in (True, False):
+        y, stats, ws = Canary(rows * c, t), Canary(2 * rows, torch.float32), Canary(need // 4, torch.float32)
+        out = [Canary(rows * c, t), Canary(c, torch.float32), Canary(c, torch.float32)]
+        _lib.call("mz_layer_norm_fwd", p(x), c, p(w), p(b), 0, 1e-5, rows, c, dt, y.ptr(), stats.ptr(), stats.ptr() + 4 * rows, s)
+        _lib.call("mz_layer_norm_bwd", p(x), c, p(dy), c, p(w), 0, stats.ptr(), stats.ptr() + 4 * rows, rows, c, dt,
+                  out[0].ptr() if with_dx else None, out[1].ptr(), out[2].ptr(), ws.ptr(), need, s)
+        assert (ws.all[:512] == 7.0).all() and (ws.all[-512:] == 7.0).all()
+        for canary, want in zip(out[1 - with_dx:], (dx, dw, db)[1 - with_dx:]):
+            canary.check("layer_norm")
+            assert torch.equal(canary.inner, want.reshape(-1))
+
+
 # ------------------------------------------------------------------------------------------- gated feed-forward
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("rows", [9, 64, 300])
