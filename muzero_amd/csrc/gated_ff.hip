@@ -316,7 +316,7 @@ int check_shape(const char* who, int64_t M, int64_t K, int64_t F, int32_t dtype,
   return MZ_OK;
 }
 int check_stride(const char* who, const Shape& h, int64_t ldx) {
-  MZ_REQUIRE(ldx >= h.K && ldx * elem_bytes(h.dtype) <= (1 << 22),
+  MZ_REQUIRE(ldx >= h.K && ldx <= (1 << 22) / elem_bytes(h.dtype),
              "%s: stride of x out of range (%lld, K = %lld; rows up to 4 MiB apart)", who, (long long)ldx, (long long)h.K);
   return MZ_OK;
 }

@@ -523,10 +523,17 @@ template <typename T> int ln_bwd(const LnArgs& a, void* dweight, void* dbias, hi
 
 int64_t partial_floats(int64_t rows, int32_t C) { return std::min<int64_t>(rows, max_partials(C)) * 2 * C; }
 
+int check_rows(const char* who, int64_t rows, int32_t C, int64_t ld) {
+  MZ_REQUIRE(ld >= C || rows == 1, "%s: rows overlap (stride %lld < C = %d)", who, (long long)ld, C);
+  MZ_REQUIRE(rows == 1 || ld <= (1ll << 48) / rows, "%s: %lld rows %lld elements apart lie past any memory", who, (long long)rows,
+             (long long)ld);
+  return MZ_OK;
+}
+
 int check(const char* who, int64_t rows, int32_t C, int64_t ld, int32_t dtype, int32_t affine_dtype) {
   MZ_REQUIRE(rows > 0 && C > 0 && C <= (1 << 24), "%s: rows > 0 and 0 < C <= 2^24 expected (rows = %lld, C = %d)", who,
              (long long)rows, C);
-  MZ_REQUIRE(ld >= C || rows == 1, "%s: rows overlap (stride %lld < C = %d)", who, (long long)ld, C);
+  if (int rc = check_rows(who, rows, C, ld)) return rc;
   MZ_REQUIRE(dtype == MZ_F32 || dtype == MZ_BF16 || dtype == MZ_F16, "%s: unknown element type %d", who, dtype);
   MZ_REQUIRE(affine_dtype == MZ_F32 || affine_dtype == dtype, "%s: parameters are float32 or of the activations' type", who);
   return MZ_OK;
@@ -561,7 +568,7 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
   MZ_REQUIRE(x && dy && mean && rstd, "mz_layer_norm_bwd: null tensor");
   MZ_REQUIRE(dx || dweight || dbias, "mz_layer_norm_bwd: no gradient asked for");
   if (int rc = check("mz_layer_norm_bwd", rows, C, ldx, dtype, affine_dtype)) return rc;
-  MZ_REQUIRE(lddy >= C || rows == 1, "mz_layer_norm_bwd: rows of dy overlap (stride %lld < C = %d)", (long long)lddy, C);
+  if (int rc = check_rows("mz_layer_norm_bwd: dy", rows, C, lddy)) return rc;
   const bool params = dweight || dbias;
   MZ_REQUIRE(!params || (workspace && workspace_bytes >= mz_layer_norm_workspace_bytes(rows, C) && (size_t)workspace % 4 == 0),
              "mz_layer_norm_bwd: workspace too small or not aligned to float");

@@ -107,3 +107,16 @@ def test_layer_norm_workspace_is_what_the_launch_uses():
     assert need(65536, 65536) == 32 * 2 * 65536 * 4 + 65536 * 4                 # not 537 MB
     assert need(1024, 1 << 24) == 1 * 2 * (1 << 24) * 4 + 1024 * 4              # not 137 GB
     assert need(3, 20000) == 3 * 2 * 20000 * 4 + 3 * 4
+
+
+def test_strides_whose_bytes_pass_64_bits():
+    """A stride of 2^62 elements is 2^64 or 2^63 bytes: out of range, not 0."""
+    for ld in (1 << 62, (1 << 48) // 4 + 1):
+        _fails("mz_layer_norm_fwd", ONE, ld, None, None, 0, 1e-5, 4, 8, 0, ONE, None, None, None, match="apart")
+        _fails("mz_layer_norm_bwd", ONE, 8, ONE, ld, None, 0, ONE, ONE, 4, 8, 0, ONE, None, None, None, 0, None, match="apart")
+    _fails("mz_layer_norm_fwd", ONE, 8, None, None, 0, 1e-5, 1 << 60, 8, 0, ONE, None, None, None, match="apart")
+    for ldx in (1 << 62, 1 << 61, (1 << 63) - 1, (1 << 62) + 64, (1 << 61) + 64):
+        for dt in (0, 1, 2):
+            _fails("mz_gated_ff_fwd", ONE, ldx, ONE, ONE, None, None, 100, 64, 32, dt, 0, ONE, None, 0, None, match="stride")
+            _fails("mz_gated_ff_bwd", ONE, ldx, ONE, ONE, None, None, ONE, 100, 64, 32, dt, 0, ONE, None, None, None, None, None, 1 << 30,
+                   None, match="stride")
