@@ -150,6 +150,10 @@ constexpr int kMaxSplits = 32, kCus = 256;         // of an MI355X: the choice, 
 const TileCost& cost_of(int dtype, int tile) { return (dtype == MZ_F32 ? kCost32 : kCost16)[tile]; }
 float join_time(int64_t elements, int splits) { return splits > 1 ? (float)elements * splits * 8.f / 8e6f : 0.f; }
 
+// Workgroups that a launch can have: HIP counts its threads in 32 bits (16 less, for rounding up to all XCDs).  The pair products'
+// workgroups in the smaller tiles are as many as the chip holds, what counts there is the numbering of the tiles (gemm_blocks).
+int64_t max_groups(int tile, bool pair) { return pair && tile != 0 ? 0x3ffffff0ll : (1ll << 32) / (tile == 0 ? 512 : 256) - 16; }
+
 // f(the product of nr x nc results, `problems` of them, in `tile` with its sum cut into 1, 2, 3 .. parts)
 template <typename Fn> void for_cuts(int64_t nr, int64_t nc, int64_t steps, int tile, int problems, bool pair, Fn&& f) {
   const int side = mz_gff::tile_side(tile);
@@ -157,6 +161,7 @@ template <typename Fn> void for_cuts(int64_t nr, int64_t nc, int64_t steps, int 
   for (int want = 1; want <= (pair ? 1 : kMaxSplits); want += want < 4 ? 1 : want < 8 ? 2 : want < 16 ? 4 : 8) {
     if (want > 1 && want > steps / 2) break;
     const int64_t per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+    if (whole * splits > max_groups(tile, pair)) break;
     f(Split{tile, (int)splits, (int)per, 0.f, whole * splits});
   }
 }
@@ -175,7 +180,7 @@ float time_alone(const Split& s, int64_t elements, int dtype, int mode) {
 Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only = -1) {
   const bool pair = mode <= mz_gff::kGateGrad;
   const int problems = mode == mz_gff::kWeightGrad ? 2 : 1;
-  Split best = {2, 1, (int)steps, -1.f, 0};
+  Split best = {2, 1, (int)steps, -1.f, 0};        // stays where no tile is large enough: refused before anything is launched
   for (int t = dtype == MZ_F32 ? 1 : 0; t < 3; ++t) {
     if (only >= 0 && t != only) continue;
     for_cuts(nr, nc, steps, t, problems, pair, [&](Split s) {
@@ -183,6 +188,7 @@ Split pick(int64_t nr, int64_t nc, int64_t steps, int dtype, int mode, int only 
       if (best.time < 0.f || s.time < best.time) best = s;
     });
   }
+  if (best.time < 0.f) best.time = 1e30f;
   return best;
 }
 
@@ -253,7 +259,8 @@ Backward make_plan(const Shape& h) {
   // 22.7 / 34.2, and the weights' second reading 1 x 4096 x 8192 77.8 / 127.4.
   b.parts = h.dtype != MZ_F32 && h.M * h.F <= 8192 && h.K * h.F <= 1 << 21 ? 2 : 1;
   const int only = b.parts == 2 ? 2 : -1;          // in the smallest tiles
-  b.gate_tile = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad, only).tile;
+  const Split gate = pick(h.F, h.M, h.steps(h.nk_K()), h.dtype, mz_gff::kGateGrad, only);
+  b.gate_tile = gate.groups ? gate.tile : -1;
   const int64_t fs = 2 * b.parts * h.steps(h.nk_F()), ms = b.parts * h.steps(h.nk_M());
   b.dx = b.dx_only = pick(h.K, h.M, fs, h.dtype, mz_gff::kInputGrad, only);
   b.dw = b.dw_only = pick(h.K, h.F, ms, h.dtype, mz_gff::kWeightGrad, only);
@@ -265,6 +272,7 @@ Backward make_plan(const Shape& h) {
   for (int t = b.parts; t < 3; ++t)                // parts: the smallest tiles only; the largest has no kernel of both
     for_cuts(h.K, h.M, fs, t, 1, false, [&](const Split& x) {
       for_cuts(h.K, h.F, ms, t, 2, false, [&](const Split& w) {
+        if (x.groups + w.groups > max_groups(t, false)) return;
         const float time = time_together(cost_of(h.dtype, t), x, w) + join_time(h.M * h.K, x.splits) + join_time(2 * h.F * h.K, w.splits);
         if (time >= least) return;
         b.both = true;
@@ -283,7 +291,7 @@ Backward make_plan(const Shape& h) {
   if (!clearly(b.dx_only, b.dx, h.M * h.K, mz_gff::kInputGrad)) b.dx_only = b.dx;
   if (!clearly(b.dw_only, b.dw, 2 * h.F * h.K, mz_gff::kWeightGrad)) b.dw_only = b.dw;
   b.dgu_bytes = round_up(h.M * h.Fp * elem_bytes(h.dtype), 256);
-  const int side = mz_gff::tile_side(b.gate_tile);
+  const int side = mz_gff::tile_side(b.gate_tile < 0 ? 2 : b.gate_tile);
   b.col_bytes = round_up((h.M + side - 1) / side * 2 * h.F * 4, 256);
   const int64_t only_bytes = std::max(partial_bytes(b.dx_only, h.M * h.K), partial_bytes(b.dw_only, 2 * h.F * h.K));
   b.partial_bytes = std::max(partial_bytes(b.dx, h.M * h.K) + partial_bytes(b.dw, 2 * h.F * h.K), only_bytes);
@@ -315,6 +323,10 @@ int check_shape(const char* who, int64_t M, int64_t K, int64_t F, int32_t dtype,
   MZ_REQUIRE(activation >= 0 && activation <= mz_gff::kSigmoid, "%s: unknown activation %d", who, activation);
   return MZ_OK;
 }
+int check_tiles(const char* who, bool fits) {
+  MZ_REQUIRE(fits, "%s: too many output tiles for a launch", who);
+  return MZ_OK;
+}
 int check_stride(const char* who, const Shape& h, int64_t ldx) {
   MZ_REQUIRE(ldx >= h.K && ldx <= (1 << 22) / elem_bytes(h.dtype),
              "%s: stride of x out of range (%lld, K = %lld; rows up to 4 MiB apart)", who, (long long)ldx, (long long)h.K);
@@ -336,9 +348,11 @@ int mz_gated_ff_plan(int64_t M, int64_t K, int64_t F, int32_t dtype, int32_t wan
   if (int rc = check_shape("mz_gated_ff_plan", M, K, F, dtype, 0)) return rc;
   const Shape sh = make_shape(M, K, F, dtype);
   const Backward b = plan_backward(sh);
-  plan[0] = M <= kFew ? 0 : mz_gff::tile_side(pick(F, M, sh.steps(sh.nk_K()), dtype, mz_gff::kForward).tile);
-  plan[1] = mz_gff::tile_side(b.gate_tile);
+  const Split fwd = pick(F, M, sh.steps(sh.nk_K()), dtype, mz_gff::kForward);
   const Split &dx = want_dw ? b.dx : b.dx_only, &dw = want_dx ? b.dw : b.dw_only;
+  if (int rc = check_tiles("mz_gated_ff_plan", fwd.groups && b.gate_tile >= 0 && (!want_dx || dx.groups) && (!want_dw || dw.groups))) return rc;
+  plan[0] = M <= kFew ? 0 : mz_gff::tile_side(fwd.tile);
+  plan[1] = mz_gff::tile_side(b.gate_tile);
   plan[2] = want_dx ? mz_gff::tile_side(dx.tile) : 0;
   plan[3] = want_dx ? dx.splits : 0;
   plan[4] = want_dw ? mz_gff::tile_side(dw.tile) : 0;
@@ -371,7 +385,9 @@ int mz_gated_ff_fwd(const void* x, int64_t ldx, const void* w_gate, const void* 
     return mz::check_launch("mz_gated_ff_fwd");
   }
   a.steps_per_split = (int)sh.steps(a.nk);
-  if (int rc = launch(a, dtype, mz_gff::kForward, pick(F, M, sh.steps(a.nk), dtype, mz_gff::kForward).tile, s)) return rc;
+  const Split cut = pick(F, M, sh.steps(a.nk), dtype, mz_gff::kForward);
+  if (int rc = check_tiles("mz_gated_ff_fwd", cut.groups > 0)) return rc;
+  if (int rc = launch(a, dtype, mz_gff::kForward, cut.tile, s)) return rc;
   return mz::check_launch("mz_gated_ff_fwd");
 }
 
@@ -390,6 +406,8 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   MZ_REQUIRE(workspace && workspace_bytes >= need && (size_t)workspace % 16 == 0,
              "mz_gated_ff_bwd: workspace too small (%lld of %lld bytes) or not 16-byte aligned", (long long)workspace_bytes,
              (long long)need);
+  const Split &cut_x = dw_gate ? plan.dx : plan.dx_only, &cut_w = dx ? plan.dw : plan.dw_only;
+  if (int rc = check_tiles("mz_gated_ff_bwd", plan.gate_tile >= 0 && (!dx || cut_x.groups) && (!dw_gate || cut_w.groups))) return rc;
   hipStream_t s = mz::as_stream(stream);
   char* dg = static_cast<char*>(workspace);
   char* du = dg + plan.dgu_bytes;
@@ -414,7 +432,6 @@ int mz_gated_ff_bwd(const void* x, int64_t ldx, const void* w_gate, const void* 
   a.splits = 1;
   a.steps_per_split = (int)sh.steps(a.nk);
   if (int rc = launch(a, dtype, mz_gff::kGateGrad, plan.gate_tile, s)) return rc;
-  const Split &cut_x = dw_gate ? plan.dx : plan.dx_only, &cut_w = dx ? plan.dw : plan.dw_only;
   Args p = {}, q = {};                             // dx; dw
   p.r[0] = w_gate; p.r[1] = w_up;
   p.c[0] = dg; p.c[1] = du; p.c[2] = a.out[2]; p.c[3] = a.out[3];

@@ -6,7 +6,7 @@ import ctypes as C
 import pytest
 import torch
 
-from tests.test_blocks_gpu import TYPES, Canary, check_gated_ff, ff_inputs, ff_run
+from tests.test_blocks_gpu import TYPES, U, Canary, check_gated_ff, ff_inputs, ff_run, half, within
 
 MZ = {"f32": 0, "bf16": 1, "f16": 2}
 
@@ -94,6 +94,24 @@ def test_shared_launches_have_to_win_clearly_against_the_largest_tiles():
         assert plan_of(rows, k, f, "bf16")["together"] == together
 
 
+def test_launches_stay_within_what_hip_can_count():
+    """Threads of a launch are counted in 32 bits: 2^24 workgroups of 64 x 64 tiles are one too many, larger tiles take over; what
+    no tile is large enough for is refused before anything is launched."""
+    from muzero_amd import _lib
+    assert plan_of(1 << 29, 1, 1, "bf16")["dx"] == 64 and plan_of((1 << 30) + 37, 1, 1, "bf16")["dx"] > 64
+    assert plan_of(2 * 10 ** 9, 8, 8, "f32")["dx"] == 128 and plan_of(2 * 10 ** 9, 8, 8, "bf16")["dx"] > 64
+    one = C.c_void_p(16)
+    for rows, k, f, dt in ((1 << 33, 8, 8, 0), (1 << 34, 8, 8, 1), (1 << 36, 1 << 20, 1 << 20, 1)):
+        for want in ((1, 0), (1, 1)):
+            with pytest.raises(_lib.MuZeroAmdError, match="too many output tiles"):
+                _lib.call("mz_gated_ff_plan", rows, k, f, dt, *want, (C.c_int32 * 8)())
+        need = _lib.lib().mz_gated_ff_workspace_bytes(rows, k, f, dt, 1)
+        with pytest.raises(_lib.MuZeroAmdError, match="mz_gated_ff_bwd.*too many output tiles"):
+            _lib.call("mz_gated_ff_bwd", one, k, one, one, None, None, one, rows, k, f, dt, 0, one, None, None, None, None, one, need, None)
+    with pytest.raises(_lib.MuZeroAmdError, match="mz_gated_ff_fwd.*too many output tiles"):
+        _lib.call("mz_gated_ff_fwd", one, 8, one, one, None, None, 1 << 36, 8, 1 << 20, 1, 0, one, None, 0, None)
+
+
 def test_plan_refuses():
     from muzero_amd import _lib
     p = (C.c_int32 * 8)()
@@ -170,3 +188,32 @@ def test_a_gradient_alone_against_float64(rows, k, f, t, which, want):
     for c, v in zip(out, grads):
         c.check(which)
         assert torch.equal(c.inner, v.reshape(-1))
+
+
+@pytest.mark.gpu
+def test_more_rows_than_the_smallest_tiles_can_number():
+    """2^30 + 37 rows of one column: the last rows' results are a small call's, the gradient of the weight is theirs."""
+    from muzero_amd import blocks
+    t, rows, live = torch.bfloat16, (1 << 30) + 37, 37
+    assert plan_of(rows, 1, 1, "bf16")["dx"] > 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tail = torch.randn(live, 1, generator=g, device="cuda").to(t)
+    x = torch.zeros(rows, 1, dtype=t, device="cuda")
+    x[-live:] = tail
+    wg, wu = (torch.randn(1, 1, generator=g, device="cuda").to(t).requires_grad_() for _ in range(2))
+    dh = torch.zeros(rows, 1, dtype=t, device="cuda")
+    dh[-live:] = 1.0
+    x.requires_grad_()
+    h = blocks.gated_ff(x, wg, wu)
+    dx, dwg, dwu = torch.autograd.grad(h, (x, wg, wu), dh)
+    assert torch.equal(h[-live:], blocks.gated_ff(tail, wg, wu)) and not h[:-live].any() and not dx[:-live].any()
+    xd, gd, ud = tail.double(), wg.detach().double(), wu.detach().double()
+    gate, up = xd @ gd.t(), xd @ ud.t()
+    sig = torch.sigmoid(gate)
+    dg, du = up * sig * (1 + gate * (1 - sig)), gate * sig
+    # dg and du: off by their rounding, and by some 32 u of the activation's arithmetic (|gate| stays below 8)
+    off = (half(t) + 32 * U) * 1.01
+    e_dg, e_du = off * dg.abs() + 32 * U * up.abs() * (1 + gate.abs()), off * du.abs()
+    within(dx[-live:], dg @ gd + du @ ud, e_dg @ gd.abs() + e_du @ ud.abs(), "dx")
+    within(dwg, dg.t() @ xd, (e_dg + 40 * U * dg.abs()).t() @ xd.abs(), "dw_gate")
+    within(dwu, du.t() @ xd, (e_du + 40 * U * du.abs()).t() @ xd.abs(), "dw_up")
