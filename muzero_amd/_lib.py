@@ -163,13 +163,8 @@ def call(name, *args):
     """Call an int-returning entry point and turn a negative code into an exception."""
     rc = getattr(lib(), name)(*args)
     if rc != 0:
-        fail(name, rc)
-
-
-def fail(name, rc):
-    """Raise the library's message for entry point `name`, which has returned `rc`."""
-    msg = lib().mz_last_error().decode(errors="replace")
-    raise MuZeroAmdError(f"{name} failed ({rc}): {msg}")
+        msg = lib().mz_last_error().decode(errors="replace")
+        raise MuZeroAmdError(f"{name} failed ({rc}): {msg}")
 
 
 def expect(t, name, dtype=None, shape=None, cuda=True, contiguous=True):
