@@ -200,3 +200,39 @@ def test_gated_ff_gradients_are_off_by_one_rounding_or_two(rows, k, f, carried, 
         off = ((v.double() - ref).norm() / ref.norm()).item()
         if v.numel() >= 10000:
             assert off <= 1.1 * one * (1 if carried else 2 ** 0.5), (name, off, one)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("rows", [3, 40])
+@pytest.mark.parametrize("activation", ["silu", "gelu", "sigmoid"])
+def test_gated_ff_activations_keep_their_digits_far_from_zero(activation, rows, t):
+    """Gates that are given exactly (one column of ones): activation and slope relative to their own size, however small.
+    Room: an exponential of g is off by u |g|, as g log2(e) is rounded.  Of g^2 / 2: erfc takes z = g sqrt(1/2), off by u for the
+    constant and u for the product, so z^2 = g^2 / 2 by 4 u, and its exponential by 4 u times that.  24 u for the functions
+    and products themselves; 16-bit types the hardware's exponential, 4 u of its argument more."""
+    from muzero_amd import blocks
+    t = TYPES[t]
+    reach = {"silu": 80.0, "sigmoid": 80.0, "gelu": 12.0}[activation]
+    if t == torch.float16:                           # results in float16's normal range
+        reach = {"silu": 10.0, "sigmoid": 9.0, "gelu": 3.8}[activation]
+    gate = torch.linspace(-reach, reach, 1001, device="cuda").to(t)
+    f = gate.numel()
+    x = torch.ones(rows, 1, dtype=t, device="cuda")
+    wg, wu = gate[:, None].clone().requires_grad_(), torch.ones(f, 1, dtype=t, device="cuda").requires_grad_()
+    h = blocks.gated_ff(x, wg, wu, activation=activation)
+    dh = torch.zeros(rows, f, dtype=t, device="cuda")
+    dh[1] = 1.0
+    dwg, dwu = torch.autograd.grad(h, (wg, wu), dh)     # one row: act'(g) and act(g) themselves
+    g = gate.double()
+    sig, small = torch.sigmoid(g), torch.sigmoid(-g)
+    cdf = 0.5 * torch.special.erfc(-g * 0.5 ** 0.5)
+    density = torch.exp(-0.5 * g * g) / (2 * math.pi) ** 0.5
+    act, slope, size = {"silu": (g * sig, sig * (1 + g * small), sig * (1 + g.abs() * small)), "sigmoid": (sig, sig * small, sig * small),
+                        "gelu": (g * cdf, cdf + g * density, cdf + g.abs() * density)}[activation]
+    power = g * g / 2 if activation == "gelu" else g.abs()
+    rel = (24 + (4 if activation == "gelu" else 2) * power + (0 if t == torch.float32 else 4 * power)) * U
+    within(h.detach(), act.expand(rows, f), (rel * act.abs()).expand(rows, f), "h")
+    # rounded to the type on the way, 3 rows with the remainder carried, 40 without
+    again = 0.0 if t == torch.float32 else half(t) if rows * f > 8192 else half(t) ** 2
+    within(dwu[:, 0], act, (rel + again) * act.abs() + tiny(t), "dw_up")
+    within(dwg[:, 0], slope, rel * size + again * slope.abs() + tiny(t), "dw_gate")
