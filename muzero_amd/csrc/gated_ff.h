@@ -15,14 +15,15 @@
 // a buffer descriptor that returns zeros for what lies outside the matrix (ragged edges cost a compare, no branch).
 // One barrier a step.
 //
-// What bounds it (MI355X): a step of the 256 x 256 tile keeps the matrix cores and LDS busy for 2048 cycles each (64
-// matrix instructions of 16 cycles a wavefront, two wavefronts a SIMD; 192 KB read and 64 KB staged at 128 bytes a cycle)
-// and takes 1.4 us, 3000 cycles or so at the clock the chip holds there; the 128 x 128 tile moves half as much again
-// through LDS an operation.  8192 x 2048 x 8192 bf16: forward 426 us, input gradient 422, weight gradient 429 (1.28 to 1.30
-// PFLOP/s), gate gradient 488 (1.13); the library's plain product of that size 452 (1.22).  18432 x 256 x 1024 bf16, where
-// a tile has four steps: forward 31 us, gate gradient 43 (113 MB of dh, dg and du), input gradient 28 - 288 tiles on 256
-// compute units - and weight gradient 27, the two in one launch 48.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the
-// 151 TFLOP/s of a large product.
+// What bounds it (MI355X): a step of the 256 x 256 tile is 2048 cycles of the matrix cores (64 matrix instructions of 16 cycles a
+// wavefront, two wavefronts a SIMD) and about 1300 of LDS (192 KB read at 256 bytes a cycle, 64 KB staged at 128), and takes
+// 3000 or so.  By the counters (profiles/blocks_kernels.txt) matrix cores are busy for 61 to 68 % of it and LDS for 40 to 44 %:
+// neither is full, wavefronts wait 40 to 44 % of their time, 7 to 12 % for LDS, the rest at the barrier and for their turn at
+// the matrix cores.  The 128 x 128 tile moves half as much again through LDS an operation.  8192 x 2048 x 8192 bf16: forward
+// 424 us, input gradient 432, weight gradient 456 (1.21 to 1.30 PFLOP/s), gate gradient 484 (1.14); the library's plain product
+// of that size 452 (1.22).  18432 x 256 x 1024 bf16, where a tile has four steps: forward 30 us, gate gradient 44 (113 MB of dh,
+// dg and du; matrix cores 22 %, LDS 36 %, of it a fifth bank conflicts of the epilogue), input and weight gradient in one launch
+// 49.  float32: 18432 x 256 x 1024 forward 160 us, 121 of the 151 TFLOP/s of a large product.
 #pragma once
 #include "block_common.h"
 
@@ -459,8 +460,8 @@ __device__ __forceinline__ void gff_gemm(Args a, unsigned block, unsigned blocks
       load_unit(second, u);
     }
     __syncthreads();
-    // a pair product's sums start at the biases in the 16-bit types: two additions less for every output of the epilogue
-    // (18432 x 256 x 1024 bf16: 27.8 us, added there 29.7).  Each of the sum's additions, one for 32 values of k, then loses up to 2^-24
+    // a pair product's sums start at the biases in the 16-bit types: two additions less for every output of the epilogue, 1.9 us
+    // of the 18432 x 256 x 1024 bf16 forward pass.  Each of the sum's additions, one for 32 values of k, then loses up to 2^-24
     // of the bias: 2^-14 of it at K = 2^15, an eighth of float16's half step, so that longer sums add it last, and so does
     // float32, which keeps those digits.
     const bool bias_now = kBiasFirst && a.nk_all <= kBiasFirstK;

@@ -18,7 +18,7 @@
 //
 // Measured on an MI355X, forward / backward with both launches: 65536 x 4096 bf16 204 / 330 us (5.3 and 4.9 TB/s; a copy
 // of 2 GiB runs at 5.0), 4000 x 16384 float32 98 / 167 us, 18432 x 256 bf16 5.7 / 11.7 us, 4097 x 1001 float32 9.4 / 18.3 us,
-// 1000 x 256 bf16 4.1 / 7.1 us: the smaller ones live in the Infinity Cache and are bound by the launches' own time - a third of
+// 1000 x 256 bf16 2.6 / 5.5 us: the smaller ones live in the Infinity Cache and are bound by the launches' own time - a third of
 // the backward's is the second launch, a few workgroups that add up what up to 768 have left.  Rows wider than registers: 2000 x
 // 32768 bf16 256 / 324 us.  What t costs: nothing at 65536 x 4096, 0.8 us of 8.6 in the forward pass of 4097 x 1001, and where
 // wide rows' parameters alone want gradients a pass over x (2000 x 32768: 53 us without, 92).
