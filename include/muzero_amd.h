@@ -596,8 +596,9 @@ int mz_layer_norm_bwd(const void* x, int64_t ldx, const void* dy, int64_t lddy, 
 /* Gated feed-forward projection in one kernel: h = act(x w_gate^T + b_gate) * (x w_up^T + b_up).  x: [M] rows of K
  * elements, ldx apart; w_gate, w_up: [F][K]; b_gate, b_up: [F] or NULL; h: [M][F]; all of `dtype`, float32
  * accumulation.  activation: 0 SiLU, 1 GELU (erf), 2 ReLU, 3 sigmoid.  M up to 2^36, K and F up to 2^20, and no more output
- * tiles than a launch can number: M x K of dx up to 2^23 tiles of 256 x 256 (float32: 2^24 of 128 x 128); rows of x up to 4 MiB apart.  No alignment beyond the elements' is needed.  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which may
- * be 0 (then NULL will do).
+ * tiles than a launch can number (M x K of dx: up to 2^23 tiles of 256 x 256, float32 2^24 of 128 x 128); rows of x up to 4
+ * MiB apart.  No alignment beyond the elements' is needed.  workspace: mz_gated_ff_workspace_bytes(M, K, F, dtype, 0) bytes, which
+ * is 0, the forward pass needs none (NULL will do).
  * Backward: recomputes both products; dh [M][F] -> dx [M][K], dw_gate / dw_up [F][K] (both or neither), db_gate / db_up
  * [F]; NULL for what is not wanted.  The gradients of the two products are rounded to `dtype` between the launches
  * (16-bit types with M F <= 8192 and K F <= 2^21 carry what that rounding left in a second term).

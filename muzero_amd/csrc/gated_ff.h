@@ -778,13 +778,12 @@ __global__ __launch_bounds__(WR * WC * 64, min_waves(S)) void gff_both_kernel(Ar
   else gff_gemm<T, mz_gff::kWeightGrad, S, S, WR, WC, kAnyActivation>(w, w_first ? blockIdx.x : blockIdx.x - blocks_x, blocks_w, lds);
 }
 
-// workgroups of a product in S x S tiles, a multiple of the 8 XCDs: one a tile, or for pair products what the chip holds;
-// -1 where the tiles are too many to number
+// workgroups of a product in S x S tiles, a multiple of the 8 XCDs: one a tile, or for pair products what the chip holds (that a
+// launch can have them is the choice of the tile's to see to: max_groups in gated_ff.hip)
 template <int MODE, int S> long gemm_blocks(const Args& a) {
   constexpr bool kPair = MODE <= mz_gff::kGateGrad;
   constexpr int TR = kPair ? S / 2 : S;
   const long total = ((a.nr + TR - 1) / TR) * ((a.nc + S - 1) / S) * (MODE == mz_gff::kWeightGrad ? 2 : 1) * a.splits;
-  if (total > 0x3ffffff0l) return -1;
   const long held = (long)mz::compute_units() / 8 * 8 * (S == 256 ? 1 : S == 128 ? 2 : 4), blocks = (total + 7) / 8 * 8;
   return kPair && S != 256 && blocks > held ? held : blocks;
 }
@@ -795,7 +794,6 @@ template <typename T, int MODE, int S, int WR, int WC, int ACT> int launch_kerne
   const auto kernel = gff_gemm_kernel<T, MODE, S, WR, WC, ACT>;
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
   const long blocks = gemm_blocks<MODE, S>(a);
-  if (blocks < 0) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(WR * WC * 64), kLds, s, a);
   return MZ_OK;
 }
@@ -833,7 +831,6 @@ template <typename T, int S> int launch_both_in(const Args& x, const Args& w, hi
   const auto kernel = gff_both_kernel<T, S, 2, 2>;
   if (int rc = mz::ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), kLds, done, "mz_gated_ff")) return rc;
   const long bx = gemm_blocks<mz_gff::kInputGrad, S>(x), bw = gemm_blocks<mz_gff::kWeightGrad, S>(w);
-  if (bx < 0 || bw < 0) return mz::fail(MZ_E_ARG, "mz_gated_ff: too many tiles");
   hipLaunchKernelGGL(kernel, dim3((unsigned)(bx + bw)), dim3(256), kLds, s, x, w, (unsigned)bx, (unsigned)bw,
                      w.steps_per_split > x.steps_per_split ? 1 : 0);
   return MZ_OK;

@@ -154,7 +154,7 @@ const TileCost& cost_of(int dtype, int tile) { return (dtype == MZ_F32 ? kCost32
 float join_time(int64_t elements, int splits) { return splits > 1 ? (float)elements * splits * 8.f / 8e6f : 0.f; }
 
 // Workgroups that a launch can have: HIP counts its threads in 32 bits (16 less, for rounding up to all XCDs).  The pair products'
-// workgroups in the smaller tiles are as many as the chip holds, what counts there is the numbering of the tiles (gemm_blocks).
+// workgroups in the smaller tiles are as many as the chip holds; their tiles are numbered in 32 bits.
 int64_t max_groups(int tile, bool pair) { return pair && tile != 0 ? 0x3ffffff0ll : (1ll << 32) / (tile == 0 ? 512 : 256) - 16; }
 
 // f(the product of nr x nc results, `problems` of them, in `tile` with its sum cut into 1, 2, 3 .. parts)
